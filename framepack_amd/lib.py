@@ -31,6 +31,18 @@ SIGNATURES = {
     "fp_layernorm_modulate_bf16": [P, L, P, P, P, L, I, I, F, P],
     "fp_layernorm_affine_bf16": [P, L, P, P, P, L, I, I, F, P],
     "fp_gate_residual_bf16": [P, L, P, L, P, I, I, P],
+    "fp_rmsnorm_residual_bf16": [P, L, P, L, P, P, L, P, L, I, I, F, P],
+    "fp_rmsnorm_residual_f16": [P, L, P, L, P, P, L, P, L, I, I, F, P],
+    "fp_rmsnorm_residual_fp8": [P, L, P, L, P, P, L, P, P, L, I, I, F, P],
+    "fp_rmsnorm_residual_backward_workspace_bytes": [I, I],
+    "fp_rmsnorm_residual_backward_bf16": [P, L, P, L, P, L, P, P, L, P, I, I, F, P, L, P],
+    "fp_rmsnorm_residual_backward_f16": [P, L, P, L, P, L, P, P, L, P, I, I, F, P, L, P],
+    "fp_gated_ff_bf16": [P, L, P, L, P, L, P, P, P, L, P, P, L, I, I, I, I, P],
+    "fp_gated_ff_f16": [P, L, P, L, P, L, P, P, P, L, P, P, L, I, I, I, I, P],
+    "fp_gated_ff_fp8": [P, L, P, P, L, P, P, L, P, P, P, P, L, I, I, I, I, P],
+    "fp_gated_ff_backward_workspace_bytes": [I, I, I],
+    "fp_gated_ff_backward_bf16": [P, L, P, L, P, L, P, L, P, L, P, L, P, L, P, P, L, P, P, I, I, I, I, P, L, P],
+    "fp_gated_ff_backward_f16": [P, L, P, L, P, L, P, L, P, L, P, L, P, L, P, P, L, P, P, I, I, I, I, P, L, P],
     "fp_silu_gemv_bf16": [P, P, P, P, I, I, I, P],
     "fp_rel_l1_acc_floats": [],
     "fp_rel_l1_bf16": [P, P, L, P, P],

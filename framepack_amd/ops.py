@@ -674,3 +674,246 @@ def attention_framecausal(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, q_
             p = softmax_framecausal_f32_(logits, r0, q_per_frame, k_per_frame, scale)
             gemm(p, vt[:, :n], None, out=out[r0:r1])
     return out
+
+
+# ---- K12, K13: a language model's pre-norm and gated feed-forward block, forward, in 8 bits, and backward ---------------
+
+ACT_SILU, ACT_GELU = 0, 1          # GELU: the tanh form, as in EPI_GELU
+
+
+def _mat(t: torch.Tensor, what: str, dtypes, shape=None):
+    """(tensor, rows, cols, row stride) of a matrix argument of K12 / K13: [.., rows, cols] as `_rows2d` takes it, of one
+    of `dtypes`, and of `shape` if given.  A single row's stride says nothing and is replaced by the row's length."""
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.dim() < 2:
+        raise ValueError(f"{what}: expected a [rows, cols] tensor, got {tuple(t.shape)}")
+    if t.dim() > 2:
+        t = t.reshape(-1, t.shape[-1]) if t.is_contiguous() else t.squeeze(0)
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{what}: expected a [rows, cols] tensor with unit inner stride, got {tuple(t.shape)} / {t.stride()}")
+    rows, cols = t.shape
+    if cols == 0 or (shape is not None and (rows, cols) != tuple(shape)):
+        raise ValueError(f"{what}: expected {'at least one column' if shape is None else list(shape)}, got {[rows, cols]}")
+    return t, rows, cols, (t.stride(0) if rows > 1 else (cols + 15) // 16 * 16)
+
+
+def _vec(t: torch.Tensor, what: str, dtype, n: int) -> torch.Tensor:
+    """A vector argument of n values; made contiguous where it is not."""
+    if t.dtype != dtype or t.numel() != n:
+        raise ValueError(f"{what}: expected {n} values of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    return t.reshape(-1).contiguous()
+
+
+def _out(t: Optional[torch.Tensor], what: str, dtype, rows: int, cols: int, device):
+    """An output matrix: allocated if None, else of this type and size with rows that do not overlap each other."""
+    if t is None:
+        t = torch.empty((rows, cols), dtype=dtype, device=device)
+    t2, _, _, rs = _mat(t, what, (dtype,), (rows, cols))
+    if rs < cols:
+        raise ValueError(f"{what}: rows of {cols} values overlap at a row stride of {rs}")
+    return t, t2, rs
+
+
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices have bytes in common (taken as such where the row strides differ and the ranges meet)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    ea, eb = a.element_size(), b.element_size()
+    ra, rb = a.shape[0], b.shape[0]
+    wa, wb = a.shape[1] * ea, b.shape[1] * eb
+    sa, sb = a.stride(0) * ea, b.stride(0) * eb
+    sa, sb = sa if ra > 1 else sb, sb if rb > 1 else sa                # (a single row has any stride)
+    d = b.data_ptr() - a.data_ptr()
+    if not -((rb - 1) * sb + wb) < d < (ra - 1) * sa + wa:
+        return False
+    if (ra > 1 or rb > 1) and sa == sb and wa <= sa and wb <= sb:
+        q, r = divmod(d, sa)                   # b's row j begins r bytes into a's row j + q
+        return (r < wa and -rb < q < ra) or (r + wb > sa and -rb < q + 1 < ra)
+    return True
+
+
+def _apart(outs, ins, same=()) -> None:
+    """Refuses outputs that share memory with each other or with an input; `same`: pairs (output, input) that may be one
+    and the same matrix (read before it is written), but not overlap in any other way."""
+    for i, (na, a) in enumerate(outs):
+        for nb, b in outs[i + 1:]:
+            if _share(a, b):
+                raise ValueError(f"{na} and {nb} share memory")
+        for nb, b in ins:
+            if b is None or not _share(a, b):
+                continue
+            if (na, nb) in same and a.data_ptr() == b.data_ptr() and (a.shape[0] <= 1 or a.stride(0) == b.stride(0)):
+                continue
+            raise ValueError(f"{na} shares memory with {nb}")
+
+
+def _rmsnorm_args(x, weight, resid, resid_out, dtypes, eps):
+    _dev(x, weight, resid, resid_out)
+    x2, rows, cols, xs = _mat(x, "x", dtypes)
+    w = _vec(weight, "weight", x.dtype, cols)
+    if not eps >= 0:
+        raise ValueError(f"eps: expected a number of at least 0, got {eps}")
+    if resid is None:
+        if resid_out is not None:
+            raise ValueError("resid_out without resid")
+        return x2, rows, cols, xs, w, None, 0, x, None, 0
+    r2, _, _, rs = _mat(resid, "resid", (x.dtype,), (rows, cols))
+    h, h2, hs = _out(resid_out, "resid_out", x.dtype, rows, cols, x.device)
+    return x2, rows, cols, xs, w, r2, rs, h, h2, hs
+
+
+def rmsnorm_residual(x: torch.Tensor, weight: torch.Tensor, resid: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                     out: Optional[torch.Tensor] = None, resid_out: Optional[torch.Tensor] = None):
+    """K12: h = resid + x, out = h / sqrt(mean(h^2) + eps) * weight; returns (out, h).  Without resid, h is x itself.
+    x, resid [rows, cols] (row-strided ok, any cols), weight [cols], one type: bf16 or f16.  The norm is taken of the
+    32-bit sum; h is that sum rounded to the type.  out and resid_out may each be x or resid itself."""
+    x2, rows, cols, xs, w, r2, rs, h, h2, hs = _rmsnorm_args(x, weight, resid, resid_out, (BF16, F16), eps)
+    _dev(out)
+    out, o2, os_ = _out(out, "out", x.dtype, rows, cols, x.device)
+    outs = [("out", o2)] + ([] if h2 is None else [("resid_out", h2)])
+    _apart(outs, [("x", x2), ("resid", r2), ("weight", w[None])],
+           {(o, i) for o in ("out", "resid_out") for i in ("x", "resid")})
+    if rows == 0:
+        return out, h
+    name = "fp_rmsnorm_residual_bf16" if x.dtype == BF16 else "fp_rmsnorm_residual_f16"
+    _lib.check(getattr(_lib.load(), name)(x2.data_ptr(), xs, _ptr(r2), rs, w.data_ptr(), o2.data_ptr(), os_, _ptr(h2), hs,
+                                          rows, cols, eps, _stream(x)), name)
+    return out, h
+
+
+def rmsnorm_residual_fp8(x: torch.Tensor, weight: torch.Tensor, resid: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                         out: Optional[torch.Tensor] = None, out_scale: Optional[torch.Tensor] = None,
+                         resid_out: Optional[torch.Tensor] = None):
+    """K12 into 8 bits: (q e4m3 [rows, cols], scale fp32 [rows], h) with out of `rmsnorm_residual` ~ scale * q, the A
+    operand of `gated_ff_fp8` and `gemm_fp8`.  scale = max|row| / 448 (1 for a row of zeros); q is rounded once, from 32
+    bits.  bf16 only."""
+    x2, rows, cols, xs, w, r2, rs, h, h2, hs = _rmsnorm_args(x, weight, resid, resid_out, (BF16,), eps)
+    _dev(out, out_scale)
+    out, o2, os_ = _out(out, "out", FP8, rows, cols, x.device)
+    if out_scale is None:
+        out_scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    if out_scale.dtype != torch.float32 or out_scale.numel() != rows or not out_scale.is_contiguous():
+        raise ValueError(f"out_scale: expected {rows} contiguous float32 values")
+    outs = [("out", o2), ("out_scale", out_scale.reshape(1, -1))] + ([] if h2 is None else [("resid_out", h2)])
+    _apart(outs, [("x", x2), ("resid", r2), ("weight", w[None])], {("resid_out", "x"), ("resid_out", "resid")})
+    if rows == 0:
+        return out, out_scale, h
+    _lib.check(_lib.load().fp_rmsnorm_residual_fp8(x2.data_ptr(), xs, _ptr(r2), rs, w.data_ptr(), o2.data_ptr(), os_,
+                                                   out_scale.data_ptr(), _ptr(h2), hs, rows, cols, eps, _stream(x)),
+               "fp_rmsnorm_residual_fp8")
+    return out, out_scale, h
+
+
+def rmsnorm_residual_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, dh: Optional[torch.Tensor] = None,
+                              eps: float = 1e-6, dx: Optional[torch.Tensor] = None):
+    """Gradient of K12: (dx, dweight) from dy (of out), h as `rmsnorm_residual` returned it and dh, the gradient that
+    reaches h by its other uses (None: none).  dx is the gradient of x and of resid alike; dx may be dh itself.
+    All [rows, cols] of one type, bf16 or f16; dweight [cols] of weight's type, summed in 32 bits in a fixed order."""
+    _dev(dy, h, weight, dh, dx)
+    h2, rows, cols, hs = _mat(h, "h", (BF16, F16))
+    y2, _, _, ys = _mat(dy, "dy", (h.dtype,), (rows, cols))
+    w = _vec(weight, "weight", h.dtype, cols)
+    if not eps >= 0:
+        raise ValueError(f"eps: expected a number of at least 0, got {eps}")
+    d2, ds = None, 0
+    if dh is not None:
+        d2, _, _, ds = _mat(dh, "dh", (h.dtype,), (rows, cols))
+    dx, dx2, dxs = _out(dx, "dx", h.dtype, rows, cols, h.device)
+    _apart([("dx", dx2)], [("dy", y2), ("h", h2), ("dh", d2), ("weight", w[None])], {("dx", "dh")})
+    if rows == 0:
+        return dx, torch.zeros((cols,), dtype=h.dtype, device=h.device)
+    dw = torch.empty((cols,), dtype=h.dtype, device=h.device)
+    lib = _lib.load()
+    # (per call: the caching allocator keeps it apart from other streams' and other captured graphs' calls)
+    ws = torch.empty((lib.fp_rmsnorm_residual_backward_workspace_bytes(rows, cols),), dtype=torch.uint8, device=h.device)
+    name = "fp_rmsnorm_residual_backward_bf16" if h.dtype == BF16 else "fp_rmsnorm_residual_backward_f16"
+    _lib.check(getattr(lib, name)(y2.data_ptr(), ys, h2.data_ptr(), hs, _ptr(d2), ds, w.data_ptr(), dx2.data_ptr(), dxs,
+                                  dw.data_ptr(), rows, cols, eps, ws.data_ptr(), ws.numel(), _stream(h)), name)
+    return dx, dw
+
+
+def _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, dtypes, bias_dtype):
+    x2, M, K, ldx = _mat(x, "x", dtypes)
+    g2, F, _, ldg = _mat(w_gate, "w_gate", (x.dtype,))
+    if g2.shape[1] != K:
+        raise ValueError(f"w_gate: expected [inner, {K}], got {list(g2.shape)}")
+    u2, _, _, ldu = _mat(w_up, "w_up", (x.dtype,), (F, K))
+    if F == 0:
+        raise ValueError("w_gate: expected at least one row")
+    if act not in (ACT_SILU, ACT_GELU):
+        raise ValueError(f"act: expected ACT_SILU or ACT_GELU, got {act!r}")
+    if (b_gate is None) != (b_up is None):
+        raise ValueError("b_gate and b_up: both or neither")
+    if b_gate is not None:
+        b_gate, b_up = _vec(b_gate, "b_gate", bias_dtype, F), _vec(b_up, "b_up", bias_dtype, F)
+    return x2, M, K, ldx, g2, F, ldg, u2, ldu, b_gate, b_up
+
+
+def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
+             b_up: Optional[torch.Tensor] = None, act: int = ACT_SILU, out: Optional[torch.Tensor] = None, keep: bool = False):
+    """K13: h = act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up) in one kernel, act = ACT_SILU or ACT_GELU; returns h
+    [M, inner], with keep (h, gate, up): the two projections before the activation, as `gated_ff_backward` takes them.
+    x [M, K], w_gate, w_up [inner, K] (nn.Linear layout; row-strided ok, slices of one fused weight too), any sizes; one
+    type, bf16 or f16.  The block's second linear is `gemm`, with the residual in its epilogue (EPI_RESIDUAL)."""
+    _dev(x, w_gate, w_up, b_gate, b_up, out)
+    x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, (BF16, F16), x.dtype)
+    out, o2, ldo = _out(out, "out", x.dtype, M, F, x.device)
+    _apart([("out", o2)], [("x", x2), ("w_gate", g2), ("w_up", u2), ("b_gate", None if bg is None else bg[None]),
+                           ("b_up", None if bu is None else bu[None])])
+    gate = torch.empty((M, F), dtype=x.dtype, device=x.device) if keep else None
+    up = torch.empty((M, F), dtype=x.dtype, device=x.device) if keep else None
+    if M > 0:
+        name = "fp_gated_ff_bf16" if x.dtype == BF16 else "fp_gated_ff_f16"
+        _lib.check(getattr(_lib.load(), name)(x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, _ptr(bg), _ptr(bu),
+                                              o2.data_ptr(), ldo, _ptr(gate), _ptr(up), F, M, F, K, act, _stream(x)), name)
+    return (out, gate, up) if keep else out
+
+
+def gated_ff_fp8(x_q: torch.Tensor, x_scale: torch.Tensor, wg_q: torch.Tensor, wg_scale: torch.Tensor, wu_q: torch.Tensor,
+                 wu_scale: torch.Tensor, b_gate: Optional[torch.Tensor] = None, b_up: Optional[torch.Tensor] = None,
+                 act: int = ACT_SILU, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """K13 on e4m3 operands: bf16 h = act(g) * u with g = x_scale[m] * wg_scale[n] * (x_q @ wg_q.T) + b_gate and u alike.
+    x_q [M, K] with x_scale [M] as `rmsnorm_residual_fp8` and `quantize_rows_fp8` return them, weights [inner, K] with
+    scales [inner] as `quantize_weight_fp8` prepares them; biases bf16.  K a multiple of 128, inner of 8, matrices 16-byte
+    aligned with row strides of multiples of 16, as `gemm_fp8`."""
+    _dev(x_q, x_scale, wg_q, wg_scale, wu_q, wu_scale, b_gate, b_up, out)
+    x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x_q, wg_q, wu_q, b_gate, b_up, act, (FP8,), BF16)
+    xs, gs, us = (_vec(t, n, torch.float32, k) for t, n, k in ((x_scale, "x_scale", M), (wg_scale, "wg_scale", F),
+                                                              (wu_scale, "wu_scale", F)))
+    out, o2, ldo = _out(out, "out", BF16, M, F, x_q.device)
+    _apart([("out", o2)], [("x_q", x2), ("wg_q", g2), ("wu_q", u2), ("x_scale", xs[None]), ("wg_scale", gs[None]),
+                           ("wu_scale", us[None]), ("b_gate", None if bg is None else bg[None]),
+                           ("b_up", None if bu is None else bu[None])])
+    if M == 0:
+        return out
+    _lib.check(_lib.load().fp_gated_ff_fp8(x2.data_ptr(), ldx, xs.data_ptr(), g2.data_ptr(), ldg, gs.data_ptr(), u2.data_ptr(),
+                                           ldu, us.data_ptr(), _ptr(bg), _ptr(bu), o2.data_ptr(), ldo, M, F, K, act,
+                                           _stream(x_q)), "fp_gated_ff_fp8")
+    return out
+
+
+def gated_ff_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor,
+                      up: torch.Tensor, act: int = ACT_SILU, bias: bool = False):
+    """Gradient of K13: (dx, dw_gate, dw_up, db_gate, db_up) from dh (of h) and the projections that `gated_ff(keep=True)`
+    returned; the biases' are None unless `bias`.  One type throughout, bf16 or f16; the gradients of the projections are
+    rounded to it between the two steps, sums are held in 32 bits and taken in a fixed order.  dw_gate and dw_up are the
+    halves of one [2 * inner, K] tensor (the gradient of a fused weight)."""
+    _dev(dh, x, w_gate, w_up, gate, up)
+    x2, M, K, ldx, g2, F, ldg, u2, ldu, _, _ = _gated_ff_args(x, w_gate, w_up, None, None, act, (BF16, F16), x.dtype)
+    (d2, _, _, ldd), (p2, _, _, ldp), (q2, _, _, ldq) = (_mat(t, n, (x.dtype,), (M, F)) for t, n in ((dh, "dh"), (gate, "gate"),
+                                                                                                    (up, "up")))
+    if M == 0:
+        dw = torch.zeros((2 * F, K), dtype=x.dtype, device=x.device)
+        db = torch.zeros((2, F), dtype=x.dtype, device=x.device) if bias else (None, None)
+        return torch.empty((0, K), dtype=x.dtype, device=x.device), dw[:F], dw[F:], db[0], db[1]
+    dx = torch.empty((M, K), dtype=x.dtype, device=x.device)
+    dw = torch.empty((2 * F, K), dtype=x.dtype, device=x.device)
+    db = torch.empty((2, F), dtype=x.dtype, device=x.device) if bias else (None, None)
+    lib = _lib.load()
+    ws = torch.empty((lib.fp_gated_ff_backward_workspace_bytes(M, F, K),), dtype=torch.uint8, device=x.device)
+    name = "fp_gated_ff_backward_bf16" if x.dtype == BF16 else "fp_gated_ff_backward_f16"
+    _lib.check(getattr(lib, name)(d2.data_ptr(), ldd, x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, p2.data_ptr(),
+                                  ldp, q2.data_ptr(), ldq, dx.data_ptr(), K, dw[:F].data_ptr(), dw[F:].data_ptr(), K,
+                                  _ptr(db[0]), _ptr(db[1]), M, F, K, act, ws.data_ptr(), ws.numel(), _stream(x)), name)
+    return dx, dw[:F], dw[F:], db[0], db[1]

@@ -202,6 +202,73 @@ int fp_gemm_fp8_bf16(const void* a, int64_t lda, const void* a_scale, const void
                      const void* w_scale, const void* bias, void* c, int64_t ldc, int M, int N, int K, int epilogue,
                      int gelu_from, const void* resid, int64_t ldr, const void* gate, void* stream);
 
+/* ---- K12, K13: a language model's pre-norm and gated feed-forward block (no counterpart in the reference) ---------
+ * Pointers need their type's alignment only and strides and sizes are free unless noted; 16-byte aligned pointers with
+ * strides and sizes of multiples of 8 elements take the wide paths.  Input rows may repeat (stride 0); output rows must
+ * not overlap.  `dtype` suffix: the type of every matrix and vector of the call unless noted. */
+
+/* K12  h = resid + x;  y = h / sqrt(mean(h^2) + eps) * weight,  x, resid, y, h: [rows, cols], weight: [cols].
+ * The norm is taken of the 32-bit sum, h receives it rounded.  resid and h may both be NULL: h = x, nothing but y is
+ * written.  y and h may each be the very matrix x or resid (same pointer and stride).  cols is any positive number. */
+int fp_rmsnorm_residual_bf16(const void* x, int64_t x_row_stride, const void* resid, int64_t resid_row_stride,
+                             const void* weight, void* y, int64_t y_row_stride, void* h, int64_t h_row_stride, int rows,
+                             int cols, float eps, void* stream);
+int fp_rmsnorm_residual_f16(const void* x, int64_t x_row_stride, const void* resid, int64_t resid_row_stride,
+                            const void* weight, void* y, int64_t y_row_stride, void* h, int64_t h_row_stride, int rows,
+                            int cols, float eps, void* stream);
+
+/* K12 into 8 bits: x, resid, weight, h bf16 as above, q: e4m3 [rows, cols] (row stride ldq bytes) and q_scale: fp32
+ * [rows] with y ~ q_scale * q, q_scale = max|y| / 448 (1 for a row of zeros): the A operand of fp_gemm_fp8_bf16 and
+ * fp_gated_ff_fp8.  q is rounded once, from the 32-bit y.  A NaN is left out of the row's maximum and stays a NaN. */
+int fp_rmsnorm_residual_fp8(const void* x, int64_t x_row_stride, const void* resid, int64_t resid_row_stride,
+                            const void* weight, void* q, int64_t ldq, void* q_scale, void* h, int64_t h_row_stride,
+                            int rows, int cols, float eps, void* stream);
+
+/* Gradient of K12, with r = 1 / sqrt(mean(h^2) + eps), n = h r, dn = dy weight:
+ *   dx = dh + r (dn - n mean(dn n)) (the gradient of x and of resid);  dweight = sum over rows of dy n.
+ * dh (may be NULL): the gradient that reaches h by its other uses; dx may be the very matrix dh.  rows > 0.  Sums in
+ * fp32 in a fixed order.  workspace: fp_rmsnorm_residual_backward_workspace_bytes(rows, cols) bytes, 16-byte aligned. */
+int64_t fp_rmsnorm_residual_backward_workspace_bytes(int rows, int cols);
+int fp_rmsnorm_residual_backward_bf16(const void* dy, int64_t dy_row_stride, const void* h, int64_t h_row_stride,
+                                      const void* dh, int64_t dh_row_stride, const void* weight, void* dx,
+                                      int64_t dx_row_stride, void* dweight, int rows, int cols, float eps,
+                                      void* workspace, int64_t workspace_bytes, void* stream);
+int fp_rmsnorm_residual_backward_f16(const void* dy, int64_t dy_row_stride, const void* h, int64_t h_row_stride,
+                                     const void* dh, int64_t dh_row_stride, const void* weight, void* dx,
+                                     int64_t dx_row_stride, void* dweight, int rows, int cols, float eps,
+                                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* K13  h = act(g) * u,  g = x . w_gate^T + b_gate,  u = x . w_up^T + b_up;  act: 0 = SiLU, 1 = tanh-GELU.
+ * x: [M, K], w_gate, w_up: [F, K] (nn.Linear layout), biases [F] (both or neither), h: [M, F].  gate, up (both or
+ * neither, row stride ldp): receive g and u for the gradient.  No output may overlap an input. */
+int fp_gated_ff_bf16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
+                     const void* b_gate, const void* b_up, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M,
+                     int F, int K, int act, void* stream);
+int fp_gated_ff_f16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
+                    const void* b_gate, const void* b_up, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M,
+                    int F, int K, int act, void* stream);
+
+/* K13 on e4m3 operands: g = x_scale[m] * wg_scale[n] * (x . w_gate^T) + b_gate and u alike; h and the biases bf16, the
+ * scales fp32.  K % 128 == 0, F % 8 == 0, the matrices 16-byte aligned with row strides of multiples of 16 elements
+ * (h: of 8), scales and biases 16-byte aligned. */
+int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, const void* w_gate, int64_t ldwg, const void* wg_scale,
+                    const void* w_up, int64_t ldwu, const void* wu_scale, const void* b_gate, const void* b_up, void* h,
+                    int64_t ldh, int M, int F, int K, int act, void* stream);
+
+/* Gradient of K13 from dh and the kept g and u:  dg = dh u act'(g), du = dh act(g) (rounded to the type), then
+ *   dx = dg . w_gate + du . w_up [M, K];  dw_gate = dg^T . x, dw_up = du^T . x [F, K] (row stride lddw);
+ *   db_gate, db_up [F] = column sums of dg, du (both or neither NULL).
+ * M > 0.  Sums in fp32 in a fixed order.  workspace: fp_gated_ff_backward_workspace_bytes(M, F, K), 16-byte aligned. */
+int64_t fp_gated_ff_backward_workspace_bytes(int M, int F, int K);
+int fp_gated_ff_backward_bf16(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
+                              const void* w_up, int64_t ldwu, const void* gate, int64_t ldg, const void* up, int64_t ldu,
+                              void* dx, int64_t lddx, void* dw_gate, void* dw_up, int64_t lddw, void* db_gate, void* db_up,
+                              int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
+int fp_gated_ff_backward_f16(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
+                             const void* w_up, int64_t ldwu, const void* gate, int64_t ldg, const void* up, int64_t ldu,
+                             void* dx, int64_t lddx, void* dw_gate, void* dw_up, int64_t lddw, void* db_gate, void* db_up,
+                             int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- K11: causal-3D VAE decode (fp16, channels-last [T, H, W, C] volumes) -------------------------------
  * The reference's code for this path is diffusers_helper/hunyuan.py:93-103 (vae_decode); everything under its
  * `vae.decode(...)` call is diffusers 0.33.1 AutoencoderKLHunyuanVideo (third-party, absent from the reference

@@ -1,0 +1,149 @@
+"""What the entry points of K12 and K13 refuse, on the CPU: the tensor-level checks (the device check aside, everything
+that is refused is refused before the library is called) and the C ABI's (a refused call launches nothing)."""
+import pytest
+import torch
+
+from framepack_amd import lib as fplib
+from framepack_amd import ops
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture
+def no_device_check(monkeypatch):
+    monkeypatch.setattr(ops, "_dev", lambda *ts: None)
+
+    class Lib:
+        def __getattr__(self, name):
+            raise AssertionError("the library was called")
+
+    monkeypatch.setattr(fplib, "load", lambda: Lib())
+
+
+def mats(*shapes, dtype=BF):
+    return [torch.zeros(*s, dtype=dtype) for s in shapes]
+
+
+def test_cpu_tensors_are_refused():
+    x, w, m = torch.zeros(4, 64, dtype=BF), torch.ones(64, dtype=BF), torch.zeros(16, 64, dtype=BF)
+    for call in (lambda: ops.rmsnorm_residual(x, w), lambda: ops.rmsnorm_residual_fp8(x, w), lambda: ops.gated_ff(x, m, m),
+                 lambda: ops.rmsnorm_residual_backward(x, x, w), lambda: ops.gated_ff_backward(m, x, m, m, m, m)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+def test_norm_refusals(no_device_check):
+    x, r, w = torch.zeros(4, 64, dtype=BF), torch.zeros(4, 64, dtype=BF), torch.ones(64, dtype=BF)
+    big = torch.zeros(4, 200, dtype=BF)
+    cases = [
+        (lambda: ops.rmsnorm_residual(x.float(), w), "expected torch.bfloat16 or"),
+        (lambda: ops.rmsnorm_residual(x, w.half()), "weight"),
+        (lambda: ops.rmsnorm_residual(x, w[:32]), "weight"),
+        (lambda: ops.rmsnorm_residual(x, w, r[:3]), "resid"),
+        (lambda: ops.rmsnorm_residual(x, w, r.half()), "resid"),
+        (lambda: ops.rmsnorm_residual(x[0], w), "rows, cols"),
+        (lambda: ops.rmsnorm_residual(x.t(), w), "unit inner stride"),
+        (lambda: ops.rmsnorm_residual(torch.zeros(4, 128, dtype=BF)[:, ::2], w), "unit inner stride"),
+        (lambda: ops.rmsnorm_residual(torch.zeros(4, 0, dtype=BF), w[:0]), "column"),
+        (lambda: ops.rmsnorm_residual(x, w, eps=-1.0), "eps"),
+        (lambda: ops.rmsnorm_residual(x, w, eps=float("nan")), "eps"),
+        (lambda: ops.rmsnorm_residual(x, w, resid_out=r), "without resid"),
+        (lambda: ops.rmsnorm_residual(x, w, r, out=torch.zeros(4, 32, dtype=BF)), "out"),
+        (lambda: ops.rmsnorm_residual(x, w, r, out=x[:1].expand(4, 64)), "overlap"),
+        (lambda: ops.rmsnorm_residual(x, w, r, out=x, resid_out=x), "share memory"),
+        (lambda: ops.rmsnorm_residual(big[:, :64], w, r, out=big[:, 8:72]), "shares memory"),
+        (lambda: ops.rmsnorm_residual(big[:3, :64], w, out=big[1:, :64]), "shares memory"),
+        (lambda: ops.rmsnorm_residual(x, w, out=w[None].expand(4, 64)), "overlap"),
+        (lambda: ops.rmsnorm_residual(x[:1], w, out=w[None]), "shares memory"),
+        (lambda: ops.rmsnorm_residual_fp8(x.half(), w.half()), "x"),
+        (lambda: ops.rmsnorm_residual_fp8(x, w, out=r), "out"),
+        (lambda: ops.rmsnorm_residual_fp8(x, w, out_scale=torch.zeros(3)), "out_scale"),
+        (lambda: ops.rmsnorm_residual_fp8(x, w, out_scale=torch.zeros(8)[::2]), "out_scale"),
+        (lambda: ops.rmsnorm_residual_fp8(x, w, out=x.view(ops.FP8)[:, :64]), "shares memory"),
+        (lambda: ops.rmsnorm_residual_backward(x, r[:3], w), "dy"),
+        (lambda: ops.rmsnorm_residual_backward(x, r, w, dh=r[:, :32]), "dh"),
+        (lambda: ops.rmsnorm_residual_backward(x, r, w, dx=x), "shares memory"),
+        (lambda: ops.rmsnorm_residual_backward(x, r, w, dx=r), "shares memory"),
+        (lambda: ops.rmsnorm_residual_backward(x.half(), r, w), "dy"),
+    ]
+    for call, text in cases:
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_gated_ff_refusals(no_device_check):
+    x, wg, wu, b = torch.zeros(4, 64, dtype=BF), torch.zeros(16, 64, dtype=BF), torch.zeros(16, 64, dtype=BF), torch.zeros(16, dtype=BF)
+    g, u, dh = mats((4, 16), (4, 16), (4, 16))
+    x8, w8, s4, s16 = torch.zeros(4, 128, dtype=ops.FP8), torch.zeros(16, 128, dtype=ops.FP8), torch.ones(4), torch.ones(16)
+    cases = [
+        (lambda: ops.gated_ff(x.float(), wg.float(), wu.float()), "x"),
+        (lambda: ops.gated_ff(x, wg.half(), wu), "w_gate"),
+        (lambda: ops.gated_ff(x, wg, wu[:8]), "w_up"),
+        (lambda: ops.gated_ff(x, wg[:, :32], wu), "w_gate"),
+        (lambda: ops.gated_ff(x, wg[:0], wu[:0]), "row"),
+        (lambda: ops.gated_ff(x, wg.t().contiguous().t(), wu), "unit inner stride"),
+        (lambda: ops.gated_ff(x, wg, wu, b, None), "both or neither"),
+        (lambda: ops.gated_ff(x, wg, wu, b, b[:8]), "b_up"),
+        (lambda: ops.gated_ff(x, wg, wu, b.float(), b.float()), "b_gate"),
+        (lambda: ops.gated_ff(x, wg, wu, act=2), "act"),
+        (lambda: ops.gated_ff(x, wg, wu, out=g[:, :8]), "out"),
+        (lambda: ops.gated_ff(x, wg, wu, out=g[:1].expand(4, 16)), "overlap"),
+        (lambda: ops.gated_ff(x, wg, wu, out=x[:, :16]), "shares memory"),
+        (lambda: ops.gated_ff_fp8(x, s4, wg, s16, wu, s16), "x"),
+        (lambda: ops.gated_ff_fp8(x8, s4[:3], w8, s16, w8, s16), "x_scale"),
+        (lambda: ops.gated_ff_fp8(x8, s4, w8, s16.half(), w8, s16), "wg_scale"),
+        (lambda: ops.gated_ff_fp8(x8, s4, w8, s16, w8, s16, out=g.half()), "out"),
+        (lambda: ops.gated_ff_backward(dh[:3], x, wg, wu, g, u), "dh"),
+        (lambda: ops.gated_ff_backward(dh, x, wg, wu, g, u[:, :8]), "up"),
+        (lambda: ops.gated_ff_backward(dh, x, wg, wu, g.half(), u), "gate"),
+        (lambda: ops.gated_ff_backward(dh, x, wg, wu, g, u, act=None), "act"),
+    ]
+    for call, text in cases:
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_disjoint_columns_and_rows_of_one_buffer_do_not_share():
+    big = torch.zeros(10, 96, dtype=BF)
+    a, b = big[:, :32], big[:, 32:64]
+    assert not ops._share(a, b) and not ops._share(b, a) and not ops._share(big[:5], big[5:])
+    assert ops._share(big[:, :33], b) and ops._share(b, big[:, :33]) and ops._share(big[:6], big[5:]) and ops._share(a, a)
+    assert ops._share(big[1:, 80:], big.view(-1)[90:90 + 96].view(1, 96)) is True
+    assert not ops._share(big[:1, :8], big[:, 8:]) and not ops._share(big[:, 8:], big[9:, :8])
+    assert not ops._share(big[:0], big) and ops._share(big[:1].expand(4, 96), big)
+
+
+def test_the_library_refuses_without_launching():
+    L = fplib.load()
+    p, n, m = 1 << 20, 4, 64                                # addresses that nothing may touch
+
+    def refused(name, *a):
+        assert getattr(L, name)(*a) == 1, (name, a)
+
+    ok = [p, m, p, m, p, p, m, p, m, n, m, 1e-6, None]
+    for name in ("fp_rmsnorm_residual_bf16", "fp_rmsnorm_residual_f16"):
+        for i, v in ((0, None), (4, None), (5, None), (1, -1), (3, -1), (6, m - 1), (8, m - 1), (9, -1), (10, 0), (11, -1.0),
+                     (7, None), (2, None)):
+            refused(name, *[v if j == i else t for j, t in enumerate(ok)])
+        refused(name, *[p + 1 if j == 0 else t for j, t in enumerate(ok)])          # not even the type's alignment
+        assert getattr(L, name)(*[0 if j == 9 else t for j, t in enumerate(ok)]) == 0          # no rows: nothing to do
+    ok = [p, m, p, m, p, p, m, p, p, m, n, m, 1e-6, None]
+    for i, v in ((0, None), (7, None), (7, p + 2), (5, None), (6, m - 1), (10, -1), (12, -1.0)):
+        refused("fp_rmsnorm_residual_fp8", *[v if j == i else t for j, t in enumerate(ok)])
+    ok = [p, m, p, m, p, m, p, p, m, p, n, m, 1e-6, p, 1 << 30, None]
+    for i, v in ((0, None), (2, None), (6, None), (7, None), (9, None), (8, m - 1), (10, 0), (11, 0), (13, None), (13, p + 4), (14, 16)):
+        refused("fp_rmsnorm_residual_backward_bf16", *[v if j == i else t for j, t in enumerate(ok)])
+    assert L.fp_rmsnorm_residual_backward_workspace_bytes(0, 8) == 0 and L.fp_gated_ff_backward_workspace_bytes(4, 0, 8) == 0
+    F, K = 16, 128
+    ok = [p, K, p, K, p, K, p, p, p, F, p, p, F, n, F, K, 0, None]
+    for i, v in ((0, None), (2, None), (4, None), (8, None), (6, None), (7, None), (10, None), (9, F - 1), (12, F - 1), (3, K - 1),
+                 (13, -1), (14, 0), (15, 0), (16, 2)):
+        refused("fp_gated_ff_bf16", *[v if j == i else t for j, t in enumerate(ok)])
+    ok = [p, K, p, p, K, p, p, K, p, p, p, p, F, n, F, K, 0, None]
+    for i, v in ((0, None), (2, None), (5, None), (8, None), (1, K + 8), (4, K + 8), (7, K + 8), (0, p + 8), (3, p + 8), (6, p + 8),
+                 (11, p + 8), (12, F + 4), (14, 12), (15, 64), (5, p + 4), (9, p + 2), (9, None), (16, -1)):
+        refused("fp_gated_ff_fp8", *[v if j == i else t for j, t in enumerate(ok)])
+    ok = [p, F, p, K, p, K, p, K, p, F, p, F, p, K, p, p, K, p, p, n, F, K, 0, p, 1 << 30, None]
+    for i, v in ((0, None), (2, None), (4, None), (8, None), (12, None), (14, None), (17, None), (13, K - 1), (16, K - 1), (19, 0),
+                 (20, 0), (21, 0), (22, 3), (23, None), (24, 16)):
+        refused("fp_gated_ff_backward_f16", *[v if j == i else t for j, t in enumerate(ok)])

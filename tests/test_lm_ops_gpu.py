@@ -1,0 +1,549 @@
+"""K12 (RMS norm of a residual sum) and K13 (gated feed-forward block), forward, in 8 bits and backward, against their
+definitions in 64 bits on the same inputs.
+
+Tolerances, element by element.  u = finfo(type).eps / 2 is the relative error of one rounding to the type; every kernel
+rounds each output once, from 32-bit arithmetic whose own errors are bounded by the usual  n 2^-24 sum|terms|  for a sum of
+n terms.  Where a half-precision result is subnormal the rounding is absolute (2^-25).  The gradient of K13 rounds dg and du
+to the type between its two steps: each counts u |dg| in every sum that takes it."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from framepack_amd import ops  # noqa: E402
+
+DEV = "cuda:0"
+BF, HF = torch.bfloat16, torch.float16
+E32 = 2.0 ** -24
+EPS = 1e-6
+
+
+def randn(*shape, seed=0, scale=1.0, dtype=torch.float32):
+    g = torch.Generator("cpu").manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+def u_of(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny_of(dtype):
+    return 2.0 ** -25 if dtype == HF else 0.0
+
+
+def within(got, want, tol, what=""):
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), (got - want)[bad][:4].tolist(), want[bad][:4].tolist(),
+                           torch.as_tensor(tol, device=got.device).expand_as(want)[bad][:4].tolist())
+
+
+def rel_l2(a, b):
+    a, b = a.double(), b.double()
+    return ((a - b).norm() / b.norm().clamp_min(1e-300)).item()
+
+
+def embed(t, left, right, fill=float("nan")):
+    """t as a row-strided view into a wider buffer of another value; returns (view, buffer)."""
+    big = torch.full((t.shape[0], left + t.shape[1] + right), fill, dtype=torch.float32, device=t.device).to(t.dtype)
+    big[:, left:left + t.shape[1]] = t
+    return big[:, left:left + t.shape[1]], big
+
+
+# ---- K12 ---------------------------------------------------------------------------------------------------------
+
+def norm64(x, resid, w, eps=EPS):
+    h = x.double() if resid is None else x.double() + resid.double()
+    return h, h / torch.sqrt((h * h).mean(1, keepdim=True) + eps) * w.double()
+
+
+def norm_tol(y, dtype, cols):
+    # sum of squares: relative error cols 2^-24 of a positive sum, halved by the root; four more roundings
+    return y.abs() * (u_of(dtype) + (cols / 2 + 8) * E32) + tiny_of(dtype)
+
+
+NORM_SHAPES = [(1, 1), (3, 7), (1, 64), (5, 72), (300, 128), (4, 1000), (7, 1001), (33, 1152), (1, 4096), (257, 4096), (3, 5003),
+               (2, 8192), (9, 8200), (2, 20000), (1, 40001), (2, 70000)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES)
+def test_norm(rows, cols, dtype):
+    x, r = randn(rows, cols, seed=1, dtype=dtype), randn(rows, cols, seed=2, scale=3.0, dtype=dtype)
+    w = (1 + randn(cols, seed=3, scale=0.3)).to(dtype)
+    y, h = ops.rmsnorm_residual(x, w, r)
+    h64, y64 = norm64(x, r, w)
+    within(h, h64, h64.abs() * (u_of(dtype) + 2 * E32) + tiny_of(dtype), "h")
+    within(y, y64, norm_tol(y64, dtype, cols), "y")
+    y1, h1 = ops.rmsnorm_residual(x, w)
+    assert h1 is x
+    _, y64 = norm64(x, None, w)
+    within(y1, y64, norm_tol(y64, dtype, cols), "y without a residual")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("cols", [64, 1000, 1001])
+def test_norm_of_strided_rows_leaves_the_gaps(cols, dtype):
+    rows = 37
+    x, r = randn(rows, cols, seed=1, dtype=dtype), randn(rows, cols, seed=2, dtype=dtype)
+    w = (1 + randn(cols, seed=3, scale=0.3)).to(dtype)
+    want, want_h = ops.rmsnorm_residual(x, w, r)
+    for left, right in ((8, 16), (3, 2)):                  # aligned for wide loads or not
+        xv, _ = embed(x, left, right)
+        rv, _ = embed(r, left, right)
+        ov, obuf = embed(torch.zeros_like(x), left, right, fill=7.0)
+        hv, hbuf = embed(torch.zeros_like(x), left, right, fill=7.0)
+        y, h = ops.rmsnorm_residual(xv, w, rv, out=ov, resid_out=hv)
+        assert y.data_ptr() == ov.data_ptr() and h.data_ptr() == hv.data_ptr()
+        within(y, want, want.double().abs() * (2 * u_of(dtype)) + 2 * tiny_of(dtype))
+        assert torch.equal(h, want_h)
+        for buf in (obuf, hbuf):
+            assert (buf[:, :left] == 7).all() and (buf[:, left + cols:] == 7).all()
+    y, h = ops.rmsnorm_residual(x[:1].expand(rows, cols), w, r)             # one row of x for all
+    h64, y64 = norm64(x[:1].expand(rows, cols), r, w)
+    within(y, y64, norm_tol(y64, dtype, cols))
+
+
+@pytest.mark.parametrize("cols", [64, 1001, 4096, 20000, 70000])
+def test_norm_in_place(cols):
+    x, r, w = randn(9, cols, seed=1, dtype=BF), randn(9, cols, seed=2, dtype=BF), randn(cols, seed=3, dtype=BF)
+    y0, h0 = ops.rmsnorm_residual(x, w, r)
+    for swap in (False, True):
+        a, b = x.clone(), r.clone()
+        y, h = ops.rmsnorm_residual(a, w, b, out=b if swap else a, resid_out=a if swap else b)
+        assert torch.equal(y, y0) and torch.equal(h, h0)
+        assert torch.equal(a, h0 if swap else y0) and torch.equal(b, y0 if swap else h0)
+
+
+def test_norm_of_rows_of_zeros_infinities_and_nan_keeps_to_the_row():
+    cols = 1024
+    x, w = randn(8, cols, seed=1, dtype=BF), randn(cols, seed=3, dtype=BF)
+    r = randn(8, cols, seed=2, dtype=BF)
+    y0, h0 = ops.rmsnorm_residual(x, w, r)
+    q0, s0, _ = ops.rmsnorm_residual_fp8(x, w, r)
+    x[1], r[1] = 0, 0
+    x[3, 5] = float("nan")
+    x[5, 7] = float("inf")
+    y, h = ops.rmsnorm_residual(x, w, r)
+    q, s, hq = ops.rmsnorm_residual_fp8(x, w, r)
+    keep = [0, 2, 4, 6, 7]
+    assert torch.equal(y[keep], y0[keep]) and torch.equal(h[keep], h0[keep])
+    assert torch.equal(q[keep].view(torch.uint8), q0[keep].view(torch.uint8)) and torch.equal(s[keep], s0[keep])
+    assert (y[1] == 0).all() and (h[1] == 0).all() and s[1].item() == 1.0 and (q[1].float() == 0).all()
+    assert y[3].isnan().all() and q[3].float().isnan().all() and h[3].isnan().sum() == 1
+    # inf: the mean is inf, the finite values go to 0 and inf * 0 is NaN - as in torch
+    f = x[5].float() + r[5].float()
+    want = f * torch.rsqrt(f.square().mean() + EPS) * w.float()
+    assert torch.equal(y[5].isnan(), want.isnan()) and (y[5][~want.isnan()] == 0).all() and h[5, 7].item() == float("inf")
+    assert torch.equal(hq.isnan(), h.isnan())
+
+
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES)
+def test_norm_to_8_bits(rows, cols):
+    x, r = randn(rows, cols, seed=1, dtype=BF), randn(rows, cols, seed=2, scale=3.0, dtype=BF)
+    x[0, 0] = 90.0                                          # an outlier: only its row loses resolution
+    w = (1 + randn(cols, seed=3, scale=0.3)).to(BF)
+    q, s, h = ops.rmsnorm_residual_fp8(x, w, r)
+    h64, y64 = norm64(x, r, w)
+    within(h, h64, h64.abs() * (u_of(BF) + 2 * E32), "h")
+    amax = y64.abs().amax(1)
+    fp = (cols / 2 + 10) * E32
+    within(s, amax / 448, amax / 448 * fp, "scale")
+    deq = q.double() * s.double()[:, None]
+    # half a step of e4m3: 2^-4 of the value, 2^-10 of the scale below the normal range
+    within(deq, y64, (y64.abs() * 2.0 ** -4).clamp_min(0) * (1 + 4 * fp) + s.double()[:, None] * 2.0 ** -10 + y64.abs() * fp, "q")
+    assert not q.float().isnan().any()
+    # nearly always the nearest of all e4m3 values
+    ref = (y64 / (amax / 448)[:, None]).float().to(ops.FP8).float()
+    assert (q.float() != ref).double().mean().item() <= 1e-3 + 2 / (rows * cols)
+    ov, obuf = embed(torch.zeros(rows, cols, device=DEV), 5, 6, fill=1.0)
+    o8 = obuf.to(ops.FP8)
+    q2, s2, _ = ops.rmsnorm_residual_fp8(x, w, r, out=o8[:, 5:5 + cols])
+    within(q2.double() * s2.double()[:, None], deq, deq.abs() * 2.0 ** -3 * (1 + 4 * fp) + s.double()[:, None] * 2.0 ** -9)
+    assert (o8[:, :5].float() == 1).all() and (o8[:, 5 + cols:].float() == 1).all()
+
+
+def norm_grad64(dy, h, w, dh, eps=EPS):
+    dy, h, w = dy.double(), h.double(), w.double()
+    r = 1 / torch.sqrt((h * h).mean(1, keepdim=True) + eps)
+    n, dn = h * r, dy * w
+    k = (dn * n).mean(1, keepdim=True)
+    dx = r * (dn - n * k) + (0 if dh is None else dh.double())
+    terms = r * (dn.abs() + n.abs() * (dn * n).abs().mean(1, keepdim=True)) + (0 if dh is None else dh.double().abs())
+    return dx, (dy * n).sum(0), terms, (dy * n).abs().sum(0)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES + [(700, 64), (1500, 520), (2049, 136)])
+def test_norm_gradient(rows, cols, dtype):
+    dy, h = randn(rows, cols, seed=1, dtype=dtype), randn(rows, cols, seed=2, scale=2.0, dtype=dtype)
+    dh, w = randn(rows, cols, seed=4, dtype=dtype), (1 + randn(cols, seed=3, scale=0.3)).to(dtype)
+    h[rows // 2] = 0                                        # a row of padding
+    dy[rows // 2] = 0
+    for up in (dh, None):
+        dx, dw = ops.rmsnorm_residual_backward(dy, h, w, dh=up)
+        dx64, dw64, tx, tw = norm_grad64(dy, h, w, up)
+        within(dx, dx64, dx64.abs() * u_of(dtype) + tx * (cols + 16) * E32 * 2 + tiny_of(dtype), "dx")
+        within(dw, dw64, dw64.abs() * u_of(dtype) + tw * (rows + cols / 2 + 16) * E32 * 2 + tiny_of(dtype), "dweight")
+    again = ops.rmsnorm_residual_backward(dy, h, w)
+    assert torch.equal(again[0], dx) and torch.equal(again[1], dw)          # a fixed order
+    inplace = dh.clone()
+    got, _ = ops.rmsnorm_residual_backward(dy, h, w, dh=inplace, dx=inplace)
+    assert got.data_ptr() == inplace.data_ptr()
+    assert torch.equal(got, ops.rmsnorm_residual_backward(dy, h, w, dh=dh)[0])
+
+
+def test_norm_gradient_of_strided_and_broadcast_rows():
+    rows, cols = 40, 264
+    dy, h, dh = (randn(rows, cols, seed=i, dtype=BF) for i in (1, 2, 3))
+    w = randn(cols, seed=4, dtype=BF)
+    want = ops.rmsnorm_residual_backward(dy, h, w, dh=dh)
+    for left, right in ((8, 8), (1, 4)):
+        dxv, buf = embed(torch.zeros_like(h), left, right, fill=5.0)
+        got = ops.rmsnorm_residual_backward(embed(dy, left, right)[0], embed(h, left, right)[0], w, dh=embed(dh, left, right)[0],
+                                            dx=dxv)
+        within(got[0], want[0], want[0].double().abs() * 2 * u_of(BF) + 1e-5)
+        within(got[1], want[1], want[1].double().abs() * 2 * u_of(BF) + 1e-4)
+        assert (buf[:, :left] == 5).all() and (buf[:, left + cols:] == 5).all()
+    one = dy[:1].expand(rows, cols)
+    assert torch.equal(ops.rmsnorm_residual_backward(one, h, w)[0], ops.rmsnorm_residual_backward(one.contiguous(), h, w)[0])
+
+
+def test_norm_gradient_against_differences():
+    rows, cols = 6, 96
+    h, w, dy = randn(rows, cols, seed=1, dtype=BF), randn(cols, seed=2, dtype=BF), randn(rows, cols, seed=3, dtype=BF)
+    dx, dw = ops.rmsnorm_residual_backward(dy, h, w)
+
+    def loss(h_, w_):
+        return (dy.double() * (h_ / torch.sqrt((h_ * h_).mean(1, keepdim=True) + EPS) * w_)).sum()
+
+    v, z, d = randn(rows, cols, seed=5).double(), randn(cols, seed=6).double(), 1e-5
+    num = (loss(h.double() + d * v, w.double()) - loss(h.double() - d * v, w.double())) / (2 * d)
+    assert abs((dx.double() * v).sum() - num) <= u_of(BF) * (dx.double() * v).abs().sum() + 1e-5 * (dx.double() * v).abs().sum()
+    num = (loss(h.double(), w.double() + d * z) - loss(h.double(), w.double() - d * z)) / (2 * d)
+    assert abs((dw.double() * z).sum() - num) <= u_of(BF) * (dw.double() * z).abs().sum() + 1e-5 * (dw.double() * z).abs().sum()
+
+
+# ---- K13 ---------------------------------------------------------------------------------------------------------
+
+def act64(v, act):
+    """act(v), act'(v) for finite v."""
+    if act == ops.ACT_SILU:
+        s = torch.sigmoid(v)
+        return v * s, s * (1 + v * (1 - s))
+    k = math.sqrt(2 / math.pi)
+    t = torch.tanh(k * (v + 0.044715 * v ** 3))
+    return 0.5 * v * (1 + t), 0.5 * (1 + t) + 0.5 * v * (1 - t * t) * k * (1 + 3 * 0.044715 * v * v)
+
+
+def ff64(x, wg, wu, bg, bu, act):
+    """h, g, u and the bounds of the 32-bit sums' errors of g and u."""
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    n = 2 * (x.shape[1] + 4) * E32
+    g, u = x @ wg.t(), x @ wu.t()
+    eg, eu = n * (x.abs() @ wg.abs().t()), n * (x.abs() @ wu.abs().t())
+    if bg is not None:
+        g, u = g + bg.double(), u + bu.double()
+        eg, eu = eg + 2 * E32 * bg.double().abs(), eu + 2 * E32 * bu.double().abs()
+    return act64(g, act)[0] * u, g, u, eg, eu
+
+
+def ff_tol(h, g, u, eg, eu, act, dtype):
+    # |act'| < 1.13; the sigmoid's exponential has a relative error of about 2 |z| 2^-24, |z| < 88 where it is not 0
+    return h.abs() * (u_of(dtype) + 400 * E32) + 1.13 * eg * u.abs() + eu * act64(g, act)[0].abs() + 1.13 * eg * eu + tiny_of(dtype)
+
+
+FF_SHAPES = [(1, 1, 1), (1, 8, 64), (1, 130, 100), (2, 7, 40), (5, 64, 64), (16, 72, 128), (17, 136, 192), (33, 264, 520), (64, 520, 64),
+             (65, 129, 72), (129, 256, 128), (257, 264, 256), (300, 1000, 1001), (513, 24, 320), (1, 4096, 1024), (7, 2056, 576)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("act", [ops.ACT_SILU, ops.ACT_GELU])
+@pytest.mark.parametrize("M,F,K", FF_SHAPES)
+def test_gated_ff(M, F, K, act, dtype):
+    x = randn(M, K, seed=1, dtype=dtype)
+    wg, wu = randn(F, K, seed=2, scale=2 * K ** -0.5, dtype=dtype), randn(F, K, seed=3, scale=K ** -0.5, dtype=dtype)
+    bg, bu = randn(F, seed=4, dtype=dtype), randn(F, seed=5, dtype=dtype)
+    for b in ((None, None), (bg, bu)):
+        h64, g, u, eg, eu = ff64(x, wg, wu, *b, act)
+        h = ops.gated_ff(x, wg, wu, *b, act=act)
+        within(h, h64, ff_tol(h64, g, u, eg, eu, act, dtype), "h")
+        h2, gate, up = ops.gated_ff(x, wg, wu, *b, act=act, keep=True)
+        assert torch.equal(h, h2)
+        within(gate, g, g.abs() * u_of(dtype) + 2 * eg + tiny_of(dtype), "gate")
+        within(up, u, u.abs() * u_of(dtype) + 2 * eu + tiny_of(dtype), "up")
+
+
+@pytest.mark.parametrize("M,F,K", [(3, 64, 128), (70, 136, 192), (300, 264, 64)])
+@pytest.mark.parametrize("left,right", [(8, 24), (3, 2)])
+def test_gated_ff_of_strided_operands_leaves_the_gaps(M, F, K, left, right):
+    x, w = randn(M, K, seed=1, dtype=BF), randn(2 * F, K, seed=2, scale=K ** -0.5, dtype=BF)
+    wv, _ = embed(w, left, right)
+    xv, _ = embed(x, left, right)
+    ov, buf = embed(torch.zeros(M, F, dtype=BF, device=DEV), left, right, fill=7.0)
+    h = ops.gated_ff(xv, wv[:F], wv[F:], out=ov)
+    h64, g, u, eg, eu = ff64(x, w[:F], w[F:], None, None, ops.ACT_SILU)
+    assert h.data_ptr() == ov.data_ptr()
+    within(h, h64, ff_tol(h64, g, u, eg, eu, ops.ACT_SILU, BF))
+    assert (buf[:, :left] == 7).all() and (buf[:, left + F:] == 7).all()
+    one = x[:1].expand(M, K)                                # one row for all
+    got = ops.gated_ff(one, w[:F], w[F:])
+    assert torch.equal(got, ops.gated_ff(one.contiguous(), w[:F], w[F:]))
+    # two weights of different strides
+    got = ops.gated_ff(x, wv[:F], w[F:].contiguous())
+    within(got, h64, ff_tol(h64, g, u, eg, eu, ops.ACT_SILU, BF))
+
+
+@pytest.mark.parametrize("M", [1, 20, 70, 260])
+def test_gated_ff_keeps_infinities_and_nan_to_their_rows(M):
+    F, K = 136, 128
+    x, wg, wu = randn(M, K, seed=1, dtype=BF), randn(F, K, seed=2, dtype=BF), randn(F, K, seed=3, dtype=BF)
+    clean = ops.gated_ff(x, wg, wu)
+    x[0, 3] = float("nan")
+    if M > 1:
+        x[M - 1, 4] = float("inf")
+    h = ops.gated_ff(x, wg, wu)
+    assert h[0].isnan().all()
+    assert torch.equal(h[1:M - 1], clean[1:M - 1])
+    if M > 1:
+        ref = x[M - 1:].float()
+        g, u = ref @ wg.float().t(), ref @ wu.float().t()
+        want = torch.nn.functional.silu(g) * u
+        assert torch.equal(h[M - 1:].isnan(), want.isnan()) and torch.equal(h[M - 1:].isinf(), want.isinf())
+
+
+def quantised(t):
+    return ops.quantize_weight_fp8(t)
+
+
+@pytest.mark.parametrize("act", [ops.ACT_SILU, ops.ACT_GELU])
+@pytest.mark.parametrize("M,F,K", [(1, 8, 128), (1, 1040, 256), (3, 72, 128), (16, 136, 384), (17, 520, 128), (33, 64, 256), (65, 136, 512),
+                                   (130, 264, 128), (257, 128, 256), (300, 1000, 1152)])
+def test_gated_ff_in_8_bits(M, F, K, act):
+    x, xs = ops.quantize_rows_fp8(randn(M, K, seed=1, dtype=BF))
+    wg, gs = quantised(randn(F, K, seed=2, scale=2 * K ** -0.5))
+    wu, us = quantised(randn(F, K, seed=3, scale=K ** -0.5))
+    bg, bu = randn(F, seed=4, dtype=BF), randn(F, seed=5, dtype=BF)
+    deq = [q.double() * s.double()[:, None] for q, s in ((x, xs), (wg, gs), (wu, us))]
+    for b in ((None, None), (bg, bu)):
+        h = ops.gated_ff_fp8(x, xs, wg, gs, wu, us, *b, act=act)
+        h64, g, u, eg, eu = ff64(*deq, *b, act)
+        within(h, h64, ff_tol(h64, g, u, eg + 4 * E32 * g.abs(), eu + 4 * E32 * u.abs(), act, BF))
+    ov, buf = embed(torch.zeros(M, F, dtype=BF, device=DEV), 8, 16, fill=7.0)
+    assert torch.equal(ops.gated_ff_fp8(x, xs, wg, gs, wu, us, bg, bu, act=act, out=ov), h)
+    assert (buf[:, :8] == 7).all() and (buf[:, 8 + F:] == 7).all()
+
+
+def ff_grad64(dh, x, wg, wu, g, u, act):
+    dh, x, wg, wu, g, u = (t.double() for t in (dh, x, wg, wu, g, u))
+    a, da = act64(g, act)
+    return dh * u * da, dh * a, x, wg, wu
+
+
+def check_ff_grad(got, dh, x, wg, wu, g, u, act, dtype):
+    dx, dwg, dwu, dbg, dbu = got
+    M, F, K = dh.shape[0], dh.shape[1], x.shape[1]
+    dg, du, x, wg, wu = ff_grad64(dh, x, wg, wu, g, u, act)
+    # dg and du: 32-bit arithmetic, then one rounding.  act' = s + v s (1 - s) z' cancels near its zeros (|act'| can be
+    # far below its terms, which stay below 1.13 + |v z'| s (1 - s) < 3): an absolute part of 3 |dh u| times the 32-bit errors
+    ug = u_of(dtype) * dg.abs() + 3 * 400 * E32 * dh.double().abs() * u.double().abs() + tiny_of(dtype)
+    uu = (u_of(dtype) + 400 * E32) * du.abs() + tiny_of(dtype)
+    n = 2 * (2 * F + 8) * E32
+    want = dg @ wg + du @ wu
+    within(dx, want, want.abs() * u_of(dtype) + (ug + n * dg.abs()) @ wg.abs() + (uu + n * du.abs()) @ wu.abs() + tiny_of(dtype), "dx")
+    n = 2 * (M + 8) * E32
+    for d, e, o, b, name in ((dg, ug, dwg, dbg, "gate"), (du, uu, dwu, dbu, "up")):
+        want = d.t() @ x
+        within(o, want, want.abs() * u_of(dtype) + (e + n * d.abs()).t() @ x.abs() + tiny_of(dtype), "dw_" + name)
+        if b is not None:
+            within(b, d.sum(0), d.sum(0).abs() * u_of(dtype) + (e + n * d.abs()).sum(0) + tiny_of(dtype), "db_" + name)
+
+
+FF_GRAD_SHAPES = [(1, 1, 1), (1, 64, 64), (2, 7, 40), (5, 130, 100), (16, 72, 128), (65, 129, 72), (64, 128, 64), (129, 256, 128),
+                  (257, 264, 256), (300, 1000, 1001), (513, 24, 320), (1000, 136, 64), (200, 2056, 576)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("act", [ops.ACT_SILU, ops.ACT_GELU])
+@pytest.mark.parametrize("M,F,K", FF_GRAD_SHAPES)
+def test_gated_ff_gradient(M, F, K, act, dtype):
+    dh, x = randn(M, F, seed=1, dtype=dtype), randn(M, K, seed=2, dtype=dtype)
+    wg, wu = randn(F, K, seed=3, scale=K ** -0.5, dtype=dtype), randn(F, K, seed=4, scale=K ** -0.5, dtype=dtype)
+    g, u = randn(M, F, seed=5, scale=2.0, dtype=dtype), randn(M, F, seed=6, dtype=dtype)
+    for bias in (True, False):
+        got = ops.gated_ff_backward(dh, x, wg, wu, g, u, act=act, bias=bias)
+        assert (got[3] is not None) == bias and (got[4] is not None) == bias
+        check_ff_grad(got, dh, x, wg, wu, g, u, act, dtype)
+    again = ops.gated_ff_backward(dh, x, wg, wu, g, u, act=act)
+    assert all(torch.equal(a, b) for a, b in zip(again[:3], got[:3]))
+    if M * F * K > 1 << 20:                                # two roundings of relative rms at most u / sqrt(3) each
+        d = ff_grad64(dh, x, wg, wu, g, u, act)
+        assert rel_l2(got[0], d[0] @ d[3] + d[1] @ d[4]) < 1.0 * u_of(dtype)
+        assert rel_l2(got[1], d[0].t() @ d[2]) < 1.0 * u_of(dtype)
+
+
+@pytest.mark.parametrize("left,right", [(8, 24), (3, 2)])
+def test_gated_ff_gradient_of_strided_operands(left, right):
+    M, F, K = 70, 136, 192
+    t = [randn(M, F, seed=1, dtype=BF), randn(M, K, seed=2, dtype=BF), randn(F, K, seed=3, dtype=BF), randn(F, K, seed=4, dtype=BF),
+         randn(M, F, seed=5, dtype=BF), randn(M, F, seed=6, dtype=BF)]
+    got = ops.gated_ff_backward(*[embed(v, left, right)[0] for v in t], bias=True)
+    check_ff_grad(got, *t, ops.ACT_SILU, BF)
+    t[0] = t[0][:1].expand(M, F)                           # one gradient for all rows, as of a sum over them
+    check_ff_grad(ops.gated_ff_backward(*t, bias=True), *t, ops.ACT_SILU, BF)
+
+
+def test_gated_ff_gradient_far_from_zero_is_finite():
+    M, F, K = 4, 64, 64
+    g = torch.tensor([-300.0, -90.0, 90.0, 300.0], device=DEV).to(BF)[:, None].expand(M, F).contiguous()
+    dh, u, x = torch.ones(M, F, device=DEV, dtype=BF), torch.ones(M, F, device=DEV, dtype=BF), randn(M, K, seed=1, dtype=BF)
+    wg, wu = randn(F, K, seed=2, dtype=BF), randn(F, K, seed=3, dtype=BF)
+    for act in (ops.ACT_SILU, ops.ACT_GELU):
+        check_ff_grad(ops.gated_ff_backward(dh, x, wg, wu, g, u, act=act, bias=True), dh, x, wg, wu, g, u, act, BF)
+
+
+def test_gated_ff_gradient_against_differences():
+    M, F, K = 9, 40, 64
+    x, wg, wu = randn(M, K, seed=1, dtype=HF), randn(F, K, seed=2, scale=0.125, dtype=HF), randn(F, K, seed=3, scale=0.125, dtype=HF)
+    bg, bu, dh = randn(F, seed=4, dtype=HF), randn(F, seed=5, dtype=HF), randn(M, F, seed=6, dtype=HF)
+    for act in (ops.ACT_SILU, ops.ACT_GELU):
+        _, g, u = ops.gated_ff(x, wg, wu, bg, bu, act=act, keep=True)
+        got = ops.gated_ff_backward(dh, x, wg, wu, g, u, act=act, bias=True)
+        at = [t.double() for t in (x, wg, wu, bg, bu)]
+
+        def loss(p):
+            return (dh.double() * act64(p[0] @ p[1].t() + p[3], act)[0] * (p[0] @ p[2].t() + p[4])).sum()
+
+        for i, grad in enumerate(got):
+            v, d = randn(*grad.shape, seed=10 + i).double(), 1e-5
+            num = (loss([t + d * v if j == i else t for j, t in enumerate(at)]) -
+                   loss([t - d * v if j == i else t for j, t in enumerate(at)])) / (2 * d)
+            # g and u are rounded where they are kept, dg and du where they are handed on, the result at the end: each
+            # moves a term by at most a few u of its size; the terms add up to at most sum|dh| (|act'| |u| + |act|) |..|
+            a, da = act64(g.double(), act)
+            size = (dh.double().abs() * (da.abs() * u.double().abs() + a.abs())).sum() * 3
+            assert abs((grad.double() * v).sum() - num) <= 4 * u_of(HF) * size, (act, i)
+
+
+# ---- together, and the ways they are called -----------------------------------------------------------------------
+
+def layer_inputs(M, D, F, dtype=BF):
+    x, r = randn(M, D, seed=1, dtype=dtype), randn(M, D, seed=2, dtype=dtype)
+    w = (1 + randn(D, seed=3, scale=0.2)).to(dtype)
+    wg, wu, wd = (randn(a, b, seed=s, scale=b ** -0.5, dtype=dtype) for a, b, s in ((F, D, 4), (F, D, 5), (D, F, 6)))
+    return x, r, w, wg, wu, wd
+
+
+@pytest.mark.parametrize("M", [1, 19, 260])
+def test_a_block_of_norm_gated_ff_and_residual_linear(M):
+    D, F = 256, 640
+    x, r, w, wg, wu, wd = layer_inputs(M, D, F)
+    n, h = ops.rmsnorm_residual(x, w, r)
+    a, gate, up = ops.gated_ff(n, wg, wu, keep=True)
+    y = ops.gemm(a, wd, None, epilogue=ops.EPI_RESIDUAL, resid=h)
+    h64, n64 = norm64(x, r, w)
+    a64 = ff64(n64, wg, wu, None, None, ops.ACT_SILU)[0]
+    y64 = a64 @ wd.double().t() + h64
+    # n, a, h and y are rounded once each: rms at most u / sqrt(3) relative, the first three through maps of size about one
+    assert rel_l2(y, y64) < 2 * u_of(BF)
+    # in 8 bits: e4m3 values are within 2^-4, of relative rms at most 2^-4 / sqrt(3) = 3.6 %, in x, the weights and a:
+    # three linears' worth of two roundings each, of which the residual takes a part
+    q, s, h8 = ops.rmsnorm_residual_fp8(x, w, r)
+    assert torch.equal(h8, h)
+    a8 = ops.gated_ff_fp8(q, s, *quantised(wg.float()), *quantised(wu.float()))
+    aq, as_ = ops.quantize_rows_fp8(a8)
+    wq, ws = quantised(wd.float())
+    y8 = ops.gemm_fp8(aq, as_, wq, ws, None, epilogue=ops.EPI_RESIDUAL, resid=h)
+    assert rel_l2(y8, y64) < 3 * math.sqrt(2) * 0.036
+    # and back: the whole block's gradient against differences of its definition in 64 bits
+    dy = randn(M, D, seed=9, dtype=BF)
+    da = ops.gemm(dy, wd.t().contiguous(), None)
+    dn, dwg, dwu, _, _ = ops.gated_ff_backward(da, n, wg, wu, gate, up)
+    dx, dw = ops.rmsnorm_residual_backward(dn, h, w, dh=dy)
+
+    def loss(x_, w_):
+        h_ = r.double() + x_
+        n_ = h_ / torch.sqrt((h_ * h_).mean(1, keepdim=True) + EPS) * w_
+        return (dy.double() * (h_ + (act64(n_ @ wg.double().t(), 0)[0] * (n_ @ wu.double().t())) @ wd.double().t())).sum()
+
+    p = x.double().requires_grad_(), w.double().requires_grad_()
+    want = torch.autograd.grad(loss(*p), p)
+    # seven roundings between the loss and dx (n, gate and up, da, dg and du, dn, h, dx), of relative rms at most u / sqrt(3)
+    assert rel_l2(dx, want[0]) < math.sqrt(9 / 3) * 2 * u_of(BF)
+    assert rel_l2(dw, want[1]) < math.sqrt(9 / 3) * 2 * u_of(BF)
+
+
+@pytest.mark.parametrize("M", [1, 19, 300])
+def test_captured_replayed_and_on_another_stream(M):
+    D, F = 256, 264
+    x, r, w, wg, wu, _ = layer_inputs(M, D, F)
+    dh = randn(M, F, seed=8, dtype=BF)
+    q8, s8 = ops.quantize_rows_fp8(x)
+    w8 = (*quantised(wg.float()), *quantised(wu.float()))
+
+    def step():
+        n, h = ops.rmsnorm_residual(x, w, r)
+        q, s, _ = ops.rmsnorm_residual_fp8(x, w, r)
+        a, g, u = ops.gated_ff(n, wg, wu, keep=True)
+        dn, dwg, dwu, dbg, dbu = ops.gated_ff_backward(dh, n, wg, wu, g, u, bias=True)
+        dx, dw = ops.rmsnorm_residual_backward(dn, h, w)
+        return [n, h, q.view(torch.uint8), s, a, g, u, dn, dwg, dwu, dbg, dbu, dx, dw, ops.gated_ff_fp8(q8, s8, *w8)]
+
+    eager = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(eager, other))
+    graphs, outs = [], []
+    for _ in range(2):                                     # two graphs alive at once, captured one after the other
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    x0 = x.clone()
+    for k in range(3):
+        x.copy_(x0 * (1 + k))
+        for o in outs:
+            for t in o:
+                t.zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for o in outs:
+            assert all(torch.equal(a, b) for a, b in zip(want, o)), k
+
+
+def test_empty_batches():
+    x, w, wg = torch.empty(0, 64, dtype=BF, device=DEV), torch.ones(64, dtype=BF, device=DEV), randn(16, 64, dtype=BF)
+    y, h = ops.rmsnorm_residual(x, w, x)
+    assert y.shape == (0, 64) and h.shape == (0, 64)
+    q, s, h = ops.rmsnorm_residual_fp8(x, w, x)
+    assert q.shape == (0, 64) and s.shape == (0,)
+    dx, dw = ops.rmsnorm_residual_backward(x, x, w)
+    assert dx.shape == (0, 64) and (dw == 0).all()
+    assert [t.shape[0] for t in ops.gated_ff(x, wg, wg, keep=True)] == [0, 0, 0]
+    e = torch.empty(0, 16, dtype=BF, device=DEV)
+    dx, dwg, dwu, dbg, dbu = ops.gated_ff_backward(e, x, wg, wg, e, e, bias=True)
+    assert dx.shape == (0, 64) and all((t == 0).all() for t in (dwg, dwu, dbg, dbu)) and dwg.shape == (16, 64)
+
+
+def test_matrices_past_two_gigabytes():
+    rows, cols = 70000, 16384                              # 2.3 GB a matrix: byte offsets past 2^31, elements past 2^30
+    x = torch.randn(64, cols, device=DEV).to(BF).repeat(rows // 64 + 1, 1)[:rows]
+    w = randn(cols, seed=1, dtype=BF)
+    y, h = ops.rmsnorm_residual(x, w, x)
+    want, _ = ops.rmsnorm_residual(x[:64].contiguous(), w, x[:64].contiguous())
+    assert torch.equal(y[rows // 64 * 64 - 64:rows // 64 * 64], want) and torch.equal(y[:64], want)
+    del y, h
+    wg = randn(64, cols, seed=2, scale=cols ** -0.5, dtype=BF)
+    a = ops.gated_ff(x, wg, wg)
+    want = ops.gated_ff(x[:256].contiguous(), wg, wg)
+    k = rows // 256 * 256
+    assert torch.equal(a[:256], want) and torch.equal(a[k - 256:k], want)
