@@ -3,9 +3,14 @@
 // include/framepack_hip.h.
 //
 //   dg = dh u act'(g)   du = dh act(g)   dx = dg . Wg + du . Wu   dWg = dg^T . x   dWu = du^T . x   db = column sums
+#include "gated_ff.h"
 #include "gemm_pipeline.h"
 
 extern "C" int64_t fp_gated_ff_backward_workspace_bytes(int M, int F, int K);
+extern "C" int fp_gemm_bf16(const void*, int64_t, const void*, int, const void*, int64_t, const void*, void*, int64_t, int, int, int, int,
+                            int, const void*, int64_t, const void*, void*);
+extern "C" int fp_gemm_f16(const void*, int64_t, const void*, int, const void*, int64_t, const void*, void*, int64_t, int, int, int, int,
+                           int, const void*, int64_t, const void*, void*);
 
 namespace {
 
@@ -33,10 +38,7 @@ __device__ __forceinline__ void act_grad(float v, int act, float& a, float& da) 
 }
 
 // ---- any size, any strides: 64 x 64 output tiles, one element per load -------------------------------------------
-// GLU:  c = act(a . b0^T + bias0) * (a . b1^T + bias1)        (p0, p1: the two projections, or null)
-// else: c = a . b0^T (+ a1 . b1^T)
-// a[m][k] = a[m * a_rs + k * a_ks] and so on: every orientation of the gradient's products is one call.
-// e4m3 operands are widened to bf16, which holds them exactly; a_scale [M], b_scale0/1 [N] (or null).
+// For operands that the wide loads cannot read.  e4m3 operands are widened to bf16, which holds them exactly.
 template <typename TI> struct widen {
     typedef TI type;
     typedef TI vec8 __attribute__((ext_vector_type(8)));
@@ -47,16 +49,22 @@ template <> struct widen<fp8e4> {
     typedef bf16x8 vec8;
     static __device__ __forceinline__ bf16 of(fp8e4 v) { return (bf16)__builtin_amdgcn_cvt_f32_fp8((int)v.bits, 0); }
 };
-struct Operand {
-    const void* p;
-    int64_t rs, ks;
+struct GluCall {
+    const void* x;
+    int64_t ldx;
+    const float* xs;
+    const void *w[2];               // gate, up
+    int64_t ldw[2];
+    const float* ws[2];
+    const void* b[2];
+    void* h;
+    int64_t ldh;
+    void* pre[2];
+    int64_t ldp;
+    int M, F, K, act;
 };
-template <typename TI, typename TO, bool GLU>
-__global__ __launch_bounds__(256) void any_gemm_kernel(Operand a, Operand b0, Operand a1, Operand b1, const float* __restrict__ a_scale,
-                                                       const float* __restrict__ s0, const float* __restrict__ s1,
-                                                       const TO* __restrict__ bias0, const TO* __restrict__ bias1,
-                                                       TO* __restrict__ c, int64_t ldc, TO* __restrict__ p0, TO* __restrict__ p1,
-                                                       int64_t ldp, int M, int N, int K, int act) {
+template <typename TI, typename TO>
+__global__ __launch_bounds__(256) void glu_any_kernel(GluCall q) {
     typedef typename widen<TI>::type TM;
     typedef typename widen<TI>::vec8 TM8;
     __shared__ __attribute__((aligned(16))) TM sa[64][40], sb[2][64][40];      // rows of 32, padded to 80 B
@@ -64,36 +72,31 @@ __global__ __launch_bounds__(256) void any_gemm_kernel(Operand a, Operand b0, Op
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
     f32x4 acc[2][2][2] = {};
-    auto stage = [&](TM (*dst)[40], const Operand& o, int64_t r0, int rows, int k0) {
-        const TI* p = reinterpret_cast<const TI*>(o.p);
-        // the axis with unit stride goes along the lanes
-        const bool kfast = o.ks == 1;
+    auto stage = [&](TM (*dst)[40], const void* base, int64_t ld, int64_t r0, int rows, int k0) {
+        const TI* p = reinterpret_cast<const TI*>(base);
         for (int i = tid; i < 64 * 32; i += 256) {
-            const int r = kfast ? i >> 5 : i & 63, k = kfast ? i & 31 : i >> 6;
+            const int r = i >> 5, k = i & 31;
             TM v = (TM)0.f;
-            if (r0 + r < rows && k0 + k < K) v = widen<TI>::of(p[(r0 + r) * o.rs + (int64_t)(k0 + k) * o.ks]);
+            if (r0 + r < rows && k0 + k < q.K) v = widen<TI>::of(p[(r0 + r) * ld + k0 + k]);
             dst[r][k] = v;
         }
     };
-    const int segs = !GLU && a1.p ? 2 : 1;
-    for (int seg = 0; seg < segs; ++seg)
-        for (int k0 = 0; k0 < K; k0 += 32) {
-            stage(sa, seg ? a1 : a, m0, M, k0);
-            stage(sb[0], seg ? b1 : b0, n0, N, k0);
-            if constexpr (GLU) stage(sb[1], b1, n0, N, k0);
-            __syncthreads();
+    for (int k0 = 0; k0 < q.K; k0 += 32) {
+        stage(sa, q.x, q.ldx, m0, q.M, k0);
+        stage(sb[0], q.w[0], q.ldw[0], n0, q.F, k0);
+        stage(sb[1], q.w[1], q.ldw[1], n0, q.F, k0);
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const TM8 av = *reinterpret_cast<const TM8*>(&sa[wm + i * 16 + (lane & 15)][(lane >> 4) * 8]);
+        for (int i = 0; i < 2; ++i) {
+            const TM8 av = *reinterpret_cast<const TM8*>(&sa[wm + i * 16 + (lane & 15)][(lane >> 4) * 8]);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int g = 0; g < (GLU ? 2 : 1); ++g)
-                        acc[g][i][j] = mfma16(*reinterpret_cast<const TM8*>(&sb[g][wn + j * 16 + (lane & 15)][(lane >> 4) * 8]), av,
-                                              acc[g][i][j]);
-            }
-            __syncthreads();
+                for (int g = 0; g < 2; ++g)
+                    acc[g][i][j] = mfma16(*reinterpret_cast<const TM8*>(&sb[g][wn + j * 16 + (lane & 15)][(lane >> 4) * 8]), av, acc[g][i][j]);
         }
+        __syncthreads();
+    }
     // (operands swapped: the lane's low bits are the row, its four registers four columns)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -102,59 +105,238 @@ __global__ __launch_bounds__(256) void any_gemm_kernel(Operand a, Operand b0, Op
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int64_t m = m0 + wm + i * 16 + (lane & 15), n = n0 + wn + j * 16 + (lane >> 4) * 4 + e;
-                if (m >= M || n >= N) continue;
-                float v = acc[0][i][j][e];
-                if constexpr (GLU) {
-                    const float as = a_scale ? a_scale[m] : 1.f;
-                    const float g = v * (s0 ? as * s0[n] : 1.f) + (bias0 ? (float)bias0[n] : 0.f);
-                    const float u = acc[1][i][j][e] * (s1 ? as * s1[n] : 1.f) + (bias1 ? (float)bias1[n] : 0.f);
-                    if (p0) p0[m * ldp + n] = (TO)g;
-                    if (p1) p1[m * ldp + n] = (TO)u;
-                    v = act_of(g, act) * u;
+                if (m >= q.M || n >= q.F) continue;
+                float v[2];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    v[g] = acc[g][i][j][e] * (q.xs ? q.xs[m] * q.ws[g][n] : 1.f);
+                    if (q.b[g]) v[g] += (float)reinterpret_cast<const TO*>(q.b[g])[n];
+                    if (q.pre[g]) reinterpret_cast<TO*>(q.pre[g])[m * q.ldp + n] = (TO)v[g];
                 }
-                c[m * ldc + n] = (TO)v;
+                reinterpret_cast<TO*>(q.h)[m * q.ldh + n] = (TO)(act_of(v[0], q.act) * v[1]);
             }
 }
 
-// dg, du [M, F] (row stride F) from dh and the two projections; grid (ceil(F / 256), rows)
+// ---- the gradient -------------------------------------------------------------------------------------------------
+// The products of the gradient contract over F (dx) and over the rows (dWg, dWu), the matrix-core kernel over the unit
+// stride of both operands: so dg | du is laid out both ways round by the kernel that computes it, and the weights and x
+// are transposed.  All of it is zero-padded to whole K tiles of 64 in the workspace, which also takes care of sizes and
+// strides that the wide loads cannot read.
+constexpr int64_t up64(int64_t v) { return (v + 63) & ~(int64_t)63; }
+constexpr int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
+
+// 8 values of a row of `cols`, zeros behind its end; wide: 16-byte aligned rows
+template <typename T> struct vec8;
+template <> struct vec8<bf16> { typedef bf16x8 type; };
+template <> struct vec8<_Float16> { typedef h16x8 type; };
 template <typename T>
-__global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh, int64_t ldh, const T* __restrict__ gate, int64_t ldg,
-                                                       const T* __restrict__ up, int64_t ldu, T* __restrict__ dg,
-                                                       T* __restrict__ du, int M, int F, int act) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= F) return;
-    for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
-        float a, da;
-        act_grad((float)gate[m * ldg + c], act, a, da);
-        const float d = (float)dh[m * ldh + c];
-        dg[m * F + c] = (T)(d * (float)up[m * ldu + c] * da);
-        du[m * F + c] = (T)(d * a);
+__device__ __forceinline__ typename vec8<T>::type load8(const T* row, int c, int cols, bool wide) {
+    if (wide && c + 8 <= cols) return *reinterpret_cast<const typename vec8<T>::type*>(row + c);
+    typename vec8<T>::type v = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (c + j < cols) v[j] = row[c + j];
+    return v;
+}
+
+// A 64 x 64 tile in LDS, written by rows and read by columns: 16-byte chunks, the chunk index XORed with row / 8 so that the
+// eight rows a lane gathers a column chunk from and the lanes' neighbouring columns fall into different banks.
+template <typename T>
+__device__ __forceinline__ void tile_put(T* t, int row, int chunk, const typename vec8<T>::type& v) {
+    *reinterpret_cast<typename vec8<T>::type*>(t + row * 64 + ((chunk ^ (row >> 3)) << 3)) = v;
+}
+template <typename T>
+__device__ __forceinline__ typename vec8<T>::type tile_get_t(const T* t, int col, int rchunk) {      // rows 8 rchunk .. + 7 of a column
+    typename vec8<T>::type v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = t[(rchunk * 8 + j) * 64 + (((col >> 3) ^ rchunk) << 3) + (col & 7)];
+    return v;
+}
+
+// dst[c][r] = src[r][c], dst [cols_p, ld] with rows zero-padded from `rows` to rows_p (a multiple of 64) and zero rows from
+// cols to cols_p; grid (ceil(cols_p / 64), rows_p / 64)
+template <typename T>
+__device__ void transpose_tile(const T* __restrict__ src, int64_t ld_src, int rows, int cols, T* __restrict__ dst, int64_t ld_dst, int cols_p,
+                               int64_t r0, int c0, bool wide, T* tile) {
+    for (int i = threadIdx.x; i < 512; i += 256) {
+        const int r = i >> 3, ch = i & 7;
+        typename vec8<T>::type v = {};
+        if (r0 + r < rows) v = load8(src + (r0 + r) * ld_src, c0 + ch * 8, cols, wide);
+        tile_put(tile, r, ch, v);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 512; i += 256) {
+        const int c = i >> 3, ch = i & 7;
+        if (c0 + c < cols_p) *reinterpret_cast<typename vec8<T>::type*>(dst + (int64_t)(c0 + c) * ld_dst + r0 + ch * 8) = tile_get_t(tile, c, ch);
     }
 }
+struct Transposes {                 // up to three of them in one launch, one after the other in blockIdx.x
+    const void* src[3];
+    void* dst[3];
+    int64_t ld_src[3], ld_dst[3];
+    int rows[3], cols[3], tiles[3], col_tiles[3];
+};
 template <typename T>
-__global__ __launch_bounds__(256) void bias_grad_kernel(const T* __restrict__ dg, const T* __restrict__ du, T* __restrict__ dbg,
-                                                        T* __restrict__ dbu, int M, int F) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= F) return;
-    const T* p = blockIdx.y ? du : dg;
-    float s = 0.f;
-    for (int64_t m = 0; m < M; ++m) s += (float)p[m * F + c];
-    (blockIdx.y ? dbu : dbg)[c] = (T)s;
+__global__ __launch_bounds__(256) void transpose_kernel(Transposes t, int cols_p) {
+    __shared__ __attribute__((aligned(16))) T tile[64 * 64];
+    int b = blockIdx.x, i = 0;
+    while (i < 2 && b >= t.tiles[i]) b -= t.tiles[i++];
+    const T* src = (const T*)t.src[i];
+    const bool wide = ((uintptr_t)src & 15) == 0 && t.ld_src[i] % 8 == 0;
+    transpose_tile<T>(src, t.ld_src[i], t.rows[i], t.cols[i], (T*)t.dst[i], t.ld_dst[i], cols_p, (int64_t)(b / t.col_tiles[i]) * 64,
+                      b % t.col_tiles[i] * 64, wide, tile);
 }
 
-bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// dg | du as [M, 2 Fp] and as [2 Fp, Mp], both zero-padded; colsum: the tile's column sums [row tile][2 Fp] (or null).
+// Grid (Fp / 64, Mp / 64).  One read of dh, g, u; two writes of dg and du.
+template <typename T>
+__global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh, int64_t ldh, const T* __restrict__ gate, int64_t ldg,
+                                                       const T* __restrict__ up, int64_t ldu, T* __restrict__ dgu, T* __restrict__ dgut,
+                                                       float* __restrict__ colsum, int M, int F, int Fp, int Mp, int act, bool wide) {
+    typedef typename vec8<T>::type V;
+    __shared__ __attribute__((aligned(16))) T tg[64 * 64], tu[64 * 64];
+    __shared__ float cs[2][4][64];
+    const int64_t m0 = (int64_t)blockIdx.y * 64;
+    const int f0 = blockIdx.x * 64, ch = threadIdx.x & 7;
+    float sg[8] = {}, su[8] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = (threadIdx.x >> 3) + 32 * i;
+        const int64_t m = m0 + r;
+        V og = {}, ou = {};
+        if (m < M) {
+            const V d = load8(dh + m * ldh, f0 + ch * 8, F, wide), g = load8(gate + m * ldg, f0 + ch * 8, F, wide),
+                    u = load8(up + m * ldu, f0 + ch * 8, F, wide);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float a, da;
+                act_grad((float)g[j], act, a, da);
+                const float vg = (float)d[j] * (float)u[j] * da, vu = (float)d[j] * a;
+                const bool in = f0 + ch * 8 + j < F;
+                sg[j] += in ? vg : 0.f;
+                su[j] += in ? vu : 0.f;
+                og[j] = (T)(in ? vg : 0.f);
+                ou[j] = (T)(in ? vu : 0.f);
+            }
+            *reinterpret_cast<V*>(dgu + m * (2 * (int64_t)Fp) + f0 + ch * 8) = og;
+            *reinterpret_cast<V*>(dgu + m * (2 * (int64_t)Fp) + Fp + f0 + ch * 8) = ou;
+        }
+        tile_put(tg, r, ch, og);
+        tile_put(tu, r, ch, ou);
+    }
+    if (colsum) {       // over the 8 rows of a wave and pass, then over the waves, in a fixed order
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int o = 8; o < 64; o <<= 1) {
+                sg[j] += __shfl_xor(sg[j], o, 64);
+                su[j] += __shfl_xor(su[j], o, 64);
+            }
+            if ((threadIdx.x & 63) < 8) {
+                cs[0][threadIdx.x >> 6][ch * 8 + j] = sg[j];
+                cs[1][threadIdx.x >> 6][ch * 8 + j] = su[j];
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int f = (threadIdx.x >> 3) + 32 * i;
+        *reinterpret_cast<V*>(dgut + (int64_t)(f0 + f) * Mp + m0 + ch * 8) = tile_get_t(tg, f, ch);
+        *reinterpret_cast<V*>(dgut + (int64_t)(Fp + f0 + f) * Mp + m0 + ch * 8) = tile_get_t(tu, f, ch);
+    }
+    if (colsum && threadIdx.x < 128) {
+        const int w = threadIdx.x >> 6, c = threadIdx.x & 63;
+        colsum[(int64_t)blockIdx.y * (2 * Fp) + w * Fp + f0 + c] = (cs[w][0][c] + cs[w][1][c]) + (cs[w][2][c] + cs[w][3][c]);
+    }
+}
+// db = sum of the row tiles' column sums; grid (ceil(F / 64), 2), four lanes rows apart per column
+template <typename T>
+__global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ colsum, int tiles, int F, int Fp, T* __restrict__ dbg,
+                                                        T* __restrict__ dbu) {
+    __shared__ float red[4][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+    float s = 0.f;
+    if (c < F)
+        for (int t = q; t < tiles; t += 4) s += colsum[(int64_t)t * (2 * Fp) + blockIdx.y * Fp + c];
+    red[q][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (q == 0 && c < F) (blockIdx.y ? dbu : dbg)[c] = (T)((red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
+}
+// out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns
+template <typename T>
+__global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, int splits, T* __restrict__ out, int64_t M, int N, int Np) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int per = Np / 4;
+    if (i >= M * per) return;
+    const int64_t m = i / per;
+    const int n = (int)(i - m * per) * 4;
+    f32x4 s = *reinterpret_cast<const f32x4*>(part + m * Np + n);
+    for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + ((int64_t)k * M + m) * Np + n);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (n + j < N) out[m * N + n + j] = (T)s[j];
+}
 
-template <typename TI, typename TO, bool GLU>
-int any_gemm(Operand a, Operand b0, Operand a1, Operand b1, const float* as, const float* s0, const float* s1, const void* bias0,
-             const void* bias1, void* c, int64_t ldc, void* p0, void* p1, int64_t ldp, int M, int N, int K, int act, hipStream_t st) {
-    const dim3 grid((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
-    FP_REQUIRE(grid.y < 65536);
-    any_gemm_kernel<TI, TO, GLU><<<grid, dim3(256), 0, st>>>(a, b0, a1, b1, as, s0, s1, (const TO*)bias0, (const TO*)bias1, (TO*)c, ldc,
-                                                             (TO*)p0, (TO*)p1, ldp, M, N, K, act);
+// How a product [M, N] over K (a multiple of 64) is cut: whole (0 parts: straight to 16 bits) where its 256 x 256 tiles fill
+// half the chip or more, else into parts of K of at least 4 tiles until they do.  N % 8 != 0: always through 32 bits (the
+// 16-bit stores are 16 bytes wide).
+struct Cut {
+    int splits, ks_per;
+};
+Cut cut(int64_t M, int N, int K) {
+    const int64_t tiles = (M + 255) / 256 * ((N + 255) / 256);
+    const int nk = K / 64;
+    int64_t s = tiles >= 128 ? 1 : 256 / tiles;
+    if (s > nk / 4) s = nk / 4;
+    if (s < 1) s = 1;
+    const int per = (int)((nk + s - 1) / s);
+    const int splits = (nk + per - 1) / per;
+    return {splits == 1 && N % 8 == 0 ? 0 : splits, per};
+}
+int64_t cut_bytes(int64_t M, int N, int K) { return (int64_t)cut(M, N, K).splits * M * up8(N) * 4; }
+
+struct GradSpace {                  // byte offsets in the workspace, each a multiple of 256
+    int64_t dgu, dgut, wt, xt, colsum, parts, end;
+};
+GradSpace grad_space(int64_t M, int64_t F, int64_t K) {
+    const int64_t Fp = up64(F), Mp = up64(M), Kp = up8(K);
+    GradSpace g;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t o = at;
+        at += (bytes + 255) & ~(int64_t)255;
+        return o;
+    };
+    g.dgu = take(M * 2 * Fp * 2);
+    g.dgut = take(2 * Fp * Mp * 2);
+    g.wt = take(Kp * 2 * Fp * 2);
+    g.xt = take(Kp * Mp * 2);
+    g.colsum = take(Mp / 64 * 2 * Fp * 4);
+    const int64_t a = cut_bytes(M, (int)K, (int)(2 * Fp)), b = cut_bytes(F, (int)K, (int)Mp), c = cut_bytes(2 * F, (int)K, (int)Mp);
+    g.parts = take(a > b ? (a > c ? a : c) : (b > c ? b : c));
+    g.end = at;
+    return g;
+}
+
+// out [M, N] = a [M, K] . w [up8(N), K]^T, K a multiple of 64 and everything in the workspace's layout
+template <typename T>
+int product(const T* a, int64_t lda, const T* w, int64_t ldw, T* out, int M, int N, int K, float* parts, hipStream_t st) {
+    constexpr int type = sizeof(T) == 2 && __is_same(T, bf16) ? FF_BF16 : FF_F16;
+    const Cut c = cut(M, N, K);
+    if (c.splits == 0)
+        return (type == FF_BF16 ? fp_gemm_bf16 : fp_gemm_f16)(a, lda, nullptr, 0, w, ldw, nullptr, out, N, M, N, K, 0, 0, nullptr, 0, nullptr, st);
+    const int Np = (int)up8(N);
+    if (int rc = fpi_gemm_parts(type, a, lda, w, ldw, parts, M, Np, K, c.splits, c.ks_per, st)) return rc;
+    add_parts_kernel<T><<<dim3((unsigned)(((int64_t)M * (Np / 4) + 255) / 256)), dim3(256), 0, st>>>(parts, c.splits, out, M, N, Np);
     FP_CHECK_LAUNCH();
     return 0;
 }
+
+constexpr int LIMIT = (1 << 21) - 64;      // M, F, K of the gradient: 2 Fp and Mp stay below gemm_w4.h's limit of 2^22 for a row stride
+
+bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename TI, typename TO>
 int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64_t ldwg, const float* gs, const void* wu, int64_t ldwu,
@@ -165,35 +347,57 @@ int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64
     FP_REQUIRE(sizeof(TI) == 1 || (aligned2(x) && aligned2(wg) && aligned2(wu) && aligned2(h) && aligned2(bg) && aligned2(bu) &&
                                    aligned2(gate) && aligned2(up)));
     if (M == 0) return 0;
-    return any_gemm<TI, TO, true>({x, ldx, 1}, {wg, ldwg, 1}, {nullptr, 0, 0}, {wu, ldwu, 1}, xs, gs, us, bg, bu, h, ldh, gate, up, ldp,
-                                  M, F, K, act, (hipStream_t)stream);
+    constexpr int type = sizeof(TI) == 1 ? FF_E4M3 : __is_same(TI, bf16) ? FF_BF16 : FF_F16;
+    // the matrix-core kernel's loads and stores are 16 bytes wide and its K tiles whole
+    constexpr int V = 16 / (int)sizeof(TI);
+    const bool wide = aligned16(x) && aligned16(wg) && aligned16(wu) && aligned16(h) && aligned16(gate) && aligned16(up) &&
+                      ((uintptr_t)bg & 7) == 0 && ((uintptr_t)bu & 7) == 0 && ldx % V == 0 && ldwg % V == 0 && ldwu % V == 0 &&
+                      ldh % 8 == 0 && (!gate || ldp % 8 == 0) && K % (8 * V) == 0 && F % 8 == 0;
+    constexpr int64_t FAR = int64_t(1) << 22;             // gemm_w4.h: 32-bit offsets within a tile
+    if (wide && ldx < FAR && ldwg < FAR && ldwu < FAR)
+        return fpi_glu(type, x, ldx, xs, wg, ldwg, gs, wu, ldwu, us, bg, bu, h, ldh, gate, up, ldp, M, F, K, act, (hipStream_t)stream);
+    const GluCall q{x, ldx, xs, {wg, wu}, {ldwg, ldwu}, {gs, us}, {bg, bu}, h, ldh, {gate, up}, ldp, M, F, K, act};
+    const dim3 grid((unsigned)((F + 63) / 64), (unsigned)((M + 63) / 64));
+    FP_REQUIRE(grid.y < 65536);
+    glu_any_kernel<TI, TO><<<grid, dim3(256), 0, (hipStream_t)stream>>>(q);
+    FP_CHECK_LAUNCH();
+    return 0;
 }
 
 template <typename T>
 int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
-                   const void* gate, int64_t ldg, const void* up, int64_t ldu, void* dx, int64_t lddx, void* dwg, void* dwu,
-                   int64_t lddw, void* dbg, void* dbu, int M, int F, int K, int act, void* ws, int64_t ws_bytes, void* stream) {
+                   const void* gate, int64_t ldg, const void* up, int64_t ldu, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
+                   int M, int F, int K, int act, void* ws, int64_t ws_bytes, void* stream) {
     FP_REQUIRE(dh && x && wg && wu && gate && up && dx && dwg && dwu && !dbg == !dbu && (act == 0 || act == 1));
-    FP_REQUIRE(aligned2(dh) && aligned2(x) && aligned2(wg) && aligned2(wu) && aligned2(gate) && aligned2(up) && aligned2(dx) &&
-               aligned2(dwg) && aligned2(dwu) && aligned2(dbg) && aligned2(dbu));
-    FP_REQUIRE(M > 0 && F > 0 && K > 0 && ldh >= 0 && ldx >= 0 && ldg >= 0 && ldu >= 0 && ldwg >= K && ldwu >= K && lddx >= K && lddw >= K);
-    FP_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= fp_gated_ff_backward_workspace_bytes(M, F, K));
+    FP_REQUIRE(aligned2(dh) && aligned2(x) && aligned2(wg) && aligned2(wu) && aligned2(gate) && aligned2(up) && aligned2(dbg) && aligned2(dbu));
+    FP_REQUIRE(aligned16(dx) && aligned16(dwg) && (K % 8 != 0 ? aligned2(dwu) : aligned16(dwu)));
+    FP_REQUIRE(M > 0 && F > 0 && K > 0 && ldh >= 0 && ldx >= 0 && ldg >= 0 && ldu >= 0 && ldwg >= K && ldwu >= K);
+    FP_REQUIRE(M <= LIMIT && F <= LIMIT && K <= LIMIT);
+    FP_REQUIRE(ws && aligned16(ws) && ws_bytes >= fp_gated_ff_backward_workspace_bytes(M, F, K));
     hipStream_t st = (hipStream_t)stream;
-    T* dg = (T*)ws;
-    T* du = dg + (int64_t)M * F;
-    glu_grad_kernel<T><<<dim3((unsigned)((F + 255) / 256), (unsigned)(M < 16384 ? M : 16384)), dim3(256), 0, st>>>(
-        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dg, du, M, F, act);
+    const GradSpace g = grad_space(M, F, K);
+    const int Fp = (int)up64(F), Mp = (int)up64(M), Kp = (int)up8(K), ktiles = (K + 63) / 64;
+    char* base = (char*)ws;
+    T *dgu = (T*)(base + g.dgu), *dgut = (T*)(base + g.dgut), *wt = (T*)(base + g.wt), *xt = (T*)(base + g.xt);
+    float *colsum = dbg ? (float*)(base + g.colsum) : nullptr, *parts = (float*)(base + g.parts);
+    const bool wide = aligned16(dh) && aligned16(gate) && aligned16(up) && ldh % 8 == 0 && ldg % 8 == 0 && ldu % 8 == 0;
+    glu_grad_kernel<T><<<dim3((unsigned)(Fp / 64), (unsigned)(Mp / 64)), dim3(256), 0, st>>>(
+        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, Fp, Mp, act, wide);
     FP_CHECK_LAUNCH();
-    const Operand none{nullptr, 0, 0};
-    if (int rc = any_gemm<T, T, false>({dg, F, 1}, {wg, 1, ldwg}, {du, F, 1}, {wu, 1, ldwu}, nullptr, nullptr, nullptr, nullptr, nullptr,
-                                       dx, lddx, nullptr, nullptr, 0, M, K, F, 0, st))
-        return rc;
-    for (int i = 0; i < 2; ++i)
-        if (int rc = any_gemm<T, T, false>({i ? du : dg, 1, F}, {x, 1, ldx}, none, none, nullptr, nullptr, nullptr, nullptr, nullptr,
-                                           i ? dwu : dwg, lddw, nullptr, nullptr, 0, F, K, M, 0, st))
-            return rc;
+    const Transposes t{{wg, wu, x},   {wt, wt + Fp, xt},  {ldwg, ldwu, ldx},
+                       {2 * Fp, 2 * Fp, Mp}, {F, F, M}, {K, K, K}, {Fp / 64 * ktiles, Fp / 64 * ktiles, Mp / 64 * ktiles}, {ktiles, ktiles, ktiles}};
+    transpose_kernel<T><<<dim3((unsigned)(t.tiles[0] + t.tiles[1] + t.tiles[2])), dim3(256), 0, st>>>(t, Kp);
+    FP_CHECK_LAUNCH();
+    if (int rc = product<T>(dgu, 2 * Fp, wt, 2 * Fp, (T*)dx, M, K, 2 * Fp, parts, st)) return rc;
+    // (dWg over dWu in one product where they are the halves of one matrix)
+    if (Fp == F && (T*)dwu == (T*)dwg + (int64_t)F * K) {
+        if (int rc = product<T>(dgut, Mp, xt, Mp, (T*)dwg, 2 * F, K, Mp, parts, st)) return rc;
+    } else {
+        if (int rc = product<T>(dgut, Mp, xt, Mp, (T*)dwg, F, K, Mp, parts, st)) return rc;
+        if (int rc = product<T>(dgut + (int64_t)Fp * Mp, Mp, xt, Mp, (T*)dwu, F, K, Mp, parts, st)) return rc;
+    }
     if (dbg) {
-        bias_grad_kernel<T><<<dim3((unsigned)((F + 255) / 256), 2), dim3(256), 0, st>>>(dg, du, (T*)dbg, (T*)dbu, M, F);
+        bias_grad_kernel<T><<<dim3((unsigned)(Fp / 64), 2), dim3(256), 0, st>>>(colsum, Mp / 64, F, Fp, (T*)dbg, (T*)dbu);
         FP_CHECK_LAUNCH();
     }
     return 0;
@@ -227,22 +431,22 @@ extern "C" int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, 
 }
 
 extern "C" int64_t fp_gated_ff_backward_workspace_bytes(int M, int F, int K) {
-    if (M <= 0 || F <= 0 || K <= 0) return 0;
-    return ((int64_t)M * F * 4 + 15) & ~(int64_t)15;
+    if (M <= 0 || F <= 0 || K <= 0 || M > LIMIT || F > LIMIT || K > LIMIT) return 0;
+    return grad_space(M, F, K).end;
 }
 
 extern "C" int fp_gated_ff_backward_bf16(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
                                          const void* w_up, int64_t ldwu, const void* gate, int64_t ldg, const void* up, int64_t ldu,
-                                         void* dx, int64_t lddx, void* dw_gate, void* dw_up, int64_t lddw, void* db_gate, void* db_up,
-                                         int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream) {
-    return ff_grad_launch<bf16>(dh, ldh, x, ldx, w_gate, ldwg, w_up, ldwu, gate, ldg, up, ldu, dx, lddx, dw_gate, dw_up, lddw, db_gate,
-                                db_up, M, F, K, act, workspace, workspace_bytes, stream);
+                                         void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int F, int K, int act,
+                                         void* workspace, int64_t workspace_bytes, void* stream) {
+    return ff_grad_launch<bf16>(dh, ldh, x, ldx, w_gate, ldwg, w_up, ldwu, gate, ldg, up, ldu, dx, dw_gate, dw_up, db_gate, db_up, M, F, K,
+                                act, workspace, workspace_bytes, stream);
 }
 
 extern "C" int fp_gated_ff_backward_f16(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
                                         const void* w_up, int64_t ldwu, const void* gate, int64_t ldg, const void* up, int64_t ldu,
-                                        void* dx, int64_t lddx, void* dw_gate, void* dw_up, int64_t lddw, void* db_gate, void* db_up,
-                                        int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream) {
-    return ff_grad_launch<_Float16>(dh, ldh, x, ldx, w_gate, ldwg, w_up, ldwu, gate, ldg, up, ldu, dx, lddx, dw_gate, dw_up, lddw,
-                                    db_gate, db_up, M, F, K, act, workspace, workspace_bytes, stream);
+                                        void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int F, int K, int act,
+                                        void* workspace, int64_t workspace_bytes, void* stream) {
+    return ff_grad_launch<_Float16>(dh, ldh, x, ldx, w_gate, ldwg, w_up, ldwu, gate, ldg, up, ldu, dx, dw_gate, dw_up, db_gate, db_up, M,
+                                    F, K, act, workspace, workspace_bytes, stream);
 }

@@ -1,0 +1,48 @@
+// K13's products on the matrix cores: instances of gemm_w4.h (see GluArgs and SplitArgs there).
+#include "gated_ff.h"
+#include "gemm_w4.h"
+
+using namespace fp_gemm;
+
+int fpi_glu(int type, const void* x, int64_t ldx, const float* xs, const void* wg, int64_t ldwg, const float* gs, const void* wu,
+            int64_t ldwu, const float* us, const void* bg, const void* bu, void* h, int64_t ldh, void* gate, void* up, int64_t ldp,
+            int M, int F, int K, int act, hipStream_t st) {
+    const GluArgs glu{wu, bu, ldwu, us, gate, up, ldp, act};
+    const int ntm = (M + BM - 1) / BM;
+    FP_REQUIRE((int64_t)ntm * ((F + 63) / 64) < (1ll << 31));
+    const ConvGeom cg{};
+    // fewer 256 x 128 tiles than half the CUs: 256 x 64 ones, twice as many at about 0.6 of the time each (as K5)
+    const bool narrow = (int64_t)ntm * ((F + 127) / 128) <= persistent_grid() / 2;
+#define FP_GLU(T, TO, NT, KEEP)                                                                                                   \
+    return launch_w4<T, 0, 0, TO, NT, 0, 0, 0, 1, KEEP>(x, ldx, 0, K, wg, ldwg, bg, h, ldh, M, F, K, 0, nullptr, 0, nullptr, cg, st, \
+                                                        xs, gs, QkNormArgs{}, Rows2{}, glu)
+    if (type == FF_E4M3) FP_GLU(fp8e4, bf16, 8, 0);
+    if (type == FF_BF16) {
+        if (gate) {
+            if (narrow) FP_GLU(bf16, bf16, 4, 1);
+            FP_GLU(bf16, bf16, 8, 1);
+        }
+        if (narrow) FP_GLU(bf16, bf16, 4, 0);
+        FP_GLU(bf16, bf16, 8, 0);
+    }
+    if (gate) {
+        if (narrow) FP_GLU(_Float16, _Float16, 4, 1);
+        FP_GLU(_Float16, _Float16, 8, 1);
+    }
+    if (narrow) FP_GLU(_Float16, _Float16, 4, 0);
+    FP_GLU(_Float16, _Float16, 8, 0);
+#undef FP_GLU
+}
+
+int fpi_gemm_parts(int type, const void* a, int64_t lda, const void* w, int64_t ldw, float* part, int M, int N, int K, int splits,
+                   int ks_per, hipStream_t st) {
+    const SplitArgs sp{splits, ks_per};
+    const ConvGeom cg{};
+    FP_REQUIRE(splits > 0 && ks_per > 0 && (int64_t)(splits - 1) * ks_per < K / BK && (int64_t)splits * ks_per >= K / BK);
+    FP_REQUIRE((int64_t)((M + BM - 1) / BM) * ((N + BN - 1) / BN) * splits < (1ll << 31));
+    if (type == FF_BF16)
+        return launch_w4<bf16, 0, 0, float, 8, 0, 0, 0, 0, 0, 1>(a, lda, 0, K, w, ldw, nullptr, part, N, M, N, K, 0, nullptr, 0, nullptr,
+                                                                cg, st, nullptr, nullptr, QkNormArgs{}, Rows2{}, GluArgs{}, sp);
+    return launch_w4<_Float16, 0, 0, float, 8, 0, 0, 0, 0, 0, 1>(a, lda, 0, K, w, ldw, nullptr, part, N, M, N, K, 0, nullptr, 0, nullptr,
+                                                                cg, st, nullptr, nullptr, QkNormArgs{}, Rows2{}, GluArgs{}, sp);
+}

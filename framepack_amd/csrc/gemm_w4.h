@@ -143,7 +143,34 @@ struct Rows2 {
     const void *w2, *bias2, *gate2;
     int m_split;
 };
-template <typename T, typename TO, int EPI, int AMODE, int NT = 8, int QKN = 0, int TALL = 0, int GRP = 0>
+// GLU (the gated feed-forward block, gated_ff.hip): h = act(A . W^T + bias) * (A . w2^T + bias2).  The workgroup's W tile
+// holds, per wave column, 8 NT rows of W and below them the same 8 NT rows of w2, so both projections of an output element
+// are accumulators of one lane (column tiles ni and ni + NT / 2) and the epilogue multiplies them in registers; the output
+// tile is 256 x (16 NT).  A wave stages its LDS rows from one of the two matrices only (wave & 1), whose base and row
+// stride stay in scalar registers: the main loop is the dense one.  KEEP: both projections are written out as well.
+struct GluArgs {
+    const void *w2, *bias2;
+    int64_t ldw2;
+    const float* w_scale2;
+    void *pre0, *pre1;                          // KEEP: A . W^T + bias and A . w2^T + bias2, row stride ldp
+    int64_t ldp;
+    int act;                                    // 0: SiLU, 1: tanh-GELU
+};
+// act(v) = v / (1 + 2^-z),  z = log2(e) v (SiLU) or 2 log2(e) sqrt(2/pi) (v + 0.044715 v^3) (tanh-GELU): one expression with
+// two constants.  v is clamped in z only (past 1e4 the quotient has long run into 0 or v), so that v^2 stays finite.
+__device__ __forceinline__ float glu_act(float v, float c0, float c1) {
+    const float t = __builtin_amdgcn_fmed3f(v, -1e4f, 1e4f);
+    return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-t * __builtin_fmaf(t * t, c1, c0)));
+}
+__device__ __forceinline__ float glu_c0(int act) { return 1.4426950408889634f * (act ? 2.f * 0.7978845608028654f : 1.f); }
+__device__ __forceinline__ float glu_c1(int act) { return act ? 1.4426950408889634f * 2.f * 0.7978845608028654f * 0.044715f : 0.f; }
+// SPLIT > 0 (gated_ff.hip's dx: few output tiles, a long K): the K tiles are dealt to `splits` workgroups per output tile in
+// runs of ks_per, and part s goes to rows [s M, (s + 1) M) of the fp32 output; the caller adds them up.
+struct SplitArgs {
+    int splits, ks_per;
+};
+template <typename T, typename TO, int EPI, int AMODE, int NT = 8, int QKN = 0, int TALL = 0, int GRP = 0, int GLU = 0,
+          int KEEP = 0, int SPLIT = 0>
 __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A, int64_t lda, int64_t a2_delta,
                                                          int k1, const T* __restrict__ W, int64_t ldw,
                                                          const TO* __restrict__ bias_, TO* __restrict__ C,
@@ -151,7 +178,10 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                                                          const TO* __restrict__ R, int64_t ldr,
                                                          const TO* __restrict__ gate_, int ntm, int ntn, ConvGeom cg,
                                                          const float* __restrict__ a_scale,
-                                                         const float* __restrict__ w_scale, QkNormArgs qk, Rows2 r2) {
+                                                         const float* __restrict__ w_scale, QkNormArgs qk, Rows2 r2,
+                                                         GluArgs glu, SplitArgs sp) {
+    static_assert(!GLU || (AMODE == 0 && !TALL && !QKN && !GRP && EPI == 0 && sizeof(TO) == 2 && NT >= 4), "gated block: the dense tile");
+    static_assert(!SPLIT || (AMODE == 0 && !TALL && !QKN && !GRP && !GLU && EPI == 0 && sizeof(TO) == 4), "parts of K: fp32 out");
     static_assert(!GRP || (AMODE == 0 && !TALL && !QKN && NT == 8 && sizeof(T) == 2), "row segments: the dense 16-bit 256 x 256 tile");
     typedef i32x4 frag_t;
     typedef TO Tx4 __attribute__((ext_vector_type(4)));
@@ -212,8 +242,14 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     // tile order: XCD-contiguous, grouped 8 row-tiles tall so that co-running tiles share A and W panels.  The
     // workgroup is persistent: it takes tiles vb = blockIdx.x, + gridDim.x, ... (gridDim.x is a multiple of 8 or
     // the whole tile count, so vb & 7 stays this workgroup's XCD).
-    const int ntiles = ntm * ntn;
-    constexpr int CW = NT * 16;     // columns per wave column
+    const int ntiles = ntm * ntn * (SPLIT ? sp.splits : 1);
+    constexpr int CW = NT * 16;     // W rows per wave column
+    constexpr int TBN = TALL || GLU ? CW : 2 * CW;                   // output columns of a tile
+    // GLU: output columns of a wave, 16-B chunks of its rows, rows per store instruction; the epilogue's stores of a tile
+    constexpr int OCW = CW / 2, CPR = OCW / 8, RPI = CPR > 0 ? 64 / CPR : 64;
+    constexpr int N_STORES = GLU ? 16 / RPI * 8 * (KEEP ? 3 : 1) : 32;
+    int part = 0;                   // SPLIT: which run of K tiles
+    int nk = K / BKE;
     unsigned a_rd[2], w_rd[2];  // fragment read addresses (below)
     const int fr = lane & 15, fq = lane >> 4;
     constexpr unsigned SECOND = SCALED ? 16u : 64u;
@@ -221,7 +257,12 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     auto setup = [&](int vb) __attribute__((always_inline)) {
         // ConvGeom::gm: gm > 0: gm row tiles x all column tiles per group; gm < 0: -gm column tiles x all row tiles
         const int GM = cg.gm != 0 ? abs(cg.gm) : 8;
-        const int wid = xcd_remap(vb, ntiles);
+        int wid = xcd_remap(vb, ntiles);
+        if constexpr (SPLIT) {
+            part = wid / (ntm * ntn);
+            wid -= part * (ntm * ntn);
+            nk = min(sp.ks_per, K / BKE - part * sp.ks_per);
+        }
         const int nmaj = cg.gm < 0 ? ntn : ntm, nmin = cg.gm < 0 ? ntm : ntn;
         const int per_group = GM * nmin;
         const int group = wid / per_group, in_group = wid % per_group;
@@ -243,7 +284,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             m_end = second ? M : r2.m_split;
             w_seg = second ? reinterpret_cast<const T*>(r2.w2) : W;
         }
-        n0 = tn * (TALL ? CW : 2 * CW);
+        n0 = tn * TBN;
         int lo_vox = 0;                             // AMODE 1: first voxel of the frame the tile's earliest tap reads (uniform)
         if (AMODE == 1) {
             const int tc = (m0 / (cg.Wo * cg.Ho)) << cg.dt, x = max(tc - 2, 0);
@@ -280,14 +321,22 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int wrw = wrow0[j] + prow;
-            pw[j] = (unsigned)(min(n0 + wrw, N - 1) - n0) * (unsigned)(ldw * sizeof(T)) + (pch ^ ((wrw >> 1) & 7)) * 16;
+            // GLU: the wave's WPW pieces are the rows of wave column wave >> 1 of one of the two matrices
+            const int col = GLU ? (wave >> 1) * (CW / 2) + j * 8 + prow : wrw;
+            pw[j] = (unsigned)(min(n0 + col, N - 1) - n0) * (unsigned)((GLU && (wave & 1) ? glu.ldw2 : ldw) * sizeof(T)) +
+                    (pch ^ ((wrw >> 1) & 7)) * 16;
         }
         abase = AMODE == 1 ? reinterpret_cast<const char*>(A) + ((int64_t)lo_vox << (cg.lcin + LOG2_TB))
                            : reinterpret_cast<const char*>(A + (int64_t)m0 * lda);
         wbase = reinterpret_cast<const char*>(w_seg + (int64_t)n0 * ldw);
-
+        if constexpr (GLU) {
+            if (wave & 1) wbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(glu.w2) + (int64_t)n0 * glu.ldw2);
+        }
+        if constexpr (SPLIT) {
+            abase += (int64_t)part * sp.ks_per * 128;
+            wbase += (int64_t)part * sp.ks_per * 128;
+        }
     };
-    const int nk = K / BKE;
     // AMODE 1: a K tile is one tap x 64 or 128 channels, and with Cin >= 2 K tiles per tap (the launcher sends narrower
     // inputs to the 8-wave kernel) the tiles 2 i and 2 i + 1 share their tap: the piece's source offset is worked out
     // at the EVEN tile and kept for the odd one (poff), which halves the gather's vector instructions - a lone wave per
@@ -495,14 +544,14 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         }
     };
     auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
-    // relaxed: the 32 output stores of the previous tile may still be in flight behind the loads this phase needs
-    // (memory operations retire in order), so the count that guarantees the loads is 16 + 32.
+    // relaxed: the N_STORES output stores of the previous tile may still be in flight behind the loads this phase needs
+    // (memory operations retire in order), so the count that guarantees the loads is 16 + N_STORES (or less).
     // PZC (fp8 only): ZC of the PREVIOUS phase, whose held-back tiles this phase issues (in the 16-bit loop the
     // held-back groups are second K steps and never start a tile)
     auto phase = [&](auto BUF, auto P, int t, auto HAVE_PREV, auto ZC, bool relaxed, auto PZC) __attribute__((always_inline)) {
         // younger than the unit a phase needs are always 2 APW + WPW pieces (APW of A-h0, APW of A-h1, WPW of W)
-        static_assert(2 * APW + WPW + 32 <= 63, "vmcnt is a 6-bit counter");
-        if (relaxed) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * APW + WPW + 32) : "memory");
+        constexpr int LATE = 2 * APW + WPW + N_STORES;        // (vmcnt is a 6-bit counter)
+        if (relaxed) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATE < 63 ? LATE : 63) : "memory");
         else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * APW + WPW) : "memory");
         __builtin_amdgcn_s_barrier();
         fence();
@@ -591,7 +640,74 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             if (gcol < N && m < M) rpre[mi & 1][i] = *reinterpret_cast<const Tx8*>(R + (int64_t)m * ldr + gcol);
         }
     };
-    auto epilogue = [&](int em0, int en0, int ecw) __attribute__((always_inline)) {
+    // GLU: lane (fr, fq) holds, for ni < NT / 2, both projections of row em0 + wr*128 + mi*16 + fr, columns en0 + wc * OCW +
+    // ni*16 + 4 fq + (0..3).  Rows leave through the wave's stage as below, OCW columns (2 OCW bytes) a row; KEEP: three images.
+    auto glu_epilogue = [&](int em0, int en0) __attribute__((always_inline)) {
+        unsigned stage_off = 2 * BUF_BYTES + wave * 8192;
+        asm volatile("" : "+v"(stage_off));
+        unsigned char* stage = smem + stage_off;
+        const int el = opaque_lane();
+        const int fr = el & 15, fq = el >> 4;
+        const int nb = en0 + wc * OCW + 4 * fq;
+        Tx4 bv[2][NT / 2];
+        f32x4 ws[2][NT / 2];
+#pragma unroll
+        for (int ni = 0; ni < NT / 2; ++ni) {
+            const int n = min(nb + ni * 16, N - 4);
+            bv[0][ni] = bv[1][ni] = Tx4{0, 0, 0, 0};
+            if (bias_) {
+                bv[0][ni] = *reinterpret_cast<const Tx4*>(bias_ + n);
+                bv[1][ni] = *reinterpret_cast<const Tx4*>(reinterpret_cast<const TO*>(glu.bias2) + n);
+            }
+            if (SCALED) {
+                ws[0][ni] = *reinterpret_cast<const f32x4*>(w_scale + n);
+                ws[1][ni] = *reinterpret_cast<const f32x4*>(glu.w_scale2 + n);
+            }
+        }
+        const float c0 = glu_c0(glu.act), c1 = glu_c1(glu.act);
+        const int lrow = el / CPR, lchk = el % CPR;
+        const int gcol = en0 + wc * OCW + lchk * 8;
+        static_for<8>([&](auto MI_) __attribute__((always_inline)) {
+            constexpr int mi = MI_;
+            constexpr int IMG = 16 * OCW * 2;                  // bytes of one image
+            unsigned char* sb = stage + (KEEP ? 0 : (mi & 1) * 4096);
+            const int mrow0 = em0 + wr * 128 + mi * 16;
+            if (mrow0 >= M) return;                            // wave-uniform
+            const float as = SCALED ? a_scale[min(mrow0 + fr, M - 1)] : 1.f;
+            static_for<NT / 2>([&](auto NI_) __attribute__((always_inline)) {
+                constexpr int ni = NI_;
+                unsigned char* sp_ = sb + fr * (OCW * 2) + ((((ni * 2) + (fq >> 1)) ^ (fr & (CPR - 1))) << 4) + (fq & 1) * 8;
+                const f32x4 ag = acc_read<(mi * 8 + ni) * 4>();
+                const f32x4 au = acc_read<(mi * 8 + ni + NT / 2) * 4>();
+                Tx4 o, og, ou;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float g = (SCALED ? ag[j] * (as * ws[0][ni][j]) : ag[j]) + (float)bv[0][ni][j];
+                    const float u = (SCALED ? au[j] * (as * ws[1][ni][j]) : au[j]) + (float)bv[1][ni][j];
+                    o[j] = (TO)(glu_act(g, c0, c1) * u);
+                    og[j] = (TO)g;
+                    ou[j] = (TO)u;
+                }
+                *reinterpret_cast<Tx4*>(sp_) = o;
+                if (KEEP) {
+                    *reinterpret_cast<Tx4*>(sp_ + IMG) = og;
+                    *reinterpret_cast<Tx4*>(sp_ + 2 * IMG) = ou;
+                }
+            });
+#pragma unroll
+            for (int img = 0; img < (KEEP ? 3 : 1); ++img) {
+                TO* dst = img == 0 ? C : reinterpret_cast<TO*>(img == 1 ? glu.pre0 : glu.pre1);
+                const int64_t ld = img == 0 ? ldc : glu.ldp;
+#pragma unroll
+                for (int i = 0; i < 16 / RPI; ++i) {
+                    const int row = lrow + RPI * i;
+                    const Tx8 ov = *reinterpret_cast<const Tx8*>(sb + img * IMG + row * (OCW * 2) + ((lchk ^ (row & (CPR - 1))) << 4));
+                    if (gcol < N && mrow0 + row < M) *reinterpret_cast<Tx8*>(dst + (int64_t)(mrow0 + row) * ld + gcol) = ov;
+                }
+            }
+        });
+    };
+    auto epilogue = [&](int em0, int en0, int ecw, int epart) __attribute__((always_inline)) {
       const int M = seg_rows(em0);              // shadows the kernel's
       const bool second = GRP && em0 >= r2.m_split;
       const TO* const bias = second ? reinterpret_cast<const TO*>(r2.bias2) : bias_;
@@ -617,7 +733,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                 if constexpr (ni >= NT) return;
                 const int n = nb + ni * 16;
                 const f32x4 av = acc_read<(mi * 8 + ni) * 4>() + bv[ni];
-                if (mrow0 + fr < M && n < N) *reinterpret_cast<f32x4*>(C + (int64_t)(mrow0 + fr) * ldc + n) = av;
+                if (mrow0 + fr < M && n < N)
+                    *reinterpret_cast<f32x4*>(C + ((SPLIT ? (int64_t)epart * M : 0) + mrow0 + fr) * ldc + n) = av;
             });
         });
       } else {
@@ -764,7 +881,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     prologue();
     bool relaxed = false;
     for (;;) {
-        const int em0 = m0, en0 = n0;
+        const int em0 = m0, en0 = n0, epart = part;
         constexpr int ecw = CW;
         phase(ic<0>{}, ic<0>{}, 0, ic<0>{}, ic<1>{}, relaxed, ic<0>{});
         phase(ic<0>{}, ic<1>{}, 0, ic<1>{}, ic<1>{}, relaxed, ic<1>{});
@@ -814,7 +931,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         }
         fence();
         asm volatile("s_nop 15\ns_nop 15" ::: "memory");        // the last MFMAs retire before their tiles are read
-        epilogue(em0, en0, ecw);
+        if constexpr (GLU) glu_epilogue(em0, en0);
+        else epilogue(em0, en0, ecw, epart);
 #if defined(FP_PROBE_REG_LOAD)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         asm volatile("" ::"v"(probe_sink));
@@ -828,7 +946,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             for (int j = 0; j < APW; ++j) poff[1][j] = tap_off(1, j, 0);
         }
         // a ragged tile skips stores, so the relaxed count would not cover the loads: drain instead
-        if (em0 + TBM > seg_rows(em0) || en0 + (TALL ? CW : 2 * CW) > N) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (em0 + TBM > seg_rows(em0) || en0 + TBN > N) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         relaxed = true;
     }
 }
@@ -846,25 +964,27 @@ inline int persistent_grid() {
     return n;
 }
 
-template <typename T, int EPI, int AMODE, typename TO = T, int NT = 8, int QKN = 0, int TALL = 0, int GRP = 0>
+template <typename T, int EPI, int AMODE, typename TO = T, int NT = 8, int QKN = 0, int TALL = 0, int GRP = 0, int GLU = 0,
+          int KEEP = 0, int SPLIT = 0>
 int launch_w4(const void* a, int64_t lda, int64_t a2_delta, int k1, const void* w, int64_t ldw, const void* bias,
               void* c, int64_t ldc, int M, int N, int K, int gelu_from, const void* resid, int64_t ldr,
               const void* gate, const ConvGeom& cg, hipStream_t st, const float* a_scale = nullptr,
-              const float* w_scale = nullptr, const QkNormArgs& qk = QkNormArgs{}, const Rows2& r2 = Rows2{}) {
+              const float* w_scale = nullptr, const QkNormArgs& qk = QkNormArgs{}, const Rows2& r2 = Rows2{},
+              const GluArgs& glu = GluArgs{}, const SplitArgs& sp = SplitArgs{}) {
     // lane offsets inside a tile are 32-bit: 255 rows x the row stride in bytes has to fit
-    if (lda >= (int64_t(1) << 22) || ldw >= (int64_t(1) << 22)) return (int)hipErrorInvalidValue;
-    constexpr int TBM = TALL ? 2 * BM : BM, TBN = TALL ? 16 * NT : 32 * NT;
+    if (lda >= (int64_t(1) << 22) || ldw >= (int64_t(1) << 22) || glu.ldw2 >= (int64_t(1) << 22)) return (int)hipErrorInvalidValue;
+    constexpr int TBM = TALL ? 2 * BM : BM, TBN = TALL || GLU ? 16 * NT : 32 * NT;
     const int ntm = GRP ? (r2.m_split + TBM - 1) / TBM + (M - r2.m_split + TBM - 1) / TBM : (M + TBM - 1) / TBM;
     const int ntn = (N + TBN - 1) / TBN;
     // operand buffers + the epilogue's row stage (TALL: all 160 KiB are operand buffers, the stage lies inside them)
     constexpr int smem = TALL ? 5 * OP_BYTES : 2 * BUF_BYTES + 4 * 8192;
-    auto kern = gemm_w4_kernel<T, TO, EPI, AMODE, NT, QKN, TALL, GRP>;
+    auto kern = gemm_w4_kernel<T, TO, EPI, AMODE, NT, QKN, TALL, GRP, GLU, KEEP, SPLIT>;
     hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != hipSuccess) return (int)e;
-    kern<<<dim3((unsigned)min(ntm * ntn, persistent_grid())), dim3(256), smem, st>>>((const T*)a, lda, a2_delta, k1, (const T*)w, ldw,
+    kern<<<dim3((unsigned)min(ntm * ntn * (SPLIT ? sp.splits : 1), persistent_grid())), dim3(256), smem, st>>>((const T*)a, lda, a2_delta, k1, (const T*)w, ldw,
                                                               (const TO*)bias, (TO*)c, ldc, M, N, K, gelu_from,
                                                               (const TO*)resid, ldr, (const TO*)gate, ntm, ntn, cg,
-                                                              a_scale, w_scale, qk, r2);
+                                                              a_scale, w_scale, qk, r2, glu, sp);
     FP_CHECK_LAUNCH();
     return 0;
 }

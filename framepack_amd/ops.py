@@ -914,6 +914,5 @@ def gated_ff_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w
     ws = torch.empty((lib.fp_gated_ff_backward_workspace_bytes(M, F, K),), dtype=torch.uint8, device=x.device)
     name = "fp_gated_ff_backward_bf16" if x.dtype == BF16 else "fp_gated_ff_backward_f16"
     _lib.check(getattr(lib, name)(d2.data_ptr(), ldd, x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, p2.data_ptr(),
-                                  ldp, q2.data_ptr(), ldq, dx.data_ptr(), K, dw[:F].data_ptr(), dw[F:].data_ptr(), K,
-                                  _ptr(db[0]), _ptr(db[1]), M, F, K, act, ws.data_ptr(), ws.numel(), _stream(x)), name)
+                                  ldp, q2.data_ptr(), ldq, dx.data_ptr(), dw.data_ptr(), dw[F:].data_ptr(), _ptr(db[0]), _ptr(db[1]), M, F, K, act, ws.data_ptr(), ws.numel(), _stream(x)), name)
     return dx, dw[:F], dw[F:], db[0], db[1]

@@ -143,7 +143,7 @@ def test_the_library_refuses_without_launching():
     for i, v in ((0, None), (2, None), (5, None), (8, None), (1, K + 8), (4, K + 8), (7, K + 8), (0, p + 8), (3, p + 8), (6, p + 8),
                  (11, p + 8), (12, F + 4), (14, 12), (15, 64), (5, p + 4), (9, p + 2), (9, None), (16, -1)):
         refused("fp_gated_ff_fp8", *[v if j == i else t for j, t in enumerate(ok)])
-    ok = [p, F, p, K, p, K, p, K, p, F, p, F, p, K, p, p, K, p, p, n, F, K, 0, p, 1 << 30, None]
-    for i, v in ((0, None), (2, None), (4, None), (8, None), (12, None), (14, None), (17, None), (13, K - 1), (16, K - 1), (19, 0),
-                 (20, 0), (21, 0), (22, 3), (23, None), (24, 16)):
+    ok = [p, F, p, K, p, K, p, K, p, F, p, F, p, p, p, p, p, n, F, K, 0, p, 1 << 30, None]
+    for i, v in ((0, None), (2, None), (4, None), (8, None), (12, None), (13, None), (15, None), (5, K - 1), (7, K - 1), (12, p + 8),
+                 (13, p + 2), (14, p + 2), (17, 0), (18, 0), (19, 0), (17, 1 << 21), (20, 3), (21, None), (21, p + 8), (22, 16)):
         refused("fp_gated_ff_backward_f16", *[v if j == i else t for j, t in enumerate(ok)])
