@@ -30,17 +30,152 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     return v;
 }
 
-// y / scale to e4m3: the quotient by one Newton step on y * (1 / scale), so that it rounds as a division does
-__device__ __forceinline__ unsigned char to_e4m3(float y, float scale, float inv) {
+// y / scale by one Newton step on y * (1 / scale), so that it rounds as a division does
+__device__ __forceinline__ float divide(float y, float scale, float inv) {
     const float q = y * inv;
-    const float v = __builtin_fmaf(__builtin_fmaf(-q, scale, y), inv, q);
-    return (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(v, 0.f, 0, false) & 0xff);
+    return __builtin_fmaf(__builtin_fmaf(-q, scale, y), inv, q);
 }
-// The row's scale.  A row of zeros gets 1; below the smallest normal number 1 / scale would overflow.
-__device__ __forceinline__ float row_scale(float amax) { return amax > 0.f ? fmaxf(amax / FP8_MAX, 0x1p-126f) : 1.f; }
+// The row's scale.  A row of zeros gets 1; between the bounds neither scale nor 1 / scale is infinite.
+__device__ __forceinline__ float row_scale(float amax) {
+    return amax > 0.f ? fminf(fmaxf(amax / FP8_MAX, 0x1p-126f), 0x1p127f) : 1.f;
+}
 
-// One workgroup per row, three passes over it (the second and third from the caches).  The sum h is held in 32 bits for
-// the norm and rounded once where it is stored.
+// 8 elements of a row from column c on, zeros behind its end.  The wide access needs no more than the type's alignment
+// (unaligned accesses are on for global memory on this target), so rows of any stride and length take it; only the last,
+// partial chunk of a row goes element by element.
+template <typename T> struct vec8;
+template <> struct vec8<bf16> { typedef bf16x8 type; };
+template <> struct vec8<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8))); };
+template <typename T> struct any8 { typedef typename vec8<T>::type type __attribute__((aligned(2))); };
+template <typename T>
+__device__ __forceinline__ typename vec8<T>::type load8(const T* row, int c, int cols) {
+    if (c + 8 <= cols) return *reinterpret_cast<const typename any8<T>::type*>(row + c);
+    typename vec8<T>::type v = {};
+#pragma unroll
+    for (int j = 0; j < 7; ++j)
+        if (c + j < cols) v[j] = row[c + j];
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* row, int c, int cols, const typename vec8<T>::type& v) {
+    if (c + 8 <= cols) {
+        *reinterpret_cast<typename any8<T>::type*>(row + c) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 7; ++j)
+            if (c + j < cols) row[c + j] = v[j];
+    }
+}
+typedef unsigned int any_u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+
+// sum over the TPR lanes of a row (a wave, or the workgroup: red holds a float per wave)
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+    v = wave_sum(v);
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < TPR / 64; ++i) v += red[i];
+    }
+    return v;
+}
+template <int TPR>
+__device__ __forceinline__ float row_max(float v, float* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < TPR / 64; ++i) v = fmaxf(v, red[i]);
+    }
+    return v;
+}
+
+// TPR lanes per row (64: four rows a workgroup), the row in registers (NCH chunks of 8 a lane) between the sum of squares
+// and the write: one read of x and resid, one write of y and h.  The sum h is held in 32 bits for the norm and rounded
+// once where it is stored.  (y and h may lie on x and resid: those four are not __restrict__; a lane has read all its
+// elements of the row before it writes one, and no other lane reads them.)
+template <typename T, bool Q8, int TPR, int NCH>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(const T* x, int64_t x_rs, const T* resid, int64_t r_rs,
+                                                                        const T* __restrict__ w, T* y, int64_t y_rs,
+                                                                        float* __restrict__ q_scale, T* h, int64_t h_rs, int rows,
+                                                                        int cols, float eps) {
+    typedef typename vec8<T>::type V;
+    __shared__ float red[2][TPR / 64];
+    const int lane = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * (TPR < 256 ? 256 / TPR : 1) + threadIdx.x / TPR;
+    if (TPR == 64 && row >= rows) return;                  // (whole waves; TPR > 64: the grid is the rows)
+    const T* xr = x + row * x_rs;
+    V xv[NCH], rv[NCH];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) xv[i] = load8(xr, (i * TPR + lane) * 8, cols);
+    if (resid) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) rv[i] = load8(resid + row * r_rs, (i * TPR + lane) * 8, cols);
+    }
+    float v[NCH][8], ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[i][j] = (float)xv[i][j];
+            if (resid) v[i][j] += (float)rv[i][j];
+            ss += v[i][j] * v[i][j];
+        }
+    const float r = 1.f / sqrtf(row_sum<TPR>(ss, red[0]) / (float)cols + eps);
+    if (resid) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            V o;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = (T)v[i][j];
+            store8(h + row * h_rs, (i * TPR + lane) * 8, cols, o);
+        }
+    }
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const V wv = load8(w, (i * TPR + lane) * 8, cols);
+        V o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[i][j] = v[i][j] * r * (float)wv[j];
+            if constexpr (Q8) m = fmaxf(m, fabsf(v[i][j]));
+            else o[j] = (T)v[i][j];
+        }
+        if constexpr (!Q8) store8(y + row * y_rs, (i * TPR + lane) * 8, cols, o);
+    }
+    if constexpr (Q8) {
+        const float scale = row_scale(row_max<TPR>(m, red[1])), inv = 1.f / scale;
+        if (lane == 0) q_scale[row] = scale;
+        unsigned char* qr = reinterpret_cast<unsigned char*>(y) + row * y_rs;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = (i * TPR + lane) * 8;
+            u32x2 o;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                int p = 0;
+                p = __builtin_amdgcn_cvt_pk_fp8_f32(divide(v[i][4 * k], scale, inv), divide(v[i][4 * k + 1], scale, inv), p, false);
+                p = __builtin_amdgcn_cvt_pk_fp8_f32(divide(v[i][4 * k + 2], scale, inv), divide(v[i][4 * k + 3], scale, inv), p, true);
+                o[k] = (unsigned)p;
+            }
+            if (c + 8 <= cols) {
+                *reinterpret_cast<any_u32x2*>(qr + c) = o;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 7; ++j)
+                    if (c + j < cols) qr[c + j] = (unsigned char)(o[j >> 2] >> (8 * (j & 3)));
+            }
+        }
+    }
+}
+
+// Rows of more than 65536 columns: one workgroup per row, two or three passes over it (all but the first from the caches).
 // (y and h may lie on x and resid: those four are not __restrict__, and a lane reads an element before it writes it)
 template <typename T, bool Q8>
 __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(const T* x, int64_t x_rs, const T* resid, int64_t r_rs,
@@ -67,13 +202,106 @@ __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(const T* x, int64_t x
     }
     for (int c = threadIdx.x; c < cols; c += 256) {
         const float v = at(c), o = v * r * (float)w[c];
-        if constexpr (Q8) reinterpret_cast<unsigned char*>(y)[row * y_rs + c] = to_e4m3(o, scale, inv);
+        if constexpr (Q8) reinterpret_cast<unsigned char*>(y)[row * y_rs + c] = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(divide(o, scale, inv), 0.f, 0, false) & 0xff);
         else y[row * y_rs + c] = (T)o;
         if (rr) h[row * h_rs + c] = (T)v;
     }
 }
 
-// dx of one row per workgroup (dx may lie on dh); the row's r is left in `rstd` for the weight's gradient
+// The gradient.  TPR lanes per row as above; a workgroup takes rows blockIdx.x, + gridDim.x, ..., keeps the weight's gradient
+// of its columns in registers over all of them and leaves one partial row of it: one read of dy, h and dh, one write of dx.
+// The next row is loaded before the current one's sums, so that the loads of two rows are in flight at every barrier.
+template <typename T, int TPR, int NCH>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_grad_kernel(const T* __restrict__ dy, int64_t dy_rs, const T* __restrict__ h,
+                                                                             int64_t h_rs, const T* dh, int64_t dh_rs,
+                                                                             const T* __restrict__ w, T* dx, int64_t dx_rs,
+                                                                             float* __restrict__ part, int rows, int cols, float eps) {
+    typedef typename vec8<T>::type V;
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;         // rows a workgroup has in hand
+    __shared__ float red[2][2][TPR / 64];                  // (alternating: one barrier a row)
+    const int lane = threadIdx.x % TPR;
+    const int sub = threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t row = (int64_t)blockIdx.x * RPB + sub;
+    V yv[NCH], hv[NCH], uv[NCH];
+    float dw[NCH][8] = {};
+    auto fetch = [&](int64_t r) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = (i * TPR + lane) * 8;
+            yv[i] = load8(dy + r * dy_rs, c, cols);
+            hv[i] = load8(h + r * h_rs, c, cols);
+            if (dh) uv[i] = load8(dh + r * dh_rs, c, cols);
+        }
+    };
+    if (row < rows) fetch(row);
+    for (int k = 0; row < rows; row += step, k ^= 1) {     // (TPR > 64: the same row in all lanes of the workgroup)
+        V yc[NCH], hc[NCH], uc[NCH];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            yc[i] = yv[i];
+            hc[i] = hv[i];
+            if (dh) uc[i] = uv[i];
+        }
+        if (row + step < rows) fetch(row + step);
+        float ss = 0.f, dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const V wv = load8(w, (i * TPR + lane) * 8, cols);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                ss += (float)hc[i][j] * (float)hc[i][j];
+                dot += (float)yc[i][j] * (float)wv[j] * (float)hc[i][j];
+            }
+        }
+        if constexpr (TPR > 64) {
+            ss = wave_sum(ss);
+            dot = wave_sum(dot);
+            if ((threadIdx.x & 63) == 0) {
+                red[k][0][threadIdx.x >> 6] = ss;
+                red[k][1][threadIdx.x >> 6] = dot;
+            }
+            __syncthreads();
+            ss = red[k][0][0];
+            dot = red[k][1][0];
+#pragma unroll
+            for (int i = 1; i < TPR / 64; ++i) {
+                ss += red[k][0][i];
+                dot += red[k][1][i];
+            }
+        } else {
+            ss = wave_sum(ss);
+            dot = wave_sum(dot);
+        }
+        const float r = 1.f / sqrtf(ss / (float)cols + eps);
+        const float kk = dot * r * r / (float)cols;        // mean(dn n) r
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = (i * TPR + lane) * 8;
+            const V wv = load8(w, c, cols);
+            V o;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float g = (float)yc[i][j], v = (float)hc[i][j];
+                dw[i][j] += g * (v * r);
+                o[j] = (T)((dh ? (float)uc[i][j] : 0.f) + r * (g * (float)wv[j] - v * kk));
+            }
+            store8(dx + row * dx_rs, c, cols, o);
+        }
+    }
+    float* pr = part + ((int64_t)blockIdx.x * RPB + sub) * ((cols + 7) & ~7);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int c = (i * TPR + lane) * 8;
+        if (c < cols) {
+            *reinterpret_cast<f32x4*>(pr + c) = f32x4{dw[i][0], dw[i][1], dw[i][2], dw[i][3]};
+            *reinterpret_cast<f32x4*>(pr + c + 4) = f32x4{dw[i][4], dw[i][5], dw[i][6], dw[i][7]};
+        }
+    }
+}
+
+// Longer rows: dx of one row per workgroup in two passes (dx may lie on dh), the row's r left in `rstd`; then
+// part[g][c] = sum of dy n over the rows of group g (a contiguous run), grid (ceil(cols / 256), groups).
 template <typename T>
 __global__ __launch_bounds__(256) void rmsnorm_grad_rows_kernel(const T* __restrict__ dy, int64_t dy_rs, const T* __restrict__ h,
                                                                 int64_t h_rs, const T* dh, int64_t dh_rs,
@@ -95,35 +323,52 @@ __global__ __launch_bounds__(256) void rmsnorm_grad_rows_kernel(const T* __restr
     }
     if (threadIdx.x == 0) rstd[row] = r;
 }
-
-// partial[g][c] = sum of dy n over the rows of group g (a contiguous run); grid (ceil(cols / 256), groups)
 template <typename T>
-__global__ __launch_bounds__(256) void rmsnorm_dweight_partial_kernel(const T* __restrict__ dy, int64_t dy_rs,
-                                                                      const T* __restrict__ h, int64_t h_rs,
-                                                                      const float* __restrict__ rstd, float* __restrict__ part,
-                                                                      int rows, int cols) {
+__global__ __launch_bounds__(256) void rmsnorm_dweight_rows_kernel(const T* __restrict__ dy, int64_t dy_rs, const T* __restrict__ h,
+                                                                   int64_t h_rs, const float* __restrict__ rstd, float* __restrict__ part,
+                                                                   int rows, int cols) {
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= cols) return;
     const int per = (rows + gridDim.y - 1) / gridDim.y;
     const int64_t r0 = (int64_t)blockIdx.y * per, r1 = min(r0 + per, (int64_t)rows);
     float s = 0.f;
     for (int64_t r = r0; r < r1; ++r) s += (float)dy[r * dy_rs + c] * ((float)h[r * h_rs + c] * rstd[r]);
-    part[(int64_t)blockIdx.y * cols + c] = s;
+    part[(int64_t)blockIdx.y * ((cols + 7) & ~7) + c] = s;
 }
+// dw = sum of the partial rows: a workgroup takes 64 columns, 16 groups of 16 lanes take every 16th row each and are added
+// up in a fixed order
 template <typename T>
-__global__ __launch_bounds__(256) void rmsnorm_dweight_reduce_kernel(const float* __restrict__ part, int groups, int cols,
-                                                                     T* __restrict__ dw) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
-    float s = 0.f;
-    for (int g = 0; g < groups; ++g) s += part[(int64_t)g * cols + c];
-    dw[c] = (T)s;
+__global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(const float* __restrict__ part, int parts, int cols, T* __restrict__ dw) {
+    __shared__ f32x4 red[16][16];
+    const int q = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 64 + q * 4, ld = (cols + 7) & ~7;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (c < ld) {
+#pragma unroll 8
+        for (int i = g; i < parts; i += 16) s += *reinterpret_cast<const f32x4*>(part + (int64_t)i * ld + c);
+    }
+    red[g][q] = s;
+    __syncthreads();
+    if (g == 0) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) s += red[i][q];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < cols) dw[c + j] = (T)s[j];
+    }
 }
 
 bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
 
-constexpr int GROUPS = 256;       // of rows, in the weight's gradient
-int grad_groups(int rows) { return rows < GROUPS ? rows : GROUPS; }
+constexpr int REG_COLS = 65536;      // the longest row that is held in registers (1024 lanes, 8 chunks each)
+// lanes per row: a wave where the rows alone fill the chip and a lane's share stays small (no barrier), else a workgroup
+constexpr int WAVE_COLS = 4096, GROUP_COLS = 8192;
+
+// the gradient's partial rows of dweight
+int grad_parts(int rows, int cols) {
+    if (cols > REG_COLS) return rows < 256 ? rows : 256;
+    const int rpb = cols <= 1024 ? 4 : 1, groups = (rows + rpb - 1) / rpb;
+    return (groups < 768 ? groups : 768) * rpb;
+}
 
 template <typename T, bool Q8>
 int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, const void* w, void* y, int64_t y_rs,
@@ -133,8 +378,29 @@ int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, co
     FP_REQUIRE(aligned2(x) && aligned2(resid) && aligned2(w) && (Q8 || aligned2(y)) && aligned2(h));
     FP_REQUIRE(!Q8 || (q_scale && ((uintptr_t)q_scale & 3) == 0));
     if (rows == 0) return 0;
-    rmsnorm_rows_kernel<T, Q8><<<dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream>>>(
-        (const T*)x, x_rs, (const T*)resid, r_rs, (const T*)w, (T*)y, y_rs, (float*)q_scale, (T*)h, h_rs, cols, eps);
+    hipStream_t st = (hipStream_t)stream;
+#define FP_NORM(TPR, NCH)                                                                                                         \
+    rmsnorm_kernel<T, Q8, TPR, NCH><<<dim3((unsigned)(TPR < 256 ? (rows + 3) / 4 : rows)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>( \
+        (const T*)x, x_rs, (const T*)resid, r_rs, (const T*)w, (T*)y, y_rs, (float*)q_scale, (T*)h, h_rs, rows, cols, eps)
+    const int nch = (cols + 7) / 8;
+    if (cols <= 512 || (cols <= WAVE_COLS && rows >= 2048)) {
+        if (nch <= 64) FP_NORM(64, 1);
+        else if (nch <= 128) FP_NORM(64, 2);
+        else if (nch <= 256) FP_NORM(64, 4);
+        else FP_NORM(64, 8);
+    } else if (cols <= GROUP_COLS) {
+        if (nch <= 256) FP_NORM(256, 1);
+        else if (nch <= 512) FP_NORM(256, 2);
+        else FP_NORM(256, 4);
+    } else if (cols <= REG_COLS) {
+        if (nch <= 2048) FP_NORM(1024, 2);
+        else if (nch <= 4096) FP_NORM(1024, 4);
+        else FP_NORM(1024, 8);
+    } else {
+        rmsnorm_rows_kernel<T, Q8><<<dim3((unsigned)rows), dim3(256), 0, st>>>((const T*)x, x_rs, (const T*)resid, r_rs, (const T*)w,
+                                                                              (T*)y, y_rs, (float*)q_scale, (T*)h, h_rs, cols, eps);
+    }
+#undef FP_NORM
     FP_CHECK_LAUNCH();
     return 0;
 }
@@ -147,17 +413,31 @@ int grad_launch(const void* dy, int64_t dy_rs, const void* h, int64_t h_rs, cons
     FP_REQUIRE(aligned2(dy) && aligned2(h) && aligned2(dh) && aligned2(w) && aligned2(dx) && aligned2(dw));
     FP_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= fp_rmsnorm_residual_backward_workspace_bytes(rows, cols));
     hipStream_t st = (hipStream_t)stream;
-    float* rstd = (float*)ws;
-    float* part = rstd + ((rows + 3) & ~3);
-    const int groups = grad_groups(rows);
-    rmsnorm_grad_rows_kernel<T><<<dim3((unsigned)rows), dim3(256), 0, st>>>((const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh,
-                                                                           dh_rs, (const T*)w, (T*)dx, dx_rs, rstd, cols, eps);
+    const int parts = grad_parts(rows, cols);
+    float* part = (float*)ws;
+#define FP_GRAD(TPR, NCH)                                                                                                        \
+    rmsnorm_grad_kernel<T, TPR, NCH><<<dim3((unsigned)(TPR < 256 ? parts / 4 : parts)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(   \
+        (const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh, dh_rs, (const T*)w, (T*)dx, dx_rs, part, rows, cols, eps)
+    const int nch = (cols + 7) / 8;
+    if (nch <= 64) FP_GRAD(64, 1);
+    else if (nch <= 128) FP_GRAD(64, 2);
+    else if (nch <= 256) FP_GRAD(256, 1);
+    else if (nch <= 512) FP_GRAD(256, 2);
+    else if (nch <= 1024) FP_GRAD(256, 4);
+    else if (nch <= 2048) FP_GRAD(1024, 2);
+    else if (nch <= 4096) FP_GRAD(1024, 4);
+    else if (nch <= 8192) FP_GRAD(1024, 8);
+    else {
+        float* rstd = part + (int64_t)parts * ((cols + 7) & ~7);
+        rmsnorm_grad_rows_kernel<T><<<dim3((unsigned)rows), dim3(256), 0, st>>>((const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh, dh_rs,
+                                                                               (const T*)w, (T*)dx, dx_rs, rstd, cols, eps);
+        FP_CHECK_LAUNCH();
+        rmsnorm_dweight_rows_kernel<T><<<dim3((unsigned)((cols + 255) / 256), (unsigned)parts), dim3(256), 0, st>>>(
+            (const T*)dy, dy_rs, (const T*)h, h_rs, rstd, part, rows, cols);
+    }
+#undef FP_GRAD
     FP_CHECK_LAUNCH();
-    const unsigned cb = (unsigned)((cols + 255) / 256);
-    rmsnorm_dweight_partial_kernel<T><<<dim3(cb, (unsigned)groups), dim3(256), 0, st>>>((const T*)dy, dy_rs, (const T*)h, h_rs, rstd,
-                                                                                       part, rows, cols);
-    FP_CHECK_LAUNCH();
-    rmsnorm_dweight_reduce_kernel<T><<<dim3(cb), dim3(256), 0, st>>>(part, groups, cols, (T*)dw);
+    rmsnorm_dweight_kernel<T><<<dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, st>>>(part, parts, cols, (T*)dw);
     FP_CHECK_LAUNCH();
     return 0;
 }
@@ -187,7 +467,7 @@ extern "C" int fp_rmsnorm_residual_fp8(const void* x, int64_t x_row_stride, cons
 
 extern "C" int64_t fp_rmsnorm_residual_backward_workspace_bytes(int rows, int cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return ((int64_t)((rows + 3) & ~3) + (int64_t)grad_groups(rows) * cols) * 4;
+    return ((int64_t)grad_parts(rows, cols) * (((int64_t)cols + 7) & ~7) + (cols > REG_COLS ? (int64_t)rows : 0)) * 4;
 }
 
 extern "C" int fp_rmsnorm_residual_backward_bf16(const void* dy, int64_t dy_row_stride, const void* h, int64_t h_row_stride,

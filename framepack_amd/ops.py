@@ -20,7 +20,13 @@ F16 = torch.float16
 ATTN_EVENTS: Optional[list] = None
 
 
+# (the handle alone: building torch's Stream object around it takes 2 us, as long as a small kernel)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t: torch.Tensor) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -681,35 +687,41 @@ def attention_framecausal(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, q_
 ACT_SILU, ACT_GELU = 0, 1          # GELU: the tanh form, as in EPI_GELU
 
 
-def _mat(t: torch.Tensor, what: str, dtypes, shape=None):
+def _mat(t: torch.Tensor, what: str, dtypes, rows: int = -1, cols: int = -1):
     """(tensor, rows, cols, row stride) of a matrix argument of K12 / K13: [.., rows, cols] as `_rows2d` takes it, of one
-    of `dtypes`, and of `shape` if given.  A single row's stride says nothing and is replaced by the row's length."""
+    of `dtypes`, of `rows` and `cols` if given.  A single row's stride says nothing and is replaced by the row's length."""
     if t.dtype not in dtypes:
         raise ValueError(f"{what}: expected {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.dim() < 2:
-        raise ValueError(f"{what}: expected a [rows, cols] tensor, got {tuple(t.shape)}")
-    if t.dim() > 2:
+    if t.dim() != 2:
+        if t.dim() < 2:
+            raise ValueError(f"{what}: expected a [rows, cols] tensor, got {tuple(t.shape)}")
         t = t.reshape(-1, t.shape[-1]) if t.is_contiguous() else t.squeeze(0)
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{what}: expected a [rows, cols] tensor with unit inner stride, got {tuple(t.shape)} / {t.stride()}")
-    rows, cols = t.shape
-    if cols == 0 or (shape is not None and (rows, cols) != tuple(shape)):
-        raise ValueError(f"{what}: expected {'at least one column' if shape is None else list(shape)}, got {[rows, cols]}")
-    return t, rows, cols, (t.stride(0) if rows > 1 else (cols + 15) // 16 * 16)
+        if t.dim() != 2:
+            raise ValueError(f"{what}: expected a [rows, cols] tensor, got {tuple(t.shape)} / {t.stride()}")
+    r, c = t.shape
+    rs, cs = t.stride()
+    if c == 0 or (rows >= 0 and r != rows) or (cols >= 0 and c != cols):
+        raise ValueError(f"{what}: expected [{rows if rows >= 0 else 'rows'}, {cols if cols >= 0 else 'at least one column'}], "
+                         f"got {[r, c]}")
+    if cs != 1 and c > 1:
+        raise ValueError(f"{what}: expected a [rows, cols] tensor with unit inner stride, got {[r, c]} / {(rs, cs)}")
+    return t, r, c, rs if r > 1 else (c + 15) // 16 * 16
 
 
 def _vec(t: torch.Tensor, what: str, dtype, n: int) -> torch.Tensor:
     """A vector argument of n values; made contiguous where it is not."""
     if t.dtype != dtype or t.numel() != n:
         raise ValueError(f"{what}: expected {n} values of {dtype}, got {tuple(t.shape)} of {t.dtype}")
-    return t.reshape(-1).contiguous()
+    return t if t.is_contiguous() else t.reshape(-1).contiguous()
 
 
-def _out(t: Optional[torch.Tensor], what: str, dtype, rows: int, cols: int, device):
-    """An output matrix: allocated if None, else of this type and size with rows that do not overlap each other."""
+def _out(t: Optional[torch.Tensor], what: str, dtype, rows: int, cols: int, like: torch.Tensor):
+    """An output matrix (as returned, 2-d view, row stride): allocated if None, else of this type and size with rows that do
+    not overlap each other."""
     if t is None:
-        t = torch.empty((rows, cols), dtype=dtype, device=device)
-    t2, _, _, rs = _mat(t, what, (dtype,), (rows, cols))
+        t = like.new_empty((rows, cols), dtype=dtype)
+        return t, t, cols if rows > 1 else (cols + 15) // 16 * 16
+    t2, _, _, rs = _mat(t, what, (dtype,), rows, cols)
     if rs < cols:
         raise ValueError(f"{what}: rows of {cols} values overlap at a row stride of {rs}")
     return t, t2, rs
@@ -741,11 +753,19 @@ def _apart(outs, ins, same=()) -> None:
             if _share(a, b):
                 raise ValueError(f"{na} and {nb} share memory")
         for nb, b in ins:
-            if b is None or not _share(a, b):
+            if b is None:
+                continue
+            b = b if b.dim() == 2 else b.reshape(1, -1)
+            if not _share(a, b):
                 continue
             if (na, nb) in same and a.data_ptr() == b.data_ptr() and (a.shape[0] <= 1 or a.stride(0) == b.stride(0)):
                 continue
             raise ValueError(f"{na} shares memory with {nb}")
+
+
+def _given(*outs):
+    """The outputs that the caller gave, as (name, matrix): only those can share memory with anything."""
+    return [(n, m) for n, t, m in outs if t is not None]
 
 
 def _rmsnorm_args(x, weight, resid, resid_out, dtypes, eps):
@@ -758,9 +778,12 @@ def _rmsnorm_args(x, weight, resid, resid_out, dtypes, eps):
         if resid_out is not None:
             raise ValueError("resid_out without resid")
         return x2, rows, cols, xs, w, None, 0, x, None, 0
-    r2, _, _, rs = _mat(resid, "resid", (x.dtype,), (rows, cols))
-    h, h2, hs = _out(resid_out, "resid_out", x.dtype, rows, cols, x.device)
+    r2, _, _, rs = _mat(resid, "resid", (x.dtype,), rows, cols)
+    h, h2, hs = _out(resid_out, "resid_out", x.dtype, rows, cols, x)
     return x2, rows, cols, xs, w, r2, rs, h, h2, hs
+
+
+_NORM_SAME = {(o, i) for o in ("out", "resid_out") for i in ("x", "resid")}
 
 
 def rmsnorm_residual(x: torch.Tensor, weight: torch.Tensor, resid: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -769,17 +792,18 @@ def rmsnorm_residual(x: torch.Tensor, weight: torch.Tensor, resid: Optional[torc
     x, resid [rows, cols] (row-strided ok, any cols), weight [cols], one type: bf16 or f16.  The norm is taken of the
     32-bit sum; h is that sum rounded to the type.  out and resid_out may each be x or resid itself."""
     x2, rows, cols, xs, w, r2, rs, h, h2, hs = _rmsnorm_args(x, weight, resid, resid_out, (BF16, F16), eps)
-    _dev(out)
-    out, o2, os_ = _out(out, "out", x.dtype, rows, cols, x.device)
-    outs = [("out", o2)] + ([] if h2 is None else [("resid_out", h2)])
-    _apart(outs, [("x", x2), ("resid", r2), ("weight", w[None])],
-           {(o, i) for o in ("out", "resid_out") for i in ("x", "resid")})
+    y, y2, ys = _out(out, "out", x.dtype, rows, cols, x)
+    if out is not None or resid_out is not None:
+        _dev(x, out)
+        _apart(_given(("out", out, y2), ("resid_out", resid_out, h2)), [("x", x2), ("resid", r2), ("weight", w)], _NORM_SAME)
     if rows == 0:
-        return out, h
-    name = "fp_rmsnorm_residual_bf16" if x.dtype == BF16 else "fp_rmsnorm_residual_f16"
-    _lib.check(getattr(_lib.load(), name)(x2.data_ptr(), xs, _ptr(r2), rs, w.data_ptr(), o2.data_ptr(), os_, _ptr(h2), hs,
-                                          rows, cols, eps, _stream(x)), name)
-    return out, h
+        return y, h
+    lib = _lib.load()
+    fn, name = ((lib.fp_rmsnorm_residual_bf16, "fp_rmsnorm_residual_bf16") if x.dtype == BF16 else
+                (lib.fp_rmsnorm_residual_f16, "fp_rmsnorm_residual_f16"))
+    _lib.check(fn(x2.data_ptr(), xs, _ptr(r2), rs, w.data_ptr(), y2.data_ptr(), ys, _ptr(h2), hs, rows, cols, eps, _stream(x)),
+               name)
+    return y, h
 
 
 def rmsnorm_residual_fp8(x: torch.Tensor, weight: torch.Tensor, resid: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -789,20 +813,23 @@ def rmsnorm_residual_fp8(x: torch.Tensor, weight: torch.Tensor, resid: Optional[
     operand of `gated_ff_fp8` and `gemm_fp8`.  scale = max|row| / 448 (1 for a row of zeros); q is rounded once, from 32
     bits.  bf16 only."""
     x2, rows, cols, xs, w, r2, rs, h, h2, hs = _rmsnorm_args(x, weight, resid, resid_out, (BF16,), eps)
-    _dev(out, out_scale)
-    out, o2, os_ = _out(out, "out", FP8, rows, cols, x.device)
+    q, q2, qs = _out(out, "out", FP8, rows, cols, x)
     if out_scale is None:
-        out_scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    if out_scale.dtype != torch.float32 or out_scale.numel() != rows or not out_scale.is_contiguous():
-        raise ValueError(f"out_scale: expected {rows} contiguous float32 values")
-    outs = [("out", o2), ("out_scale", out_scale.reshape(1, -1))] + ([] if h2 is None else [("resid_out", h2)])
-    _apart(outs, [("x", x2), ("resid", r2), ("weight", w[None])], {("resid_out", "x"), ("resid_out", "resid")})
+        s = x.new_empty((rows,), dtype=torch.float32)
+    else:
+        s = out_scale
+        if s.dtype != torch.float32 or s.numel() != rows or not s.is_contiguous():
+            raise ValueError(f"out_scale: expected {rows} contiguous float32 values")
+    if out is not None or out_scale is not None or resid_out is not None:
+        _dev(x, out, out_scale)
+        _apart(_given(("out", out, q2), ("out_scale", out_scale, s.reshape(1, -1)), ("resid_out", resid_out, h2)),
+               [("x", x2), ("resid", r2), ("weight", w)], _NORM_SAME - {("out", "x"), ("out", "resid")})
     if rows == 0:
-        return out, out_scale, h
-    _lib.check(_lib.load().fp_rmsnorm_residual_fp8(x2.data_ptr(), xs, _ptr(r2), rs, w.data_ptr(), o2.data_ptr(), os_,
-                                                   out_scale.data_ptr(), _ptr(h2), hs, rows, cols, eps, _stream(x)),
+        return q, s, h
+    _lib.check(_lib.load().fp_rmsnorm_residual_fp8(x2.data_ptr(), xs, _ptr(r2), rs, w.data_ptr(), q2.data_ptr(), qs,
+                                                   s.data_ptr(), _ptr(h2), hs, rows, cols, eps, _stream(x)),
                "fp_rmsnorm_residual_fp8")
-    return out, out_scale, h
+    return q, s, h
 
 
 def rmsnorm_residual_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, dh: Optional[torch.Tensor] = None,
@@ -812,25 +839,28 @@ def rmsnorm_residual_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.T
     All [rows, cols] of one type, bf16 or f16; dweight [cols] of weight's type, summed in 32 bits in a fixed order."""
     _dev(dy, h, weight, dh, dx)
     h2, rows, cols, hs = _mat(h, "h", (BF16, F16))
-    y2, _, _, ys = _mat(dy, "dy", (h.dtype,), (rows, cols))
+    y2, _, _, ys = _mat(dy, "dy", (h.dtype,), rows, cols)
     w = _vec(weight, "weight", h.dtype, cols)
     if not eps >= 0:
         raise ValueError(f"eps: expected a number of at least 0, got {eps}")
     d2, ds = None, 0
     if dh is not None:
-        d2, _, _, ds = _mat(dh, "dh", (h.dtype,), (rows, cols))
-    dx, dx2, dxs = _out(dx, "dx", h.dtype, rows, cols, h.device)
-    _apart([("dx", dx2)], [("dy", y2), ("h", h2), ("dh", d2), ("weight", w[None])], {("dx", "dh")})
+        d2, _, _, ds = _mat(dh, "dh", (h.dtype,), rows, cols)
+    got, dx2, dxs = _out(dx, "dx", h.dtype, rows, cols, h)
+    if dx is not None:
+        _apart([("dx", dx2)], [("dy", y2), ("h", h2), ("dh", d2), ("weight", w)], {("dx", "dh")})
     if rows == 0:
-        return dx, torch.zeros((cols,), dtype=h.dtype, device=h.device)
-    dw = torch.empty((cols,), dtype=h.dtype, device=h.device)
+        return got, h.new_zeros((cols,))
+    dw = h.new_empty((cols,))
     lib = _lib.load()
     # (per call: the caching allocator keeps it apart from other streams' and other captured graphs' calls)
-    ws = torch.empty((lib.fp_rmsnorm_residual_backward_workspace_bytes(rows, cols),), dtype=torch.uint8, device=h.device)
-    name = "fp_rmsnorm_residual_backward_bf16" if h.dtype == BF16 else "fp_rmsnorm_residual_backward_f16"
-    _lib.check(getattr(lib, name)(y2.data_ptr(), ys, h2.data_ptr(), hs, _ptr(d2), ds, w.data_ptr(), dx2.data_ptr(), dxs,
-                                  dw.data_ptr(), rows, cols, eps, ws.data_ptr(), ws.numel(), _stream(h)), name)
-    return dx, dw
+    n = lib.fp_rmsnorm_residual_backward_workspace_bytes(rows, cols)
+    ws = h.new_empty((n,), dtype=torch.uint8)
+    fn, name = ((lib.fp_rmsnorm_residual_backward_bf16, "fp_rmsnorm_residual_backward_bf16") if h.dtype == BF16 else
+                (lib.fp_rmsnorm_residual_backward_f16, "fp_rmsnorm_residual_backward_f16"))
+    _lib.check(fn(y2.data_ptr(), ys, h2.data_ptr(), hs, _ptr(d2), ds, w.data_ptr(), dx2.data_ptr(), dxs, dw.data_ptr(), rows,
+                  cols, eps, ws.data_ptr(), n, _stream(h)), name)
+    return got, dw
 
 
 def _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, dtypes, bias_dtype):
@@ -838,7 +868,7 @@ def _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, dtypes, bias_dtype):
     g2, F, _, ldg = _mat(w_gate, "w_gate", (x.dtype,))
     if g2.shape[1] != K:
         raise ValueError(f"w_gate: expected [inner, {K}], got {list(g2.shape)}")
-    u2, _, _, ldu = _mat(w_up, "w_up", (x.dtype,), (F, K))
+    u2, _, _, ldu = _mat(w_up, "w_up", (x.dtype,), F, K)
     if F == 0:
         raise ValueError("w_gate: expected at least one row")
     if act not in (ACT_SILU, ACT_GELU):
@@ -858,16 +888,17 @@ def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: 
     type, bf16 or f16.  The block's second linear is `gemm`, with the residual in its epilogue (EPI_RESIDUAL)."""
     _dev(x, w_gate, w_up, b_gate, b_up, out)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, (BF16, F16), x.dtype)
-    out, o2, ldo = _out(out, "out", x.dtype, M, F, x.device)
-    _apart([("out", o2)], [("x", x2), ("w_gate", g2), ("w_up", u2), ("b_gate", None if bg is None else bg[None]),
-                           ("b_up", None if bu is None else bu[None])])
-    gate = torch.empty((M, F), dtype=x.dtype, device=x.device) if keep else None
-    up = torch.empty((M, F), dtype=x.dtype, device=x.device) if keep else None
+    h, h2, ldh = _out(out, "out", x.dtype, M, F, x)
+    if out is not None:
+        _apart([("out", h2)], [("x", x2), ("w_gate", g2), ("w_up", u2), ("b_gate", bg), ("b_up", bu)])
+    gate = x.new_empty((M, F)) if keep else None
+    up = x.new_empty((M, F)) if keep else None
     if M > 0:
-        name = "fp_gated_ff_bf16" if x.dtype == BF16 else "fp_gated_ff_f16"
-        _lib.check(getattr(_lib.load(), name)(x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, _ptr(bg), _ptr(bu),
-                                              o2.data_ptr(), ldo, _ptr(gate), _ptr(up), F, M, F, K, act, _stream(x)), name)
-    return (out, gate, up) if keep else out
+        lib = _lib.load()
+        fn, name = (lib.fp_gated_ff_bf16, "fp_gated_ff_bf16") if x.dtype == BF16 else (lib.fp_gated_ff_f16, "fp_gated_ff_f16")
+        _lib.check(fn(x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, _ptr(bg), _ptr(bu), h2.data_ptr(), ldh,
+                      _ptr(gate), _ptr(up), F, M, F, K, act, _stream(x)), name)
+    return (h, gate, up) if keep else h
 
 
 def gated_ff_fp8(x_q: torch.Tensor, x_scale: torch.Tensor, wg_q: torch.Tensor, wg_scale: torch.Tensor, wu_q: torch.Tensor,
@@ -881,16 +912,16 @@ def gated_ff_fp8(x_q: torch.Tensor, x_scale: torch.Tensor, wg_q: torch.Tensor, w
     x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x_q, wg_q, wu_q, b_gate, b_up, act, (FP8,), BF16)
     xs, gs, us = (_vec(t, n, torch.float32, k) for t, n, k in ((x_scale, "x_scale", M), (wg_scale, "wg_scale", F),
                                                               (wu_scale, "wu_scale", F)))
-    out, o2, ldo = _out(out, "out", BF16, M, F, x_q.device)
-    _apart([("out", o2)], [("x_q", x2), ("wg_q", g2), ("wu_q", u2), ("x_scale", xs[None]), ("wg_scale", gs[None]),
-                           ("wu_scale", us[None]), ("b_gate", None if bg is None else bg[None]),
-                           ("b_up", None if bu is None else bu[None])])
+    h, h2, ldh = _out(out, "out", BF16, M, F, x_q)
+    if out is not None:
+        _apart([("out", h2)], [("x_q", x2), ("wg_q", g2), ("wu_q", u2), ("x_scale", xs), ("wg_scale", gs), ("wu_scale", us),
+                               ("b_gate", bg), ("b_up", bu)])
     if M == 0:
-        return out
+        return h
     _lib.check(_lib.load().fp_gated_ff_fp8(x2.data_ptr(), ldx, xs.data_ptr(), g2.data_ptr(), ldg, gs.data_ptr(), u2.data_ptr(),
-                                           ldu, us.data_ptr(), _ptr(bg), _ptr(bu), o2.data_ptr(), ldo, M, F, K, act,
+                                           ldu, us.data_ptr(), _ptr(bg), _ptr(bu), h2.data_ptr(), ldh, M, F, K, act,
                                            _stream(x_q)), "fp_gated_ff_fp8")
-    return out
+    return h
 
 
 def gated_ff_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor,
@@ -900,19 +931,22 @@ def gated_ff_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w
     rounded to it between the two steps, sums are held in 32 bits and taken in a fixed order.  dw_gate and dw_up are the
     halves of one [2 * inner, K] tensor (the gradient of a fused weight)."""
     _dev(dh, x, w_gate, w_up, gate, up)
+    dt = (x.dtype,)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, _, _ = _gated_ff_args(x, w_gate, w_up, None, None, act, (BF16, F16), x.dtype)
-    (d2, _, _, ldd), (p2, _, _, ldp), (q2, _, _, ldq) = (_mat(t, n, (x.dtype,), (M, F)) for t, n in ((dh, "dh"), (gate, "gate"),
-                                                                                                    (up, "up")))
-    if M == 0:
-        dw = torch.zeros((2 * F, K), dtype=x.dtype, device=x.device)
-        db = torch.zeros((2, F), dtype=x.dtype, device=x.device) if bias else (None, None)
-        return torch.empty((0, K), dtype=x.dtype, device=x.device), dw[:F], dw[F:], db[0], db[1]
-    dx = torch.empty((M, K), dtype=x.dtype, device=x.device)
-    dw = torch.empty((2 * F, K), dtype=x.dtype, device=x.device)
-    db = torch.empty((2, F), dtype=x.dtype, device=x.device) if bias else (None, None)
-    lib = _lib.load()
-    ws = torch.empty((lib.fp_gated_ff_backward_workspace_bytes(M, F, K),), dtype=torch.uint8, device=x.device)
-    name = "fp_gated_ff_backward_bf16" if x.dtype == BF16 else "fp_gated_ff_backward_f16"
-    _lib.check(getattr(lib, name)(d2.data_ptr(), ldd, x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, p2.data_ptr(),
-                                  ldp, q2.data_ptr(), ldq, dx.data_ptr(), dw.data_ptr(), dw[F:].data_ptr(), _ptr(db[0]), _ptr(db[1]), M, F, K, act, ws.data_ptr(), ws.numel(), _stream(x)), name)
-    return dx, dw[:F], dw[F:], db[0], db[1]
+    d2, _, _, ldd = _mat(dh, "dh", dt, M, F)
+    p2, _, _, ldp = _mat(gate, "gate", dt, M, F)
+    q2, _, _, ldq = _mat(up, "up", dt, M, F)
+    new = x.new_empty if M > 0 else x.new_zeros
+    dx, dw = new((M, K)), new((2 * F, K))
+    dwg, dwu = dw[:F], dw[F:]
+    dbg, dbu = new((2, F)) if bias else (None, None)
+    if M > 0:
+        lib = _lib.load()
+        n = lib.fp_gated_ff_backward_workspace_bytes(M, F, K)
+        ws = x.new_empty((n,), dtype=torch.uint8)
+        fn, name = ((lib.fp_gated_ff_backward_bf16, "fp_gated_ff_backward_bf16") if x.dtype == BF16 else
+                    (lib.fp_gated_ff_backward_f16, "fp_gated_ff_backward_f16"))
+        _lib.check(fn(d2.data_ptr(), ldd, x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, p2.data_ptr(), ldp,
+                      q2.data_ptr(), ldq, dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), _ptr(dbg), _ptr(dbu), M, F, K, act,
+                      ws.data_ptr(), n, _stream(x)), name)
+    return dx, dwg, dwu, dbg, dbu
