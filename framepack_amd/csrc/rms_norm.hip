@@ -41,32 +41,51 @@ __device__ __forceinline__ float row_scale(float amax) {
 }
 
 // 8 elements of a row from column c on, zeros behind its end.  The wide access needs no more than the type's alignment
-// (unaligned accesses are on for global memory on this target), so rows of any stride and length take it; only the last,
-// partial chunk of a row goes element by element.
+// (unaligned accesses are on for global memory on this target), so rows of any stride and length take it.  A row's partial
+// last chunk is read as its last 8 elements and moved into place by `fit` where it is used, so that the load itself is one
+// instruction that nothing waits for (as seven conditional loads it cost a row of 4095 columns a third of its time).
 template <typename T> struct vec8;
 template <> struct vec8<bf16> { typedef bf16x8 type; };
 template <> struct vec8<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8))); };
 template <typename T> struct any8 { typedef typename vec8<T>::type type __attribute__((aligned(2))); };
 template <typename T>
 __device__ __forceinline__ typename vec8<T>::type load8(const T* row, int c, int cols) {
-    if (c + 8 <= cols) return *reinterpret_cast<const typename any8<T>::type*>(row + c);
     typename vec8<T>::type v = {};
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-        if (c + j < cols) v[j] = row[c + j];
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* row, int c, int cols, const typename vec8<T>::type& v) {
-    if (c + 8 <= cols) {
-        *reinterpret_cast<typename any8<T>::type*>(row + c) = v;
+    if (cols >= 8) {                                        // (uniform)
+        if (c < cols) v = *reinterpret_cast<const typename any8<T>::type*>(row + min(c, cols - 8));
     } else {
 #pragma unroll
         for (int j = 0; j < 7; ++j)
-            if (c + j < cols) row[c + j] = v[j];
+            if (c + j < cols) v[j] = row[c + j];
+    }
+    return v;
+}
+template <typename V> __device__ __forceinline__ void fit(V& v, int c, int cols) {
+    if ((cols & 7) == 0 || cols < 8) return;                // (uniform, as is all but the last line)
+    const int s = 8 - (cols & 7);                           // elements in front of the chunk's
+    u32x4 d = __builtin_bit_cast(u32x4, v);
+    if (s & 1) d = u32x4{__builtin_amdgcn_alignbit(d[1], d[0], 16), __builtin_amdgcn_alignbit(d[2], d[1], 16),
+                         __builtin_amdgcn_alignbit(d[3], d[2], 16), d[3] >> 16};
+    if (s & 2) d = u32x4{d[1], d[2], d[3], 0u};
+    if (s & 4) d = u32x4{d[2], d[3], 0u, 0u};
+    if (c < cols && c + 8 > cols) v = __builtin_bit_cast(V, d);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* row, int c, int cols, const typename vec8<T>::type& v) {
+    typedef T A4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef T A2 __attribute__((ext_vector_type(2), aligned(2)));
+    if (c + 8 <= cols) {
+        *reinterpret_cast<typename any8<T>::type*>(row + c) = v;
+    } else if (c < cols) {
+        const int n = cols & 7;
+        if (n & 4) *reinterpret_cast<A4*>(row + c) = A4{v[0], v[1], v[2], v[3]};
+        if (n & 2) *reinterpret_cast<A2*>(row + c + (n & 4)) = n & 4 ? A2{v[4], v[5]} : A2{v[0], v[1]};
+        if (n & 1) row[c + n - 1] = n & 4 ? (n & 2 ? v[6] : v[4]) : (n & 2 ? v[2] : v[0]);
     }
 }
 typedef unsigned int any_u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned int any_u32 __attribute__((aligned(1)));
+typedef unsigned short any_u16 __attribute__((aligned(1)));
 
 // sum over the TPR lanes of a row (a wave, or the workgroup: red holds a float per wave)
 template <int TPR>
@@ -110,12 +129,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(const T*
     const int64_t row = (int64_t)blockIdx.x * (TPR < 256 ? 256 / TPR : 1) + threadIdx.x / TPR;
     if (TPR == 64 && row >= rows) return;                  // (whole waves; TPR > 64: the grid is the rows)
     const T* xr = x + row * x_rs;
-    V xv[NCH], rv[NCH];
+    V xv[NCH], rv[NCH], wv[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) xv[i] = load8(xr, (i * TPR + lane) * 8, cols);
     if (resid) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) rv[i] = load8(resid + row * r_rs, (i * TPR + lane) * 8, cols);
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) wv[i] = load8(w, (i * TPR + lane) * 8, cols);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        if ((i + 1) * TPR * 8 <= cols) continue;            // (uniform: a whole chunk in every lane)
+        fit(xv[i], (i * TPR + lane) * 8, cols);
+        if (resid) fit(rv[i], (i * TPR + lane) * 8, cols);
+        fit(wv[i], (i * TPR + lane) * 8, cols);
     }
     float v[NCH][8], ss = 0.f;
 #pragma unroll
@@ -139,11 +167,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(const T*
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        const V wv = load8(w, (i * TPR + lane) * 8, cols);
         V o;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[i][j] = v[i][j] * r * (float)wv[j];
+            v[i][j] = v[i][j] * r * (float)wv[i][j];
             if constexpr (Q8) m = fmaxf(m, fabsf(v[i][j]));
             else o[j] = (T)v[i][j];
         }
@@ -166,10 +193,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(const T*
             }
             if (c + 8 <= cols) {
                 *reinterpret_cast<any_u32x2*>(qr + c) = o;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 7; ++j)
-                    if (c + j < cols) qr[c + j] = (unsigned char)(o[j >> 2] >> (8 * (j & 3)));
+            } else if (c < cols) {
+                const int n = cols & 7;
+                const unsigned t = n & 4 ? o[1] : o[0];     // behind a whole first half, or the half itself
+                if (n & 4) *reinterpret_cast<any_u32*>(qr + c) = o[0];
+                if (n & 2) *reinterpret_cast<any_u16*>(qr + c + (n & 4)) = (unsigned short)t;
+                if (n & 1) qr[c + n - 1] = (unsigned char)(n & 2 ? t >> 16 : t);
             }
         }
     }
@@ -210,8 +239,10 @@ __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(const T* x, int64_t x
 
 // The gradient.  TPR lanes per row as above; a workgroup takes rows blockIdx.x, + gridDim.x, ..., keeps the weight's gradient
 // of its columns in registers over all of them and leaves one partial row of it: one read of dy, h and dh, one write of dx.
-// The next row is loaded before the current one's sums, so that the loads of two rows are in flight at every barrier.
-template <typename T, int TPR, int NCH>
+// DW = false (longer rows, whose share of dweight does not fit the registers as well): the row's r is left in part[row].
+// AHEAD: the next row is loaded before the current one's sums, so that the loads of two rows are in flight at every barrier
+// (where the registers hold them).
+template <typename T, int TPR, int NCH, bool AHEAD, bool DW>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_grad_kernel(const T* __restrict__ dy, int64_t dy_rs, const T* __restrict__ h,
                                                                              int64_t h_rs, const T* dh, int64_t dh_rs,
                                                                              const T* __restrict__ w, T* dx, int64_t dx_rs,
@@ -223,8 +254,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_grad_kernel(con
     const int sub = threadIdx.x / TPR;
     const int64_t step = (int64_t)gridDim.x * RPB;
     int64_t row = (int64_t)blockIdx.x * RPB + sub;
-    V yv[NCH], hv[NCH], uv[NCH];
-    float dw[NCH][8] = {};
+    V yv[NCH], hv[NCH], uv[NCH], wv[NCH];
+    float dw[DW ? NCH : 1][8] = {};
     auto fetch = [&](int64_t r) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
@@ -234,8 +265,14 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_grad_kernel(con
             if (dh) uv[i] = load8(dh + r * dh_rs, c, cols);
         }
     };
-    if (row < rows) fetch(row);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        wv[i] = load8(w, (i * TPR + lane) * 8, cols);
+        fit(wv[i], (i * TPR + lane) * 8, cols);
+    }
+    if (AHEAD && row < rows) fetch(row);
     for (int k = 0; row < rows; row += step, k ^= 1) {     // (TPR > 64: the same row in all lanes of the workgroup)
+        if (!AHEAD) fetch(row);
         V yc[NCH], hc[NCH], uc[NCH];
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
@@ -243,15 +280,19 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_grad_kernel(con
             hc[i] = hv[i];
             if (dh) uc[i] = uv[i];
         }
-        if (row + step < rows) fetch(row + step);
+        if (AHEAD && row + step < rows) fetch(row + step);
         float ss = 0.f, dot = 0.f;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const V wv = load8(w, (i * TPR + lane) * 8, cols);
+            if ((i + 1) * TPR * 8 > cols) {                 // (uniform)
+                fit(yc[i], (i * TPR + lane) * 8, cols);
+                fit(hc[i], (i * TPR + lane) * 8, cols);
+                if (dh) fit(uc[i], (i * TPR + lane) * 8, cols);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 ss += (float)hc[i][j] * (float)hc[i][j];
-                dot += (float)yc[i][j] * (float)wv[j] * (float)hc[i][j];
+                dot += (float)yc[i][j] * (float)wv[i][j] * (float)hc[i][j];
             }
         }
         if constexpr (TPR > 64) {
@@ -275,33 +316,52 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_grad_kernel(con
         }
         const float r = 1.f / sqrtf(ss / (float)cols + eps);
         const float kk = dot * r * r / (float)cols;        // mean(dn n) r
+        if (!DW && lane == 0) part[row] = r;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const int c = (i * TPR + lane) * 8;
-            const V wv = load8(w, c, cols);
             V o;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float g = (float)yc[i][j], v = (float)hc[i][j];
-                dw[i][j] += g * (v * r);
-                o[j] = (T)((dh ? (float)uc[i][j] : 0.f) + r * (g * (float)wv[j] - v * kk));
+                if constexpr (DW) dw[i][j] += g * (v * r);
+                o[j] = (T)((dh ? (float)uc[i][j] : 0.f) + r * (g * (float)wv[i][j] - v * kk));
             }
             store8(dx + row * dx_rs, c, cols, o);
         }
     }
-    float* pr = part + ((int64_t)blockIdx.x * RPB + sub) * ((cols + 7) & ~7);
+    if constexpr (DW) {
+        const int ld = (cols + 7) & ~7;
+        float* pr = part + (int64_t)blockIdx.x * ld;
+        if constexpr (RPB > 1) {                            // the waves' shares are added up here, in their order
+            __shared__ f32x4 all[RPB][NCH][2][TPR];
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int c = (i * TPR + lane) * 8;
-        if (c < cols) {
-            *reinterpret_cast<f32x4*>(pr + c) = f32x4{dw[i][0], dw[i][1], dw[i][2], dw[i][3]};
-            *reinterpret_cast<f32x4*>(pr + c + 4) = f32x4{dw[i][4], dw[i][5], dw[i][6], dw[i][7]};
+            for (int i = 0; i < NCH; ++i) {
+                all[sub][i][0][lane] = f32x4{dw[i][0], dw[i][1], dw[i][2], dw[i][3]};
+                all[sub][i][1][lane] = f32x4{dw[i][4], dw[i][5], dw[i][6], dw[i][7]};
+            }
+            __syncthreads();
+            for (int i = sub; i < 2 * NCH; i += RPB) {
+                const int c = ((i >> 1) * TPR + lane) * 8 + (i & 1) * 4;
+                f32x4 s = all[0][i >> 1][i & 1][lane];
+#pragma unroll
+                for (int k = 1; k < RPB; ++k) s += all[k][i >> 1][i & 1][lane];
+                if (c < ld) *reinterpret_cast<f32x4*>(pr + c) = s;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int c = (i * TPR + lane) * 8;
+                if (c < cols) {
+                    *reinterpret_cast<f32x4*>(pr + c) = f32x4{dw[i][0], dw[i][1], dw[i][2], dw[i][3]};
+                    *reinterpret_cast<f32x4*>(pr + c + 4) = f32x4{dw[i][4], dw[i][5], dw[i][6], dw[i][7]};
+                }
+            }
         }
     }
 }
 
-// Longer rows: dx of one row per workgroup in two passes (dx may lie on dh), the row's r left in `rstd`; then
-// part[g][c] = sum of dy n over the rows of group g (a contiguous run), grid (ceil(cols / 256), groups).
+// Rows of more than 32768 columns: dx of one row per workgroup in two passes (dx may lie on dh), the row's r left in `rstd`.
 template <typename T>
 __global__ __launch_bounds__(256) void rmsnorm_grad_rows_kernel(const T* __restrict__ dy, int64_t dy_rs, const T* __restrict__ h,
                                                                 int64_t h_rs, const T* dh, int64_t dh_rs,
@@ -323,34 +383,48 @@ __global__ __launch_bounds__(256) void rmsnorm_grad_rows_kernel(const T* __restr
     }
     if (threadIdx.x == 0) rstd[row] = r;
 }
+// part[g][c] = sum of dy n over the rows of group g (a contiguous run) from the rows' r; 8 columns a lane, grid
+// (ceil(cols / 2048), groups)
 template <typename T>
 __global__ __launch_bounds__(256) void rmsnorm_dweight_rows_kernel(const T* __restrict__ dy, int64_t dy_rs, const T* __restrict__ h,
                                                                    int64_t h_rs, const float* __restrict__ rstd, float* __restrict__ part,
                                                                    int rows, int cols) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+    typedef typename vec8<T>::type V;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * 8;
     const int per = (rows + gridDim.y - 1) / gridDim.y;
     const int64_t r0 = (int64_t)blockIdx.y * per, r1 = min(r0 + per, (int64_t)rows);
-    float s = 0.f;
-    for (int64_t r = r0; r < r1; ++r) s += (float)dy[r * dy_rs + c] * ((float)h[r * h_rs + c] * rstd[r]);
-    part[(int64_t)blockIdx.y * ((cols + 7) & ~7) + c] = s;
+    float s[8] = {};
+#pragma unroll 2
+    for (int64_t r = r0; r < r1; ++r) {
+        V y = load8(dy + r * dy_rs, c, cols), v = load8(h + r * h_rs, c, cols);
+        fit(y, c, cols);
+        fit(v, c, cols);
+        const float k = rstd[r];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += (float)y[j] * ((float)v[j] * k);
+    }
+    if (c < cols) {
+        float* pr = part + (int64_t)blockIdx.y * ((cols + 7) & ~7) + c;
+        *reinterpret_cast<f32x4*>(pr) = f32x4{s[0], s[1], s[2], s[3]};
+        *reinterpret_cast<f32x4*>(pr + 4) = f32x4{s[4], s[5], s[6], s[7]};
+    }
 }
-// dw = sum of the partial rows: a workgroup takes 64 columns, 16 groups of 16 lanes take every 16th row each and are added
+// dw = sum of the partial rows: a workgroup takes 32 columns, 32 groups of 8 lanes take every 32nd row each and are added
 // up in a fixed order
 template <typename T>
 __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(const float* __restrict__ part, int parts, int cols, T* __restrict__ dw) {
-    __shared__ f32x4 red[16][16];
-    const int q = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 64 + q * 4, ld = (cols + 7) & ~7;
+    __shared__ f32x4 red[32][8];
+    const int q = threadIdx.x & 7, g = threadIdx.x >> 3, c = blockIdx.x * 32 + q * 4, ld = (cols + 7) & ~7;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     if (c < ld) {
 #pragma unroll 8
-        for (int i = g; i < parts; i += 16) s += *reinterpret_cast<const f32x4*>(part + (int64_t)i * ld + c);
+        for (int i = g; i < parts; i += 32) s += *reinterpret_cast<const f32x4*>(part + (int64_t)i * ld + c);
     }
     red[g][q] = s;
     __syncthreads();
     if (g == 0) {
 #pragma unroll
-        for (int i = 1; i < 16; ++i) s += red[i][q];
+        for (int i = 1; i < 32; ++i) s += red[i][q];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (c + j < cols) dw[c + j] = (T)s[j];
@@ -363,11 +437,14 @@ constexpr int REG_COLS = 65536;      // the longest row that is held in register
 // lanes per row: a wave where the rows alone fill the chip and a lane's share stays small (no barrier), else a workgroup
 constexpr int WAVE_COLS = 4096, GROUP_COLS = 8192;
 
-// the gradient's partial rows of dweight
+// The gradient's partial rows of dweight.  As many workgroups as are resident at once (by the kernels' registers), but at
+// least two rows each: a partial row is written and read again, as much as half a row of the matrices.
+constexpr int GRAD_COLS = 16384;     // the longest row of the gradient's one-pass form (512 lanes, 4 chunks each)
 int grad_parts(int rows, int cols) {
-    if (cols > REG_COLS) return rows < 256 ? rows : 256;
-    const int rpb = cols <= 1024 ? 4 : 1, groups = (rows + rpb - 1) / rpb;
-    return (groups < 768 ? groups : 768) * rpb;
+    if (cols > GRAD_COLS) return rows < 64 ? rows : 64;
+    const int rpb = cols <= 1024 ? 4 : 1, most = cols <= 2048 ? 1024 : cols <= 4096 ? 768 : cols <= 8192 ? 512 : 256;
+    const int groups = (rows + 2 * rpb - 1) / (2 * rpb);
+    return groups < most ? groups : most;
 }
 
 template <typename T, bool Q8>
@@ -415,29 +492,28 @@ int grad_launch(const void* dy, int64_t dy_rs, const void* h, int64_t h_rs, cons
     hipStream_t st = (hipStream_t)stream;
     const int parts = grad_parts(rows, cols);
     float* part = (float*)ws;
-#define FP_GRAD(TPR, NCH)                                                                                                        \
-    rmsnorm_grad_kernel<T, TPR, NCH><<<dim3((unsigned)(TPR < 256 ? parts / 4 : parts)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(   \
-        (const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh, dh_rs, (const T*)w, (T*)dx, dx_rs, part, rows, cols, eps)
+    float* rstd = part + (int64_t)parts * ((cols + 7) & ~7);
+#define FP_GRAD(TPR, NCH, AHEAD, DW, GRID, PART)                                                                        \
+    rmsnorm_grad_kernel<T, TPR, NCH, AHEAD, DW><<<dim3((unsigned)(GRID)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(        \
+        (const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh, dh_rs, (const T*)w, (T*)dx, dx_rs, PART, rows, cols, eps)
     const int nch = (cols + 7) / 8;
-    if (nch <= 64) FP_GRAD(64, 1);
-    else if (nch <= 128) FP_GRAD(64, 2);
-    else if (nch <= 256) FP_GRAD(256, 1);
-    else if (nch <= 512) FP_GRAD(256, 2);
-    else if (nch <= 1024) FP_GRAD(256, 4);
-    else if (nch <= 2048) FP_GRAD(1024, 2);
-    else if (nch <= 4096) FP_GRAD(1024, 4);
-    else if (nch <= 8192) FP_GRAD(1024, 8);
+    if (nch <= 64) FP_GRAD(64, 1, true, true, parts, part);
+    else if (nch <= 128) FP_GRAD(64, 2, true, true, parts, part);
+    else if (nch <= 256) FP_GRAD(256, 1, true, true, parts, part);
+    else if (nch <= 512) FP_GRAD(256, 2, true, true, parts, part);
+    else if (nch <= 1024) FP_GRAD(256, 4, true, true, parts, part);
+    else if (nch <= 2048) FP_GRAD(512, 4, false, true, parts, part);
     else {
-        float* rstd = part + (int64_t)parts * ((cols + 7) & ~7);
-        rmsnorm_grad_rows_kernel<T><<<dim3((unsigned)rows), dim3(256), 0, st>>>((const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh, dh_rs,
-                                                                               (const T*)w, (T*)dx, dx_rs, rstd, cols, eps);
+        if (nch <= 4096) FP_GRAD(1024, 4, false, false, rows, rstd);
+        else rmsnorm_grad_rows_kernel<T><<<dim3((unsigned)rows), dim3(256), 0, st>>>((const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh,
+                                                                                    dh_rs, (const T*)w, (T*)dx, dx_rs, rstd, cols, eps);
         FP_CHECK_LAUNCH();
-        rmsnorm_dweight_rows_kernel<T><<<dim3((unsigned)((cols + 255) / 256), (unsigned)parts), dim3(256), 0, st>>>(
+        rmsnorm_dweight_rows_kernel<T><<<dim3((unsigned)((nch + 255) / 256), (unsigned)parts), dim3(256), 0, st>>>(
             (const T*)dy, dy_rs, (const T*)h, h_rs, rstd, part, rows, cols);
     }
 #undef FP_GRAD
     FP_CHECK_LAUNCH();
-    rmsnorm_dweight_kernel<T><<<dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, st>>>(part, parts, cols, (T*)dw);
+    rmsnorm_dweight_kernel<T><<<dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, st>>>(part, parts, cols, (T*)dw);
     FP_CHECK_LAUNCH();
     return 0;
 }
@@ -467,7 +543,7 @@ extern "C" int fp_rmsnorm_residual_fp8(const void* x, int64_t x_row_stride, cons
 
 extern "C" int64_t fp_rmsnorm_residual_backward_workspace_bytes(int rows, int cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return ((int64_t)grad_parts(rows, cols) * (((int64_t)cols + 7) & ~7) + (cols > REG_COLS ? (int64_t)rows : 0)) * 4;
+    return ((int64_t)grad_parts(rows, cols) * (((int64_t)cols + 7) & ~7) + (cols > GRAD_COLS ? (int64_t)rows : 0)) * 4;
 }
 
 extern "C" int fp_rmsnorm_residual_backward_bf16(const void* dy, int64_t dy_row_stride, const void* h, int64_t h_row_stride,
