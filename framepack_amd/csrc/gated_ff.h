@@ -4,8 +4,8 @@
 
 enum { FF_BF16 = 0, FF_F16 = 1, FF_E4M3 = 2 };
 
-// h = act(x . wg^T * scales + bg) * (x . wu^T * scales + bu), operands 16-byte aligned with row strides of multiples of 16
-// bytes, K a multiple of 64 (e4m3: 128), F of 8; gate / up: the projections, or null.
+// h = act(x . wg^T * scales + bg) * (x . wu^T * scales + bu); x, wg, wu 16-byte aligned with row strides of multiples of 16
+// bytes, K a multiple of 64 (e4m3: 128); gate / up: the projections, or null.
 __attribute__((visibility("hidden"))) int fpi_glu(int type, const void* x, int64_t ldx, const float* xs, const void* wg, int64_t ldwg,
                                                   const float* gs, const void* wu, int64_t ldwu, const float* us, const void* bg,
                                                   const void* bu, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M,

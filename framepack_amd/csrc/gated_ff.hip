@@ -3,9 +3,13 @@
 // include/framepack_hip.h.
 //
 //   dg = dh u act'(g)   du = dh act(g)   dx = dg . Wg + du . Wu   dWg = dg^T . x   dWu = du^T . x   db = column sums
+#include <type_traits>
 #include "gated_ff.h"
 #include "gemm_pipeline.h"
+#include "row_access.h"
 
+extern "C" int64_t fp_gated_ff_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
+                                               int M, int F, int K);
 extern "C" int64_t fp_gated_ff_backward_workspace_bytes(int M, int F, int K);
 extern "C" int fp_gemm_bf16(const void*, int64_t, const void*, int, const void*, int64_t, const void*, void*, int64_t, int, int, int, int,
                             int, const void*, int64_t, const void*, void*);
@@ -37,18 +41,6 @@ __device__ __forceinline__ void act_grad(float v, int act, float& a, float& da) 
     da = s + (p == 0.f ? 0.f : v * p * dz);
 }
 
-// ---- any size, any strides: 64 x 64 output tiles, one element per load -------------------------------------------
-// For operands that the wide loads cannot read.  e4m3 operands are widened to bf16, which holds them exactly.
-template <typename TI> struct widen {
-    typedef TI type;
-    typedef TI vec8 __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ TI of(TI v) { return v; }
-};
-template <> struct widen<fp8e4> {
-    typedef bf16 type;
-    typedef bf16x8 vec8;
-    static __device__ __forceinline__ bf16 of(fp8e4 v) { return (bf16)__builtin_amdgcn_cvt_f32_fp8((int)v.bits, 0); }
-};
 struct GluCall {
     const void* x;
     int64_t ldx;
@@ -63,58 +55,121 @@ struct GluCall {
     int64_t ldp;
     int M, F, K, act;
 };
-template <typename TI, typename TO>
-__global__ __launch_bounds__(256) void glu_any_kernel(GluCall q) {
-    typedef typename widen<TI>::type TM;
-    typedef typename widen<TI>::vec8 TM8;
-    __shared__ __attribute__((aligned(16))) TM sa[64][40], sb[2][64][40];      // rows of 32, padded to 80 B
-    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
+
+// ---- few rows: both weights stream through once -------------------------------------------------------------------
+// 16 NC output columns a workgroup: its 4 waves share out K in steps of 128 bytes a row (neighbouring waves read
+// neighbouring lines), each multiplying 2 NC tiles of 16 weight rows by MT x 16 tokens straight from registers - no weight
+// is used twice, so nothing goes through LDS but the waves' sums at the end.  A lane holds twice 16 bytes of one row a step;
+// which bytes is the same for weights and tokens, so the order of K inside a step does not matter.  Bound by the weights'
+// bytes and, from 16 tokens on, by the tokens' lines, which every workgroup reads again from the L2: NC = 2 halves them.
+// Loads need the type's alignment only; the last, partial step of K goes element by element.
+__device__ __forceinline__ f32x4 mma(bf16, const u32x4& w, const u32x4& x, f32x4 c) {
+    return mfma16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), c);
+}
+__device__ __forceinline__ f32x4 mma(_Float16, const u32x4& w, const u32x4& x, f32x4 c) {
+    return mfma16(__builtin_bit_cast(h16x8, w), __builtin_bit_cast(h16x8, x), c);
+}
+__device__ __forceinline__ f32x4 mma(fp8e4, const u32x4& w, const u32x4& x, f32x4 c) {
+    typedef long l2 __attribute__((ext_vector_type(2)));
+    const l2 a = __builtin_bit_cast(l2, w), b = __builtin_bit_cast(l2, x);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(a[0], b[0], c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(a[1], b[1], c, 0, 0, 0);
+}
+template <typename TI, typename TO, int MT, int NC, int STEPS>
+__global__ __launch_bounds__(256) void glu_few_kernel(GluCall q) {
+    constexpr int NW = 4;
+    typedef u32x4 Q __attribute__((aligned(1)));
+    constexpr int STEP = 128 / (int)sizeof(TI), E = 16 / (int)sizeof(TI);      // elements of a step, of a 16-byte load
+    constexpr int G = 2 * NC;                                                  // weight tiles: tile g is matrix g & 1, columns 16 (g >> 1)
+    __shared__ float red[NW][G][MT][16 * 17];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-    f32x4 acc[2][2][2] = {};
-    auto stage = [&](TM (*dst)[40], const void* base, int64_t ld, int64_t r0, int rows, int k0) {
-        const TI* p = reinterpret_cast<const TI*>(base);
-        for (int i = tid; i < 64 * 32; i += 256) {
-            const int r = i >> 5, k = i & 31;
-            TM v = (TM)0.f;
-            if (r0 + r < rows && k0 + k < q.K) v = widen<TI>::of(p[(r0 + r) * ld + k0 + k]);
-            dst[r][k] = v;
-        }
-    };
-    for (int k0 = 0; k0 < q.K; k0 += 32) {
-        stage(sa, q.x, q.ldx, m0, q.M, k0);
-        stage(sb[0], q.w[0], q.ldw[0], n0, q.F, k0);
-        stage(sb[1], q.w[1], q.ldw[1], n0, q.F, k0);
-        __syncthreads();
+    const int row = lane & 15, ch = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NC);
+    const int m0 = blockIdx.y * (MT * 16);
+    const TI *pw[G], *px[MT];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const TM8 av = *reinterpret_cast<const TM8*>(&sa[wm + i * 16 + (lane & 15)][(lane >> 4) * 8]);
+    for (int g = 0; g < G; ++g)
+        pw[g] = reinterpret_cast<const TI*>(q.w[g & 1]) + min(n0 + (g >> 1) * 16 + row, (int64_t)q.F - 1) * q.ldw[g & 1] + ch * E;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+    for (int t = 0; t < MT; ++t) px[t] = reinterpret_cast<const TI*>(q.x) + (int64_t)min(m0 + t * 16 + row, q.M - 1) * q.ldx + ch * E;
+    f32x4 acc[G][MT] = {};
+    const int steps = q.K / STEP;
+    auto run = [&](auto U_, int s) {                           // the loads of U steps go out together
+        constexpr int U = decltype(U_)::value;
+        u32x4 w[U][G][2], x[U][MT][2];
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
-                    acc[g][i][j] = mfma16(*reinterpret_cast<const TM8*>(&sb[g][wn + j * 16 + (lane & 15)][(lane >> 4) * 8]), av, acc[g][i][j]);
-        }
-        __syncthreads();
-    }
-    // (operands swapped: the lane's low bits are the row, its four registers four columns)
+        for (int i = 0; i < U; ++i)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+            for (int c = 0; c < 2; ++c) {
+                const int64_t at = (int64_t)(s + i * NW) * STEP + c * (STEP / 2);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+                for (int g = 0; g < G; ++g) w[i][g][c] = *reinterpret_cast<const Q*>(pw[g] + at);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t m = m0 + wm + i * 16 + (lane & 15), n = n0 + wn + j * 16 + (lane >> 4) * 4 + e;
-                if (m >= q.M || n >= q.F) continue;
-                float v[2];
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    v[g] = acc[g][i][j][e] * (q.xs ? q.xs[m] * q.ws[g][n] : 1.f);
-                    if (q.b[g]) v[g] += (float)reinterpret_cast<const TO*>(q.b[g])[n];
-                    if (q.pre[g]) reinterpret_cast<TO*>(q.pre[g])[m * q.ldp + n] = (TO)v[g];
-                }
-                reinterpret_cast<TO*>(q.h)[m * q.ldh + n] = (TO)(act_of(v[0], q.act) * v[1]);
+                for (int t = 0; t < MT; ++t) x[i][t][c] = *reinterpret_cast<const Q*>(px[t] + at);
             }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) acc[g][t] = mma(TI{}, w[i][g][c], x[i][t][c], acc[g][t]);
+    };
+    int s = wave;
+    if constexpr (STEPS > 1)
+        for (; s + (STEPS - 1) * NW < steps; s += STEPS * NW) run(std::integral_constant<int, STEPS>{}, s);
+    for (; s < steps; s += NW) run(std::integral_constant<int, 1>{}, s);
+    if (steps * STEP < q.K && wave == steps % NW) {
+        auto part = [&](const TI* p, int c) {                  // 16 bytes of the step, zeros past the end of the row
+            TI v[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                v[j] = TI{};
+                if (steps * STEP + c * (STEP / 2) + ch * E + j < q.K) v[j] = p[(int64_t)steps * STEP + c * (STEP / 2) + j];
+            }
+            u32x4 o;
+            __builtin_memcpy(&o, v, 16);
+            return o;
+        };
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            u32x4 xv[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xv[t] = part(px[t], c);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const u32x4 wv = part(pw[g], c);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[g][t] = mma(TI{}, wv, xv[t], acc[g][t]);
+            }
+        }
+    }
+    // accumulators: the lane's low bits are the token, its four registers four columns
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[wave][g][t][(ch * 4 + e) * 17 + row] = acc[g][t][e];
+    __syncthreads();
+    for (int i = tid; i < NC * MT * 256; i += NW * 64) {
+        const int col = i & 15, nc = (i >> 4) % NC, tok = (i / (16 * NC)) & 15, t = i / (256 * NC);
+        const int64_t m = m0 + t * 16 + tok, nn = n0 + nc * 16 + col;
+        if (m >= q.M || nn >= q.F) continue;
+        float v[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            v[g] = red[0][2 * nc + g][t][col * 17 + tok];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) v[g] += red[w][2 * nc + g][t][col * 17 + tok];
+            if (sizeof(TI) == 1) v[g] *= q.xs[m] * q.ws[g][nn];
+            if (q.b[g]) v[g] += (float)reinterpret_cast<const TO*>(q.b[g])[nn];
+            if (q.pre[g]) reinterpret_cast<TO*>(q.pre[g])[m * q.ldp + nn] = (TO)v[g];
+        }
+        reinterpret_cast<TO*>(q.h)[m * q.ldh + nn] = (TO)(act_of(v[0], q.act) * v[1]);
+    }
 }
 
 // ---- the gradient -------------------------------------------------------------------------------------------------
@@ -125,18 +180,27 @@ __global__ __launch_bounds__(256) void glu_any_kernel(GluCall q) {
 constexpr int64_t up64(int64_t v) { return (v + 63) & ~(int64_t)63; }
 constexpr int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
 
-// 8 values of a row of `cols`, zeros behind its end; wide: 16-byte aligned rows
-template <typename T> struct vec8;
-template <> struct vec8<bf16> { typedef bf16x8 type; };
-template <> struct vec8<_Float16> { typedef h16x8 type; };
+// Up to three matrices of the same width into rows of Kp elements (a multiple of 64), zeros behind column K
+struct Copies {
+    const void* src[3];
+    void* dst[3];
+    int64_t ld[3];
+    int rows[3];                    // 0: not this one
+};
 template <typename T>
-__device__ __forceinline__ typename vec8<T>::type load8(const T* row, int c, int cols, bool wide) {
-    if (wide && c + 8 <= cols) return *reinterpret_cast<const typename vec8<T>::type*>(row + c);
-    typename vec8<T>::type v = {};
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (c + j < cols) v[j] = row[c + j];
-    return v;
+__global__ __launch_bounds__(256) void copy_rows_kernel(Copies q, int K, int Kp) {
+    const int per = Kp / 8;
+    const int64_t n0 = (int64_t)q.rows[0] * per, n1 = n0 + (int64_t)q.rows[1] * per, n2 = n1 + (int64_t)q.rows[2] * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n2; i += (int64_t)gridDim.x * 256) {
+        const int k = i < n0 ? 0 : i < n1 ? 1 : 2;
+        const int64_t at = i - (k == 0 ? 0 : k == 1 ? n0 : n1), r = at / per;
+        const int c = (int)(at - r * per) * 8;
+        const T* src = reinterpret_cast<const T*>(k == 0 ? q.src[0] : k == 1 ? q.src[1] : q.src[2]);
+        T* dst = reinterpret_cast<T*>(k == 0 ? q.dst[0] : k == 1 ? q.dst[1] : q.dst[2]);
+        typename vec8<T>::type v = load8(src + r * (k == 0 ? q.ld[0] : k == 1 ? q.ld[1] : q.ld[2]), c, K);
+        fit(v, c, K);
+        *reinterpret_cast<typename vec8<T>::type*>(dst + r * Kp + c) = v;
+    }
 }
 
 // A 64 x 64 tile in LDS, written by rows and read by columns: 16-byte chunks, the chunk index XORed with row / 8 so that the
@@ -157,11 +221,14 @@ __device__ __forceinline__ typename vec8<T>::type tile_get_t(const T* t, int col
 // cols to cols_p; grid (ceil(cols_p / 64), rows_p / 64)
 template <typename T>
 __device__ void transpose_tile(const T* __restrict__ src, int64_t ld_src, int rows, int cols, T* __restrict__ dst, int64_t ld_dst, int cols_p,
-                               int64_t r0, int c0, bool wide, T* tile) {
+                               int64_t r0, int c0, T* tile) {
     for (int i = threadIdx.x; i < 512; i += 256) {
         const int r = i >> 3, ch = i & 7;
         typename vec8<T>::type v = {};
-        if (r0 + r < rows) v = load8(src + (r0 + r) * ld_src, c0 + ch * 8, cols, wide);
+        if (r0 + r < rows) {
+            v = load8(src + (r0 + r) * ld_src, c0 + ch * 8, cols);
+            fit(v, c0 + ch * 8, cols);
+        }
         tile_put(tile, r, ch, v);
     }
     __syncthreads();
@@ -181,10 +248,8 @@ __global__ __launch_bounds__(256) void transpose_kernel(Transposes t, int cols_p
     __shared__ __attribute__((aligned(16))) T tile[64 * 64];
     int b = blockIdx.x, i = 0;
     while (i < 2 && b >= t.tiles[i]) b -= t.tiles[i++];
-    const T* src = (const T*)t.src[i];
-    const bool wide = ((uintptr_t)src & 15) == 0 && t.ld_src[i] % 8 == 0;
-    transpose_tile<T>(src, t.ld_src[i], t.rows[i], t.cols[i], (T*)t.dst[i], t.ld_dst[i], cols_p, (int64_t)(b / t.col_tiles[i]) * 64,
-                      b % t.col_tiles[i] * 64, wide, tile);
+    transpose_tile<T>((const T*)t.src[i], t.ld_src[i], t.rows[i], t.cols[i], (T*)t.dst[i], t.ld_dst[i], cols_p, (int64_t)(b / t.col_tiles[i]) * 64,
+                      b % t.col_tiles[i] * 64, tile);
 }
 
 // dg | du as [M, 2 Fp] and as [2 Fp, Mp], both zero-padded; colsum: the tile's column sums [row tile][2 Fp] (or null).
@@ -192,7 +257,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(Transposes t, int cols_p
 template <typename T>
 __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh, int64_t ldh, const T* __restrict__ gate, int64_t ldg,
                                                        const T* __restrict__ up, int64_t ldu, T* __restrict__ dgu, T* __restrict__ dgut,
-                                                       float* __restrict__ colsum, int M, int F, int Fp, int Mp, int act, bool wide) {
+                                                       float* __restrict__ colsum, int M, int F, int Fp, int Mp, int act) {
     typedef typename vec8<T>::type V;
     __shared__ __attribute__((aligned(16))) T tg[64 * 64], tu[64 * 64];
     __shared__ float cs[2][4][64];
@@ -205,8 +270,10 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh,
         const int64_t m = m0 + r;
         V og = {}, ou = {};
         if (m < M) {
-            const V d = load8(dh + m * ldh, f0 + ch * 8, F, wide), g = load8(gate + m * ldg, f0 + ch * 8, F, wide),
-                    u = load8(up + m * ldu, f0 + ch * 8, F, wide);
+            V d = load8(dh + m * ldh, f0 + ch * 8, F), g = load8(gate + m * ldg, f0 + ch * 8, F), u = load8(up + m * ldu, f0 + ch * 8, F);
+            fit(d, f0 + ch * 8, F);
+            fit(g, f0 + ch * 8, F);
+            fit(u, f0 + ch * 8, F);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float a, da;
@@ -333,35 +400,65 @@ int product(const T* a, int64_t lda, const T* w, int64_t ldw, T* out, int M, int
     return 0;
 }
 
+// Rows up to which the weights are streamed (glu_few_kernel).  [K, F] = [4096, 14336], streamed / matrix-core kernel, us:
+// bf16 45 / 70 at 1 row, 56 / 69 at 32, 64 / 71 at 48, 70 / 73 at 64; e4m3 21 / 30 at 1, 32 / 34 at 48, 37 / 35 at 64.
+constexpr int FEW = 48;
+constexpr int64_t FAR = int64_t(1) << 22;   // gemm_w4.h: 32-bit offsets within a tile
 constexpr int LIMIT = (1 << 21) - 64;      // M, F, K of the gradient: 2 Fp and Mp stay below gemm_w4.h's limit of 2^22 for a row stride
 
 bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool wide_rows(const void* p, int64_t ld, int K) { return aligned16(p) && ld % 8 == 0 && ld < FAR && K % 64 == 0; }
 
 template <typename TI, typename TO>
 int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64_t ldwg, const float* gs, const void* wu, int64_t ldwu,
               const float* us, const void* bg, const void* bu, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M, int F,
-              int K, int act, void* stream) {
+              int K, int act, void* ws, int64_t ws_bytes, void* stream) {
     FP_REQUIRE(x && wg && wu && h && M >= 0 && F > 0 && K > 0 && (act == 0 || act == 1) && !bg == !bu && !gate == !up);
     FP_REQUIRE(ldx >= 0 && ldwg >= K && ldwu >= K && ldh >= F && (!gate || ldp >= F));
     FP_REQUIRE(sizeof(TI) == 1 || (aligned2(x) && aligned2(wg) && aligned2(wu) && aligned2(h) && aligned2(bg) && aligned2(bu) &&
                                    aligned2(gate) && aligned2(up)));
     if (M == 0) return 0;
+    hipStream_t st = (hipStream_t)stream;
     constexpr int type = sizeof(TI) == 1 ? FF_E4M3 : __is_same(TI, bf16) ? FF_BF16 : FF_F16;
-    // the matrix-core kernel's loads and stores are 16 bytes wide and its K tiles whole
-    constexpr int V = 16 / (int)sizeof(TI);
-    const bool wide = aligned16(x) && aligned16(wg) && aligned16(wu) && aligned16(h) && aligned16(gate) && aligned16(up) &&
-                      ((uintptr_t)bg & 7) == 0 && ((uintptr_t)bu & 7) == 0 && ldx % V == 0 && ldwg % V == 0 && ldwu % V == 0 &&
-                      ldh % 8 == 0 && (!gate || ldp % 8 == 0) && K % (8 * V) == 0 && F % 8 == 0;
-    constexpr int64_t FAR = int64_t(1) << 22;             // gemm_w4.h: 32-bit offsets within a tile
-    if (wide && ldx < FAR && ldwg < FAR && ldwu < FAR)
-        return fpi_glu(type, x, ldx, xs, wg, ldwg, gs, wu, ldwu, us, bg, bu, h, ldh, gate, up, ldp, M, F, K, act, (hipStream_t)stream);
     const GluCall q{x, ldx, xs, {wg, wu}, {ldwg, ldwu}, {gs, us}, {bg, bu}, h, ldh, {gate, up}, ldp, M, F, K, act};
-    const dim3 grid((unsigned)((F + 63) / 64), (unsigned)((M + 63) / 64));
-    FP_REQUIRE(grid.y < 65536);
-    glu_any_kernel<TI, TO><<<grid, dim3(256), 0, (hipStream_t)stream>>>(q);
-    FP_CHECK_LAUNCH();
-    return 0;
+    if (M <= FEW) {
+        const int mt = (M + 15) / 16;
+        // two column tiles a workgroup where that leaves a workgroup per CU; one for the fewest tokens in 16 bits
+        const bool two = F >= 8192 && (M > 8 || sizeof(TI) == 1);
+#define FP_FEW(MT, NC, STEPS) glu_few_kernel<TI, TO, MT, NC, STEPS><<<dim3((unsigned)((F + 16 * NC - 1) / (16 * NC))), dim3(256), 0, st>>>(q)
+        if (mt == 1) {
+            if (two) FP_FEW(1, 2, 1);
+            else FP_FEW(1, 1, 2);
+        } else if (mt == 2) {
+            if (two) FP_FEW(2, 2, 1);
+            else FP_FEW(2, 1, 1);
+        } else {
+            if (two) FP_FEW(3, 2, 1);
+            else FP_FEW(3, 1, 1);
+        }
+#undef FP_FEW
+        FP_CHECK_LAUNCH();
+        return 0;
+    }
+    // The matrix-core kernel stages its operands 16 bytes a lane and in whole K tiles, with 32-bit offsets inside a tile: what
+    // does not fit that is copied into rows that do.
+    if constexpr (sizeof(TI) == 2) {
+        const bool x_fits = wide_rows(x, ldx, K), g_fits = wide_rows(wg, ldwg, K), u_fits = wide_rows(wu, ldwu, K);
+        if (!x_fits || !g_fits || !u_fits) {
+            const int64_t Kp = up64(K);
+            FP_REQUIRE(K <= LIMIT && F <= LIMIT && ws && aligned16(ws) &&
+                       ws_bytes >= fp_gated_ff_workspace_bytes(x, ldx, wg, ldwg, wu, ldwu, M, F, K));
+            TI *xp = (TI*)ws, *gp = xp + (x_fits ? 0 : M * Kp), *upk = gp + (g_fits ? 0 : F * Kp);
+            const Copies c{{x, wg, wu}, {xp, gp, upk}, {ldx, ldwg, ldwu}, {x_fits ? 0 : M, g_fits ? 0 : F, u_fits ? 0 : F}};
+            const int64_t chunks = ((int64_t)c.rows[0] + c.rows[1] + c.rows[2]) * (Kp / 8);
+            copy_rows_kernel<TI><<<dim3((unsigned)(chunks < 2048 * 256 ? (chunks + 255) / 256 : 2048)), dim3(256), 0, st>>>(c, K, (int)Kp);
+            FP_CHECK_LAUNCH();
+            return fpi_glu(type, x_fits ? x : xp, x_fits ? ldx : Kp, xs, g_fits ? wg : gp, g_fits ? ldwg : Kp, gs, u_fits ? wu : upk,
+                           u_fits ? ldwu : Kp, us, bg, bu, h, ldh, gate, up, ldp, M, F, (int)Kp, act, st);
+        }
+    }
+    return fpi_glu(type, x, ldx, xs, wg, ldwg, gs, wu, ldwu, us, bg, bu, h, ldh, gate, up, ldp, M, F, K, act, st);
 }
 
 template <typename T>
@@ -380,9 +477,8 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
     char* base = (char*)ws;
     T *dgu = (T*)(base + g.dgu), *dgut = (T*)(base + g.dgut), *wt = (T*)(base + g.wt), *xt = (T*)(base + g.xt);
     float *colsum = dbg ? (float*)(base + g.colsum) : nullptr, *parts = (float*)(base + g.parts);
-    const bool wide = aligned16(dh) && aligned16(gate) && aligned16(up) && ldh % 8 == 0 && ldg % 8 == 0 && ldu % 8 == 0;
     glu_grad_kernel<T><<<dim3((unsigned)(Fp / 64), (unsigned)(Mp / 64)), dim3(256), 0, st>>>(
-        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, Fp, Mp, act, wide);
+        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, Fp, Mp, act);
     FP_CHECK_LAUNCH();
     const Transposes t{{wg, wu, x},   {wt, wt + Fp, xt},  {ldwg, ldwu, ldx},
                        {2 * Fp, 2 * Fp, Mp}, {F, F, M}, {K, K, K}, {Fp / 64 * ktiles, Fp / 64 * ktiles, Mp / 64 * ktiles}, {ktiles, ktiles, ktiles}};
@@ -405,18 +501,28 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
 
 }  // namespace
 
+extern "C" int64_t fp_gated_ff_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
+                                               int M, int F, int K) {
+    if (M <= FEW || F <= 0 || K <= 0 || F > LIMIT || K > LIMIT) return 0;
+    const int64_t rows = (wide_rows(x, ldx, K) ? 0 : (int64_t)M) + (wide_rows(w_gate, ldwg, K) ? 0 : (int64_t)F) +
+                         (wide_rows(w_up, ldwu, K) ? 0 : (int64_t)F);
+    return rows * up64(K) * 2;
+}
+
 extern "C" int fp_gated_ff_bf16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
                                 const void* b_gate, const void* b_up, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M,
-                                int F, int K, int act, void* stream) {
+                                int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream) {
     return ff_launch<bf16, bf16>(x, ldx, nullptr, w_gate, ldwg, nullptr, w_up, ldwu, nullptr, b_gate, b_up, h, ldh, gate, up, ldp, M, F,
-                                 K, act, stream);
+                                 K, act, workspace,
+                                 workspace_bytes, stream);
 }
 
 extern "C" int fp_gated_ff_f16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
                                const void* b_gate, const void* b_up, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M,
-                               int F, int K, int act, void* stream) {
+                               int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream) {
     return ff_launch<_Float16, _Float16>(x, ldx, nullptr, w_gate, ldwg, nullptr, w_up, ldwu, nullptr, b_gate, b_up, h, ldh, gate, up,
-                                         ldp, M, F, K, act, stream);
+                                         ldp, M, F, K, act, workspace,
+                                 workspace_bytes, stream);
 }
 
 extern "C" int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, const void* w_gate, int64_t ldwg, const void* wg_scale,
@@ -427,7 +533,7 @@ extern "C" int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, 
                ldwu % 16 == 0 && ldh % 8 == 0 && ldx >= 0);
     FP_REQUIRE(((uintptr_t)x_scale & 3) == 0 && aligned16(wg_scale) && aligned16(wu_scale) && aligned16(b_gate) && aligned16(b_up));
     return ff_launch<fp8e4, bf16>(x, ldx, (const float*)x_scale, w_gate, ldwg, (const float*)wg_scale, w_up, ldwu,
-                                  (const float*)wu_scale, b_gate, b_up, h, ldh, nullptr, nullptr, 0, M, F, K, act, stream);
+                                  (const float*)wu_scale, b_gate, b_up, h, ldh, nullptr, nullptr, 0, M, F, K, act, nullptr, 0, stream);
 }
 
 extern "C" int64_t fp_gated_ff_backward_workspace_bytes(int M, int F, int K) {

@@ -16,7 +16,10 @@ int fpi_glu(int type, const void* x, int64_t ldx, const float* xs, const void* w
 #define FP_GLU(T, TO, NT, KEEP)                                                                                                   \
     return launch_w4<T, 0, 0, TO, NT, 0, 0, 0, 1, KEEP>(x, ldx, 0, K, wg, ldwg, bg, h, ldh, M, F, K, 0, nullptr, 0, nullptr, cg, st, \
                                                         xs, gs, QkNormArgs{}, Rows2{}, glu)
-    if (type == FF_E4M3) FP_GLU(fp8e4, bf16, 8, 0);
+    if (type == FF_E4M3) {
+        if (narrow) FP_GLU(fp8e4, bf16, 4, 0);
+        FP_GLU(fp8e4, bf16, 8, 0);
+    }
     if (type == FF_BF16) {
         if (gate) {
             if (narrow) FP_GLU(bf16, bf16, 4, 1);

@@ -556,9 +556,9 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         __builtin_amdgcn_s_barrier();
         fence();
         if constexpr (KS == 1) {
-            // fp8: 32 MFMAs of 32 cycles per phase, column tile n outermost (its W fragment arrives two tiles
-            // ahead, in the gaps), the half's four A fragments read up front; tiles n = 6, 7 are held back behind
-            // the next barrier like the 16-bit loop's last two groups.
+            // fp8: 4 NT MFMAs of 32 cycles per phase, column tile n outermost (its W fragment arrives two tiles
+            // ahead, in the gaps), the half's four A fragments read up front; the last two column tiles are held back
+            // behind the next barrier like the 16-bit loop's last two groups.
             if constexpr (P == 0) {
                 rd_w8(BUF, ic<0>{});
                 rd_w8(BUF, ic<1>{});
@@ -567,23 +567,33 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             fence();
             if constexpr (HAVE_PREV) {
                 static_for<2>([&](auto n) __attribute__((always_inline)) {
-                    static_for<4>([&](auto mi) __attribute__((always_inline)) { mfma8(ic<1 - P>{}, mi, ic<6 + n>{}, PZC); });
+                    static_for<4>([&](auto mi) __attribute__((always_inline)) { mfma8(ic<1 - P>{}, mi, ic<NT - 2 + n>{}, PZC); });
                 });
             }
             fence();
-            static_for<6>([&](auto n) __attribute__((always_inline)) {
+            static_for<NT - 2>([&](auto n) __attribute__((always_inline)) {
                 static_for<4>([&](auto mi) __attribute__((always_inline)) {
                     mfma8(P, mi, n, ZC);
                     fence();
-                    if constexpr (P == 0) {
-                        if constexpr (mi == 0) rd_w8(BUF, ic<n + 2>{});
-                        if constexpr (mi == 2 && n < 4) issue_a1(1, n, t + 1, ic<(BUF == 1)>{}, ic<-1>{});
-                    } else {
-                        if constexpr (mi == 0) {
-                            if constexpr (n < 4) issue_a1(0, n, t + 2, ic<(BUF == 0)>{}, ic<-1>{});
-                            else issue_w1(n - 4, t + 2, ic<-1>{});
+                    if constexpr (P == 0 && mi == 0) rd_w8(BUF, ic<n + 2>{});
+                    if constexpr (NT == 8) {
+                        if constexpr (P == 0) {
+                            if constexpr (mi == 2 && n < 4) issue_a1(1, n, t + 1, ic<(BUF == 1)>{}, ic<-1>{});
+                        } else {
+                            if constexpr (mi == 0) {
+                                if constexpr (n < 4) issue_a1(0, n, t + 2, ic<(BUF == 0)>{}, ic<-1>{});
+                                else issue_w1(n - 4, t + 2, ic<-1>{});
+                            }
+                            if constexpr (mi == 2) issue_w1(2 + n, t + 2, ic<-1>{});
                         }
-                        if constexpr (mi == 2) issue_w1(2 + n, t + 2, ic<-1>{});
+                    } else {                        // NT = 4: 8 gaps for the phase's 4 (P0) or 8 (P1) pieces
+                        constexpr int q = n * 4 + mi;
+                        if constexpr (P == 0) {
+                            if constexpr (q & 1) issue_a1(1, q >> 1, t + 1, ic<(BUF == 1)>{}, ic<-1>{});
+                        } else {
+                            if constexpr (q & 1) issue_w1(q >> 1, t + 2, ic<-1>{});
+                            else issue_a1(0, q >> 1, t + 2, ic<(BUF == 0)>{}, ic<-1>{});
+                        }
                     }
                     fence();
                 });
@@ -642,6 +652,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     };
     // GLU: lane (fr, fq) holds, for ni < NT / 2, both projections of row em0 + wr*128 + mi*16 + fr, columns en0 + wc * OCW +
     // ni*16 + 4 fq + (0..3).  Rows leave through the wave's stage as below, OCW columns (2 OCW bytes) a row; KEEP: three images.
+    typedef TO Tx8_any __attribute__((ext_vector_type(8), aligned(2)));
     auto glu_epilogue = [&](int em0, int en0) __attribute__((always_inline)) {
         unsigned stage_off = 2 * BUF_BYTES + wave * 8192;
         asm volatile("" : "+v"(stage_off));
@@ -653,15 +664,18 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         f32x4 ws[2][NT / 2];
 #pragma unroll
         for (int ni = 0; ni < NT / 2; ++ni) {
-            const int n = min(nb + ni * 16, N - 4);
+            const int n = nb + ni * 16;
             bv[0][ni] = bv[1][ni] = Tx4{0, 0, 0, 0};
             if (bias_) {
-                bv[0][ni] = *reinterpret_cast<const Tx4*>(bias_ + n);
-                bv[1][ni] = *reinterpret_cast<const Tx4*>(reinterpret_cast<const TO*>(glu.bias2) + n);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    bv[0][ni][j] = bias_[min(n + j, N - 1)];
+                    bv[1][ni][j] = reinterpret_cast<const TO*>(glu.bias2)[min(n + j, N - 1)];
+                }
             }
-            if (SCALED) {
-                ws[0][ni] = *reinterpret_cast<const f32x4*>(w_scale + n);
-                ws[1][ni] = *reinterpret_cast<const f32x4*>(glu.w_scale2 + n);
+            if (SCALED) {                                      // (N % 8 == 0 there)
+                ws[0][ni] = *reinterpret_cast<const f32x4*>(w_scale + min(n, N - 4));
+                ws[1][ni] = *reinterpret_cast<const f32x4*>(glu.w_scale2 + min(n, N - 4));
             }
         }
         const float c0 = glu_c0(glu.act), c1 = glu_c1(glu.act);
@@ -702,7 +716,16 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                 for (int i = 0; i < 16 / RPI; ++i) {
                     const int row = lrow + RPI * i;
                     const Tx8 ov = *reinterpret_cast<const Tx8*>(sb + img * IMG + row * (OCW * 2) + ((lchk ^ (row & (CPR - 1))) << 4));
-                    if (gcol < N && mrow0 + row < M) *reinterpret_cast<Tx8*>(dst + (int64_t)(mrow0 + row) * ld + gcol) = ov;
+                    if (gcol >= N || mrow0 + row >= M) continue;
+                    // (any row stride, base and N: the store needs the type's alignment only; a partial chunk goes by elements)
+                    TO* to = dst + (int64_t)(mrow0 + row) * ld + gcol;
+                    if (gcol + 8 <= N) {
+                        *reinterpret_cast<Tx8_any*>(to) = ov;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 7; ++j)
+                            if (gcol + j < N) to[j] = ov[j];
+                    }
                 }
             }
         });
@@ -875,7 +898,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
       }
     };
 
-    static_assert(KS == 2 || (KS == 1 && NT == 8), "16-bit MFMA 16x16x32 (two K steps per tile) or fp8 16x16x128 (one)");
+    static_assert(KS == 2 || (KS == 1 && (NT == 8 || NT == 4)), "16-bit MFMA 16x16x32 (two K steps per tile) or fp8 16x16x128 (one)");
     int vb = blockIdx.x;
     setup(vb);
     prologue();
@@ -904,7 +927,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         if constexpr (KS == 1) {
             auto tail = [&](auto PZC) __attribute__((always_inline)) {
                 static_for<2>([&](auto n) __attribute__((always_inline)) {
-                    static_for<4>([&](auto mi) __attribute__((always_inline)) { mfma8(ic<1>{}, mi, ic<6 + n>{}, PZC); });
+                    static_for<4>([&](auto mi) __attribute__((always_inline)) { mfma8(ic<1>{}, mi, ic<NT - 2 + n>{}, PZC); });
                 });
             };
             if (nk == 1) tail(ic<1>{});          // the only K tile's held-back tiles start from C = 0

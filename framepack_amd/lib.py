@@ -37,8 +37,9 @@ SIGNATURES = {
     "fp_rmsnorm_residual_backward_workspace_bytes": [I, I],
     "fp_rmsnorm_residual_backward_bf16": [P, L, P, L, P, L, P, P, L, P, I, I, F, P, L, P],
     "fp_rmsnorm_residual_backward_f16": [P, L, P, L, P, L, P, P, L, P, I, I, F, P, L, P],
-    "fp_gated_ff_bf16": [P, L, P, L, P, L, P, P, P, L, P, P, L, I, I, I, I, P],
-    "fp_gated_ff_f16": [P, L, P, L, P, L, P, P, P, L, P, P, L, I, I, I, I, P],
+    "fp_gated_ff_workspace_bytes": [P, L, P, L, P, L, I, I, I],
+    "fp_gated_ff_bf16": [P, L, P, L, P, L, P, P, P, L, P, P, L, I, I, I, I, P, L, P],
+    "fp_gated_ff_f16": [P, L, P, L, P, L, P, P, P, L, P, P, L, I, I, I, I, P, L, P],
     "fp_gated_ff_fp8": [P, L, P, P, L, P, P, L, P, P, P, P, L, I, I, I, I, P],
     "fp_gated_ff_backward_workspace_bytes": [I, I, I],
     "fp_gated_ff_backward_bf16": [P, L, P, L, P, L, P, L, P, L, P, L, P, P, P, P, P, I, I, I, I, P, L, P],

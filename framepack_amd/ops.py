@@ -896,8 +896,11 @@ def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: 
     if M > 0:
         lib = _lib.load()
         fn, name = (lib.fp_gated_ff_bf16, "fp_gated_ff_bf16") if x.dtype == BF16 else (lib.fp_gated_ff_f16, "fp_gated_ff_f16")
-        _lib.check(fn(x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, _ptr(bg), _ptr(bu), h2.data_ptr(), ldh,
-                      _ptr(gate), _ptr(up), F, M, F, K, act, _stream(x)), name)
+        xp, gp, up_ = x2.data_ptr(), g2.data_ptr(), u2.data_ptr()
+        n = lib.fp_gated_ff_workspace_bytes(xp, ldx, gp, ldg, up_, ldu, M, F, K)
+        ws = x.new_empty((n,), dtype=torch.uint8) if n else None
+        _lib.check(fn(xp, ldx, gp, ldg, up_, ldu, _ptr(bg), _ptr(bu), h2.data_ptr(), ldh, _ptr(gate), _ptr(up), F, M, F, K, act,
+                      _ptr(ws), n, _stream(x)), name)
     return (h, gate, up) if keep else h
 
 

@@ -135,10 +135,18 @@ def test_the_library_refuses_without_launching():
         refused("fp_rmsnorm_residual_backward_bf16", *[v if j == i else t for j, t in enumerate(ok)])
     assert L.fp_rmsnorm_residual_backward_workspace_bytes(0, 8) == 0 and L.fp_gated_ff_backward_workspace_bytes(4, 0, 8) == 0
     F, K = 16, 128
-    ok = [p, K, p, K, p, K, p, p, p, F, p, p, F, n, F, K, 0, None]
+    ok = [p, K, p, K, p, K, p, p, p, F, p, p, F, n, F, K, 0, None, 0, None]
     for i, v in ((0, None), (2, None), (4, None), (8, None), (6, None), (7, None), (10, None), (9, F - 1), (12, F - 1), (3, K - 1),
                  (13, -1), (14, 0), (15, 0), (16, 2)):
         refused("fp_gated_ff_bf16", *[v if j == i else t for j, t in enumerate(ok)])
+    size = L.fp_gated_ff_workspace_bytes
+    assert size(p, K, p, K, p, K, 49, F, K) == 0 and size(p + 2, K, p, K, p, K, 48, F, K) == 0
+    assert size(p + 2, K, p, K, p, K, 49, F, K) == 49 * K * 2 and size(p, K, p, K + 4, p, K, 49, F, K) == F * K * 2
+    assert size(p, K, p, K, p, K, 49, F, K - 1) == (49 + 2 * F) * K * 2
+    ok[13], ok[15] = 49, K - 1                              # a width that has to be copied: not without the space
+    refused("fp_gated_ff_bf16", *ok)
+    refused("fp_gated_ff_f16", *[p + 8 if j == 17 else 1 << 30 if j == 18 else t for j, t in enumerate(ok)])
+    refused("fp_gated_ff_f16", *[p if j == 17 else (49 + 2 * F) * K * 2 - 1 if j == 18 else t for j, t in enumerate(ok)])
     ok = [p, K, p, p, K, p, p, K, p, p, p, p, F, n, F, K, 0, None]
     for i, v in ((0, None), (2, None), (5, None), (8, None), (1, K + 8), (4, K + 8), (7, K + 8), (0, p + 8), (3, p + 8), (6, p + 8),
                  (11, p + 8), (12, F + 4), (14, 12), (15, 64), (5, p + 4), (9, p + 2), (9, None), (16, -1)):

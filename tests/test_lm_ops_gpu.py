@@ -257,7 +257,8 @@ def ff_tol(h, g, u, eg, eu, act, dtype):
 
 
 FF_SHAPES = [(1, 1, 1), (1, 8, 64), (1, 130, 100), (2, 7, 40), (5, 64, 64), (16, 72, 128), (17, 136, 192), (33, 264, 520), (64, 520, 64),
-             (65, 129, 72), (129, 256, 128), (257, 264, 256), (300, 1000, 1001), (513, 24, 320), (1, 4096, 1024), (7, 2056, 576)]
+             (65, 129, 72), (129, 256, 128), (257, 264, 256), (300, 1000, 1001), (513, 24, 320), (1, 4096, 1024), (7, 2056, 576),
+             (8, 8200, 72), (9, 8201, 64), (30, 8192, 130), (48, 8209, 200), (70, 8195, 128), (600, 8193, 192), (66, 7, 5)]
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -321,7 +322,7 @@ def quantised(t):
 
 @pytest.mark.parametrize("act", [ops.ACT_SILU, ops.ACT_GELU])
 @pytest.mark.parametrize("M,F,K", [(1, 8, 128), (1, 1040, 256), (3, 72, 128), (16, 136, 384), (17, 520, 128), (33, 64, 256), (65, 136, 512),
-                                   (130, 264, 128), (257, 128, 256), (300, 1000, 1152)])
+                                   (130, 264, 128), (257, 128, 256), (300, 1000, 1152), (2, 8200, 256), (20, 8192, 128), (64, 8216, 384)])
 def test_gated_ff_in_8_bits(M, F, K, act):
     x, xs = ops.quantize_rows_fp8(randn(M, K, seed=1, dtype=BF))
     wg, gs = quantised(randn(F, K, seed=2, scale=2 * K ** -0.5))
