@@ -11,6 +11,7 @@ __attribute__((visibility("hidden"))) int fpi_glu(int type, const void* x, int64
                                                   const void* bu, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M,
                                                   int F, int K, int act, hipStream_t st);
 
-// part[s] [M, N] fp32 = a [M, K] . w [N, K]^T over the K tiles (64) of part s: ks_per each, the last part the rest
-__attribute__((visibility("hidden"))) int fpi_gemm_parts(int type, const void* a, int64_t lda, const void* w, int64_t ldw, float* part,
+// part[s] [M, N] fp32 = a [M, K] . w [N, K]^T over the K tiles (64) of part s: ks_per each, the last part the rest;
+// narrow: 256 x 128 tiles instead of 256 x 256
+__attribute__((visibility("hidden"))) int fpi_gemm_parts(int type, bool narrow, const void* a, int64_t lda, const void* w, int64_t ldw, float* part,
                                                          int M, int N, int K, int splits, int ks_per, hipStream_t st);

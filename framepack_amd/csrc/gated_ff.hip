@@ -175,8 +175,8 @@ __global__ __launch_bounds__(256) void glu_few_kernel(GluCall q) {
 // ---- the gradient -------------------------------------------------------------------------------------------------
 // The products of the gradient contract over F (dx) and over the rows (dWg, dWu), the matrix-core kernel over the unit
 // stride of both operands: so dg | du is laid out both ways round by the kernel that computes it, and the weights and x
-// are transposed.  All of it is zero-padded to whole K tiles of 64 in the workspace, which also takes care of sizes and
-// strides that the wide loads cannot read.
+// are transposed.  Contracted lengths are zero-padded to whole K tiles of 64 in the workspace, which also takes care of
+// sizes and strides that the wide loads cannot read.
 constexpr int64_t up64(int64_t v) { return (v + 63) & ~(int64_t)63; }
 constexpr int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
 
@@ -217,52 +217,69 @@ __device__ __forceinline__ typename vec8<T>::type tile_get_t(const T* t, int col
     return v;
 }
 
-// dst[c][r] = src[r][c], dst [cols_p, ld] with rows zero-padded from `rows` to rows_p (a multiple of 64) and zero rows from
-// cols to cols_p; grid (ceil(cols_p / 64), rows_p / 64)
+// dst[c][r] = src[r][c] for r < rows_p (a multiple of 8; zeros from `rows` on) and c < cols_p (zeros from cols on)
+struct Transposes {                 // three of them in one launch, one after the other in blockIdx.x, 64 x 64 tiles
+    const void* src[3];
+    void* dst[3];
+    int64_t ld_src[3], ld_dst[3];
+    int rows[3], rows_p[3], tiles[3], cols, cols_p, col_tiles;
+};
+// behind them (if wanted) the biases' gradients: db = sum of the row tiles' column sums, 64 columns a block
+struct ColumnSums {
+    const float* sums;              // [tiles][2 S] (or null)
+    int tiles, F, S;
+    void *dbg, *dbu;
+};
 template <typename T>
-__device__ void transpose_tile(const T* __restrict__ src, int64_t ld_src, int rows, int cols, T* __restrict__ dst, int64_t ld_dst, int cols_p,
-                               int64_t r0, int c0, T* tile) {
+__global__ __launch_bounds__(256) void transpose_kernel(Transposes t, ColumnSums cs) {
+    __shared__ __attribute__((aligned(16))) T tile[64 * 64];
+    int b = blockIdx.x, k = 0;
+    while (k < 3 && b >= t.tiles[k]) b -= t.tiles[k++];
+    if (k == 3) {
+        float(*red)[64] = reinterpret_cast<float(*)[64]>(tile);
+        const int per = (cs.F + 63) / 64, half = b / per, l = threadIdx.x & 63, c = (b - half * per) * 64 + l, q = threadIdx.x >> 6;
+        float s = 0.f;
+        if (c < cs.F)
+            for (int i = q; i < cs.tiles; i += 4) s += cs.sums[(int64_t)i * (2 * cs.S) + half * cs.S + c];
+        red[q][l] = s;
+        __syncthreads();
+        if (q == 0 && c < cs.F) reinterpret_cast<T*>(half ? cs.dbu : cs.dbg)[c] = (T)((red[0][l] + red[1][l]) + (red[2][l] + red[3][l]));
+        return;
+    }
+    const T* src = reinterpret_cast<const T*>(t.src[k]);
+    T* dst = reinterpret_cast<T*>(t.dst[k]);
+    const int64_t r0 = (int64_t)(b / t.col_tiles) * 64;
+    const int c0 = b % t.col_tiles * 64;
     for (int i = threadIdx.x; i < 512; i += 256) {
         const int r = i >> 3, ch = i & 7;
         typename vec8<T>::type v = {};
-        if (r0 + r < rows) {
-            v = load8(src + (r0 + r) * ld_src, c0 + ch * 8, cols);
-            fit(v, c0 + ch * 8, cols);
+        if (r0 + r < t.rows[k]) {
+            v = load8(src + (r0 + r) * t.ld_src[k], c0 + ch * 8, t.cols);
+            fit(v, c0 + ch * 8, t.cols);
         }
         tile_put(tile, r, ch, v);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 512; i += 256) {
         const int c = i >> 3, ch = i & 7;
-        if (c0 + c < cols_p) *reinterpret_cast<typename vec8<T>::type*>(dst + (int64_t)(c0 + c) * ld_dst + r0 + ch * 8) = tile_get_t(tile, c, ch);
+        if (c0 + c < t.cols_p && r0 + ch * 8 < t.rows_p[k])
+            *reinterpret_cast<typename vec8<T>::type*>(dst + (int64_t)(c0 + c) * t.ld_dst[k] + r0 + ch * 8) = tile_get_t(tile, c, ch);
     }
 }
-struct Transposes {                 // up to three of them in one launch, one after the other in blockIdx.x
-    const void* src[3];
-    void* dst[3];
-    int64_t ld_src[3], ld_dst[3];
-    int rows[3], cols[3], tiles[3], col_tiles[3];
-};
-template <typename T>
-__global__ __launch_bounds__(256) void transpose_kernel(Transposes t, int cols_p) {
-    __shared__ __attribute__((aligned(16))) T tile[64 * 64];
-    int b = blockIdx.x, i = 0;
-    while (i < 2 && b >= t.tiles[i]) b -= t.tiles[i++];
-    transpose_tile<T>((const T*)t.src[i], t.ld_src[i], t.rows[i], t.cols[i], (T*)t.dst[i], t.ld_dst[i], cols_p, (int64_t)(b / t.col_tiles[i]) * 64,
-                      b % t.col_tiles[i] * 64, tile);
-}
 
-// dg | du as [M, 2 Fp] and as [2 Fp, Mp], both zero-padded; colsum: the tile's column sums [row tile][2 Fp] (or null).
-// Grid (Fp / 64, Mp / 64).  One read of dh, g, u; two writes of dg and du.
+// dg | du as rows [M, Kd] - dg from column 0, du from column S on, S = F rounded up to 8, zeros in the gaps and behind them
+// up to Kd - and as columns [2 S, Mp], zeros behind row M; colsum: the tile's column sums [row tile][2 S] (or null).
+// Grid (ceil(S / 64), Mp / 64).  One read of dh, g, u; two writes of dg and du.
 template <typename T>
 __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh, int64_t ldh, const T* __restrict__ gate, int64_t ldg,
                                                        const T* __restrict__ up, int64_t ldu, T* __restrict__ dgu, T* __restrict__ dgut,
-                                                       float* __restrict__ colsum, int M, int F, int Fp, int Mp, int act) {
+                                                       float* __restrict__ colsum, int M, int F, int S, int Kd, int Mp, int act) {
     typedef typename vec8<T>::type V;
     __shared__ __attribute__((aligned(16))) T tg[64 * 64], tu[64 * 64];
     __shared__ float cs[2][4][64];
     const int64_t m0 = (int64_t)blockIdx.y * 64;
-    const int f0 = blockIdx.x * 64, ch = threadIdx.x & 7;
+    const int f0 = blockIdx.x * 64, ch = threadIdx.x & 7, c = f0 + ch * 8;
+    const bool last = blockIdx.x == gridDim.x - 1;
     float sg[8] = {}, su[8] = {};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -270,23 +287,26 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh,
         const int64_t m = m0 + r;
         V og = {}, ou = {};
         if (m < M) {
-            V d = load8(dh + m * ldh, f0 + ch * 8, F), g = load8(gate + m * ldg, f0 + ch * 8, F), u = load8(up + m * ldu, f0 + ch * 8, F);
-            fit(d, f0 + ch * 8, F);
-            fit(g, f0 + ch * 8, F);
-            fit(u, f0 + ch * 8, F);
+            V d = load8(dh + m * ldh, c, F), g = load8(gate + m * ldg, c, F), u = load8(up + m * ldu, c, F);
+            fit(d, c, F);
+            fit(g, c, F);
+            fit(u, c, F);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 8; ++j) {                   // (zeros behind column F: dg = du = 0 there)
                 float a, da;
                 act_grad((float)g[j], act, a, da);
                 const float vg = (float)d[j] * (float)u[j] * da, vu = (float)d[j] * a;
-                const bool in = f0 + ch * 8 + j < F;
-                sg[j] += in ? vg : 0.f;
-                su[j] += in ? vu : 0.f;
-                og[j] = (T)(in ? vg : 0.f);
-                ou[j] = (T)(in ? vu : 0.f);
+                sg[j] += vg;
+                su[j] += vu;
+                og[j] = (T)vg;
+                ou[j] = (T)vu;
             }
-            *reinterpret_cast<V*>(dgu + m * (2 * (int64_t)Fp) + f0 + ch * 8) = og;
-            *reinterpret_cast<V*>(dgu + m * (2 * (int64_t)Fp) + Fp + f0 + ch * 8) = ou;
+            T* row = dgu + m * Kd;
+            if (c < S) {
+                *reinterpret_cast<V*>(row + c) = og;
+                *reinterpret_cast<V*>(row + S + c) = ou;
+            }
+            if (last && 2 * S + ch * 8 < Kd) *reinterpret_cast<V*>(row + 2 * S + ch * 8) = V{};
         }
         tile_put(tg, r, ch, og);
         tile_put(tu, r, ch, ou);
@@ -309,26 +329,15 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh,
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int f = (threadIdx.x >> 3) + 32 * i;
+        if (f0 + f >= S) break;
         *reinterpret_cast<V*>(dgut + (int64_t)(f0 + f) * Mp + m0 + ch * 8) = tile_get_t(tg, f, ch);
-        *reinterpret_cast<V*>(dgut + (int64_t)(Fp + f0 + f) * Mp + m0 + ch * 8) = tile_get_t(tu, f, ch);
+        *reinterpret_cast<V*>(dgut + (int64_t)(S + f0 + f) * Mp + m0 + ch * 8) = tile_get_t(tu, f, ch);
     }
     if (colsum && threadIdx.x < 128) {
-        const int w = threadIdx.x >> 6, c = threadIdx.x & 63;
-        colsum[(int64_t)blockIdx.y * (2 * Fp) + w * Fp + f0 + c] = (cs[w][0][c] + cs[w][1][c]) + (cs[w][2][c] + cs[w][3][c]);
+        const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
+        if (f0 + l < S)
+            colsum[(int64_t)blockIdx.y * (2 * S) + w * S + f0 + l] = (cs[w][0][l] + cs[w][1][l]) + (cs[w][2][l] + cs[w][3][l]);
     }
-}
-// db = sum of the row tiles' column sums; grid (ceil(F / 64), 2), four lanes rows apart per column
-template <typename T>
-__global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ colsum, int tiles, int F, int Fp, T* __restrict__ dbg,
-                                                        T* __restrict__ dbu) {
-    __shared__ float red[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-    float s = 0.f;
-    if (c < F)
-        for (int t = q; t < tiles; t += 4) s += colsum[(int64_t)t * (2 * Fp) + blockIdx.y * Fp + c];
-    red[q][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (q == 0 && c < F) (blockIdx.y ? dbu : dbg)[c] = (T)((red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
 }
 // out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns
 template <typename T>
@@ -346,17 +355,20 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict_
 }
 
 // How a product [M, N] over K (a multiple of 64) is cut: whole (0 parts: straight to 16 bits) where its 256 x 256 tiles fill
-// half the chip or more, else into parts of K of at least 4 tiles until they do.  N % 8 != 0: always through 32 bits (the
-// 16-bit stores are 16 bytes wide).
+// half the chip, else 256 x 128 tiles in parts of K of at least 8 tiles, as many as there are CUs.  N % 8 != 0: always
+// through 32 bits (the 16-bit stores are 16 bytes wide).
 struct Cut {
     int splits, ks_per;
 };
 Cut cut(int64_t M, int N, int K) {
-    const int64_t tiles = (M + 255) / 256 * ((N + 255) / 256);
+    const int64_t tm = (M + 255) / 256;
     const int nk = K / 64;
-    int64_t s = tiles >= 128 ? 1 : 256 / tiles;
-    if (s > nk / 4) s = nk / 4;
-    if (s < 1) s = 1;
+    int64_t s = 1;
+    if (tm * ((N + 255) / 256) < 128) {
+        s = 256 / (tm * ((N + 127) / 128));
+        if (s > nk / 8) s = nk / 8;
+        if (s < 1) s = 1;
+    }
     const int per = (int)((nk + s - 1) / s);
     const int splits = (nk + per - 1) / per;
     return {splits == 1 && N % 8 == 0 ? 0 : splits, per};
@@ -367,7 +379,7 @@ struct GradSpace {                  // byte offsets in the workspace, each a mul
     int64_t dgu, dgut, wt, xt, colsum, parts, end;
 };
 GradSpace grad_space(int64_t M, int64_t F, int64_t K) {
-    const int64_t Fp = up64(F), Mp = up64(M), Kp = up8(K);
+    const int64_t S = up8(F), Kd = up64(2 * S), Mp = up64(M), Kp = up8(K);
     GradSpace g;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -375,12 +387,12 @@ GradSpace grad_space(int64_t M, int64_t F, int64_t K) {
         at += (bytes + 255) & ~(int64_t)255;
         return o;
     };
-    g.dgu = take(M * 2 * Fp * 2);
-    g.dgut = take(2 * Fp * Mp * 2);
-    g.wt = take(Kp * 2 * Fp * 2);
+    g.dgu = take(M * Kd * 2);
+    g.dgut = take(2 * S * Mp * 2);
+    g.wt = take(Kp * Kd * 2);
     g.xt = take(Kp * Mp * 2);
-    g.colsum = take(Mp / 64 * 2 * Fp * 4);
-    const int64_t a = cut_bytes(M, (int)K, (int)(2 * Fp)), b = cut_bytes(F, (int)K, (int)Mp), c = cut_bytes(2 * F, (int)K, (int)Mp);
+    g.colsum = take(Mp / 64 * 2 * S * 4);
+    const int64_t a = cut_bytes(M, (int)K, (int)Kd), b = cut_bytes(F, (int)K, (int)Mp), c = cut_bytes(2 * F, (int)K, (int)Mp);
     g.parts = take(a > b ? (a > c ? a : c) : (b > c ? b : c));
     g.end = at;
     return g;
@@ -390,11 +402,11 @@ GradSpace grad_space(int64_t M, int64_t F, int64_t K) {
 template <typename T>
 int product(const T* a, int64_t lda, const T* w, int64_t ldw, T* out, int M, int N, int K, float* parts, hipStream_t st) {
     constexpr int type = sizeof(T) == 2 && __is_same(T, bf16) ? FF_BF16 : FF_F16;
-    const Cut c = cut(M, N, K);
+    const Cut c = cut(M, N, K);         // (splits > 1 means few tiles: the narrow tile)
     if (c.splits == 0)
         return (type == FF_BF16 ? fp_gemm_bf16 : fp_gemm_f16)(a, lda, nullptr, 0, w, ldw, nullptr, out, N, M, N, K, 0, 0, nullptr, 0, nullptr, st);
     const int Np = (int)up8(N);
-    if (int rc = fpi_gemm_parts(type, a, lda, w, ldw, parts, M, Np, K, c.splits, c.ks_per, st)) return rc;
+    if (int rc = fpi_gemm_parts(type, c.splits > 1, a, lda, w, ldw, parts, M, Np, K, c.splits, c.ks_per, st)) return rc;
     add_parts_kernel<T><<<dim3((unsigned)(((int64_t)M * (Np / 4) + 255) / 256)), dim3(256), 0, st>>>(parts, c.splits, out, M, N, Np);
     FP_CHECK_LAUNCH();
     return 0;
@@ -404,7 +416,7 @@ int product(const T* a, int64_t lda, const T* w, int64_t ldw, T* out, int M, int
 // bf16 45 / 70 at 1 row, 56 / 69 at 32, 64 / 71 at 48, 70 / 73 at 64; e4m3 21 / 30 at 1, 32 / 34 at 48, 37 / 35 at 64.
 constexpr int FEW = 48;
 constexpr int64_t FAR = int64_t(1) << 22;   // gemm_w4.h: 32-bit offsets within a tile
-constexpr int LIMIT = (1 << 21) - 64;      // M, F, K of the gradient: 2 Fp and Mp stay below gemm_w4.h's limit of 2^22 for a row stride
+constexpr int LIMIT = (1 << 21) - 64;      // M, F, K of the gradient: Kd and Mp stay below gemm_w4.h's limit of 2^22 for a row stride
 
 bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -473,30 +485,24 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
     FP_REQUIRE(ws && aligned16(ws) && ws_bytes >= fp_gated_ff_backward_workspace_bytes(M, F, K));
     hipStream_t st = (hipStream_t)stream;
     const GradSpace g = grad_space(M, F, K);
-    const int Fp = (int)up64(F), Mp = (int)up64(M), Kp = (int)up8(K), ktiles = (K + 63) / 64;
+    const int S = (int)up8(F), Kd = (int)up64(2 * S), Mp = (int)up64(M), Kp = (int)up8(K), ktiles = (Kp + 63) / 64;
     char* base = (char*)ws;
     T *dgu = (T*)(base + g.dgu), *dgut = (T*)(base + g.dgut), *wt = (T*)(base + g.wt), *xt = (T*)(base + g.xt);
     float *colsum = dbg ? (float*)(base + g.colsum) : nullptr, *parts = (float*)(base + g.parts);
-    glu_grad_kernel<T><<<dim3((unsigned)(Fp / 64), (unsigned)(Mp / 64)), dim3(256), 0, st>>>(
-        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, Fp, Mp, act);
+    glu_grad_kernel<T><<<dim3((unsigned)((S + 63) / 64), (unsigned)(Mp / 64)), dim3(256), 0, st>>>(
+        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, S, Kd, Mp, act);
     FP_CHECK_LAUNCH();
-    const Transposes t{{wg, wu, x},   {wt, wt + Fp, xt},  {ldwg, ldwu, ldx},
-                       {2 * Fp, 2 * Fp, Mp}, {F, F, M}, {K, K, K}, {Fp / 64 * ktiles, Fp / 64 * ktiles, Mp / 64 * ktiles}, {ktiles, ktiles, ktiles}};
-    transpose_kernel<T><<<dim3((unsigned)(t.tiles[0] + t.tiles[1] + t.tiles[2])), dim3(256), 0, st>>>(t, Kp);
+    const int up_rows = Kd - S;
+    const Transposes t{{wg, wu, x}, {wt, wt + S, xt}, {ldwg, ldwu, ldx}, {Kd, Kd, Mp}, {F, F, M}, {S, up_rows, Mp},
+                       {(S + 63) / 64 * ktiles, (up_rows + 63) / 64 * ktiles, Mp / 64 * ktiles}, K, Kp, ktiles};
+    const ColumnSums cs{colsum, Mp / 64, F, S, dbg, dbu};
+    transpose_kernel<T><<<dim3((unsigned)(t.tiles[0] + t.tiles[1] + t.tiles[2] + (dbg ? 2 * ((F + 63) / 64) : 0))), dim3(256), 0, st>>>(t, cs);
     FP_CHECK_LAUNCH();
-    if (int rc = product<T>(dgu, 2 * Fp, wt, 2 * Fp, (T*)dx, M, K, 2 * Fp, parts, st)) return rc;
+    if (int rc = product<T>(dgu, Kd, wt, Kd, (T*)dx, M, K, Kd, parts, st)) return rc;
     // (dWg over dWu in one product where they are the halves of one matrix)
-    if (Fp == F && (T*)dwu == (T*)dwg + (int64_t)F * K) {
-        if (int rc = product<T>(dgut, Mp, xt, Mp, (T*)dwg, 2 * F, K, Mp, parts, st)) return rc;
-    } else {
-        if (int rc = product<T>(dgut, Mp, xt, Mp, (T*)dwg, F, K, Mp, parts, st)) return rc;
-        if (int rc = product<T>(dgut + (int64_t)Fp * Mp, Mp, xt, Mp, (T*)dwu, F, K, Mp, parts, st)) return rc;
-    }
-    if (dbg) {
-        bias_grad_kernel<T><<<dim3((unsigned)(Fp / 64), 2), dim3(256), 0, st>>>(colsum, Mp / 64, F, Fp, (T*)dbg, (T*)dbu);
-        FP_CHECK_LAUNCH();
-    }
-    return 0;
+    if (S == F && (T*)dwu == (T*)dwg + (int64_t)F * K) return product<T>(dgut, Mp, xt, Mp, (T*)dwg, 2 * F, K, Mp, parts, st);
+    if (int rc = product<T>(dgut, Mp, xt, Mp, (T*)dwg, F, K, Mp, parts, st)) return rc;
+    return product<T>(dgut + (int64_t)S * Mp, Mp, xt, Mp, (T*)dwu, F, K, Mp, parts, st);
 }
 
 }  // namespace
