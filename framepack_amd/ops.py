@@ -37,13 +37,16 @@ def _dev(*ts: Optional[torch.Tensor]) -> None:
     for t in ts:
         if t is None:
             continue
+        d = t.get_device()                         # -1: CPU
+        if d == cur:
+            continue
         if not t.is_cuda:
             raise RuntimeError("framepack_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
         if cur is None:
             cur = torch.cuda.current_device()
-        if t.device.index != cur:
-            raise RuntimeError(f"tensor on cuda:{t.device.index} but the current device is cuda:{cur}: "
-                               f"wrap the call in `with torch.cuda.device({t.device.index}):`")
+        if d != cur:
+            raise RuntimeError(f"tensor on cuda:{d} but the current device is cuda:{cur}: "
+                               f"wrap the call in `with torch.cuda.device({d}):`")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -719,7 +722,11 @@ def _out(t: Optional[torch.Tensor], what: str, dtype, rows: int, cols: int, like
     """An output matrix (as returned, 2-d view, row stride): allocated if None, else of this type and size with rows that do
     not overlap each other."""
     if t is None:
-        t = like.new_empty((rows, cols), dtype=dtype)
+        # (empty_like of a contiguous tensor of this very shape is the quickest to come by)
+        if like.dtype is dtype and like.shape == (rows, cols) and like.is_contiguous():
+            t = torch.empty_like(like)
+        else:
+            t = like.new_empty((rows, cols), dtype=dtype)
         return t, t, cols if rows > 1 else (cols + 15) // 16 * 16
     t2, _, _, rs = _mat(t, what, (dtype,), rows, cols)
     if rs < cols:
