@@ -11,7 +11,15 @@ __attribute__((visibility("hidden"))) int fpi_glu(int type, const void* x, int64
                                                   const void* bu, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M,
                                                   int F, int K, int act, hipStream_t st);
 
-// part[s] [M, N] fp32 = a [M, K] . w [N, K]^T over the K tiles (64) of part s: ks_per each, the last part the rest;
-// narrow: 256 x 128 tiles instead of 256 x 256
-__attribute__((visibility("hidden"))) int fpi_gemm_parts(int type, bool narrow, const void* a, int64_t lda, const void* w, int64_t ldw, float* part,
-                                                         int M, int N, int K, int splits, int ks_per, hipStream_t st);
+// The gradient's products: out [M, N] = a [M, K] . w with w's K tiles as they lie, 64 rows of N each; tile t at w + t tiles,
+// + d1 bytes from tile s1 on, + d2 from tile s2 on (gemm_w4.h, TrArgs).  out in 16 bits (splits = 0; row stride N, 16-byte
+// aligned) or fp32 parts [splits][M, N] over ks_per K tiles each.  narrow: 256 x 128 tiles instead of 256 x 256 (as the
+// parts have).  K % 64 == 0, N % 8 == 0.
+struct GradProduct {
+    bool narrow;
+    const void *a, *w;
+    int64_t lda, ldw, d1, d2;
+    int s1, s2, M, N, K, splits, ks_per;
+    void* out;
+};
+__attribute__((visibility("hidden"))) int fpi_grad_product(int type, const GradProduct& p, hipStream_t st);

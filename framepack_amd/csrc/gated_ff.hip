@@ -10,11 +10,8 @@
 
 extern "C" int64_t fp_gated_ff_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
                                                int M, int F, int K);
-extern "C" int64_t fp_gated_ff_backward_workspace_bytes(int M, int F, int K);
-extern "C" int fp_gemm_bf16(const void*, int64_t, const void*, int, const void*, int64_t, const void*, void*, int64_t, int, int, int, int,
-                            int, const void*, int64_t, const void*, void*);
-extern "C" int fp_gemm_f16(const void*, int64_t, const void*, int, const void*, int64_t, const void*, void*, int64_t, int, int, int, int,
-                           int, const void*, int64_t, const void*, void*);
+extern "C" int64_t fp_gated_ff_backward_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up,
+                                                        int64_t ldwu, int M, int F, int K);
 
 namespace {
 
@@ -173,33 +170,57 @@ __global__ __launch_bounds__(256) void glu_few_kernel(GluCall q) {
 }
 
 // ---- the gradient -------------------------------------------------------------------------------------------------
-// The products of the gradient contract over F (dx) and over the rows (dWg, dWu), the matrix-core kernel over the unit
-// stride of both operands: so dg | du is laid out both ways round by the kernel that computes it, and the weights and x
-// are transposed.  Contracted lengths are zero-padded to whole K tiles of 64 in the workspace, which also takes care of
-// sizes and strides that the wide loads cannot read.
+// The products of the gradient contract over F (dx) and over the rows (dWg, dWu): along the rows of the weights, of x and of
+// dg | du.  The matrix-core kernel takes one such operand as it lies and transposes it on the way into registers (gemm_w4.h,
+// TrArgs): the weights and x.  dg | du is written both ways round by the kernel that computes it.  4096 rows, [4096, 11008]: the
+// two products take 537 us each, with weights and x transposed beforehand 516 us each and 95 us more for that; with dg | du
+// transposed in registers too 622 us for dW (those reads run at half the rate and both operands' fill the LDS pipe) against
+// 29 us for writing it twice.
+// What is contracted is padded to whole K tiles of 64: dg | du by the kernel that computes it, the others' last tile by a
+// copy of its own.
 constexpr int64_t up64(int64_t v) { return (v + 63) & ~(int64_t)63; }
 constexpr int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
 
-// Up to three matrices of the same width into rows of Kp elements (a multiple of 64), zeros behind column K
+// Up to three matrices of the same width into zero-padded rows of their own stride; behind them (if wanted) the biases'
+// gradients: db = sum of the row tiles' column sums, 64 columns a block.
 struct Copies {
     const void* src[3];
     void* dst[3];
-    int64_t ld[3];
-    int rows[3];                    // 0: not this one
+    int64_t ld_src[3], ld_dst[3];
+    int rows[3], rows_p[3];         // rows of the source, rows written (0: not this one)
+    int cols, cols_p;               // columns of the source, columns written (a multiple of 8)
+    int64_t chunks;                 // of all of them: 8 columns each
+    unsigned blocks;                // that copy; the others add up column sums
+    const float* sums;              // [tiles][2 Fp]
+    int tiles, F, Fp;
+    void* db;                       // [2 F]
 };
 template <typename T>
-__global__ __launch_bounds__(256) void copy_rows_kernel(Copies q, int K, int Kp) {
-    const int per = Kp / 8;
-    const int64_t n0 = (int64_t)q.rows[0] * per, n1 = n0 + (int64_t)q.rows[1] * per, n2 = n1 + (int64_t)q.rows[2] * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n2; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void copy_rows_kernel(Copies q) {
+    if (blockIdx.x >= q.blocks) {
+        __shared__ float red[4][64];
+        const int b = blockIdx.x - q.blocks, per = (q.F + 63) / 64, half = b / per, l = threadIdx.x & 63, c = (b - half * per) * 64 + l,
+                  w = threadIdx.x >> 6;
+        float s = 0.f;
+        if (c < q.F)
+            for (int i = w; i < q.tiles; i += 4) s += q.sums[(int64_t)i * (2 * q.Fp) + half * q.Fp + c];
+        red[w][l] = s;
+        __syncthreads();
+        if (w == 0 && c < q.F) reinterpret_cast<T*>(q.db)[half * q.F + c] = (T)((red[0][l] + red[1][l]) + (red[2][l] + red[3][l]));
+        return;
+    }
+    const int per = q.cols_p / 8;
+    const int64_t n0 = (int64_t)q.rows_p[0] * per, n1 = n0 + (int64_t)q.rows_p[1] * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < q.chunks; i += (int64_t)q.blocks * 256) {
         const int k = i < n0 ? 0 : i < n1 ? 1 : 2;
         const int64_t at = i - (k == 0 ? 0 : k == 1 ? n0 : n1), r = at / per;
         const int c = (int)(at - r * per) * 8;
-        const T* src = reinterpret_cast<const T*>(k == 0 ? q.src[0] : k == 1 ? q.src[1] : q.src[2]);
-        T* dst = reinterpret_cast<T*>(k == 0 ? q.dst[0] : k == 1 ? q.dst[1] : q.dst[2]);
-        typename vec8<T>::type v = load8(src + r * (k == 0 ? q.ld[0] : k == 1 ? q.ld[1] : q.ld[2]), c, K);
-        fit(v, c, K);
-        *reinterpret_cast<typename vec8<T>::type*>(dst + r * Kp + c) = v;
+        typename vec8<T>::type v = {};
+        if (r < q.rows[k]) {
+            v = load8(reinterpret_cast<const T*>(q.src[k]) + r * q.ld_src[k], c, q.cols);
+            fit(v, c, q.cols);
+        }
+        *reinterpret_cast<typename vec8<T>::type*>(reinterpret_cast<T*>(q.dst[k]) + r * q.ld_dst[k] + c) = v;
     }
 }
 
@@ -217,69 +238,18 @@ __device__ __forceinline__ typename vec8<T>::type tile_get_t(const T* t, int col
     return v;
 }
 
-// dst[c][r] = src[r][c] for r < rows_p (a multiple of 8; zeros from `rows` on) and c < cols_p (zeros from cols on)
-struct Transposes {                 // three of them in one launch, one after the other in blockIdx.x, 64 x 64 tiles
-    const void* src[3];
-    void* dst[3];
-    int64_t ld_src[3], ld_dst[3];
-    int rows[3], rows_p[3], tiles[3], cols, cols_p, col_tiles;
-};
-// behind them (if wanted) the biases' gradients: db = sum of the row tiles' column sums, 64 columns a block
-struct ColumnSums {
-    const float* sums;              // [tiles][2 S] (or null)
-    int tiles, F, S;
-    void *dbg, *dbu;
-};
-template <typename T>
-__global__ __launch_bounds__(256) void transpose_kernel(Transposes t, ColumnSums cs) {
-    __shared__ __attribute__((aligned(16))) T tile[64 * 64];
-    int b = blockIdx.x, k = 0;
-    while (k < 3 && b >= t.tiles[k]) b -= t.tiles[k++];
-    if (k == 3) {
-        float(*red)[64] = reinterpret_cast<float(*)[64]>(tile);
-        const int per = (cs.F + 63) / 64, half = b / per, l = threadIdx.x & 63, c = (b - half * per) * 64 + l, q = threadIdx.x >> 6;
-        float s = 0.f;
-        if (c < cs.F)
-            for (int i = q; i < cs.tiles; i += 4) s += cs.sums[(int64_t)i * (2 * cs.S) + half * cs.S + c];
-        red[q][l] = s;
-        __syncthreads();
-        if (q == 0 && c < cs.F) reinterpret_cast<T*>(half ? cs.dbu : cs.dbg)[c] = (T)((red[0][l] + red[1][l]) + (red[2][l] + red[3][l]));
-        return;
-    }
-    const T* src = reinterpret_cast<const T*>(t.src[k]);
-    T* dst = reinterpret_cast<T*>(t.dst[k]);
-    const int64_t r0 = (int64_t)(b / t.col_tiles) * 64;
-    const int c0 = b % t.col_tiles * 64;
-    for (int i = threadIdx.x; i < 512; i += 256) {
-        const int r = i >> 3, ch = i & 7;
-        typename vec8<T>::type v = {};
-        if (r0 + r < t.rows[k]) {
-            v = load8(src + (r0 + r) * t.ld_src[k], c0 + ch * 8, t.cols);
-            fit(v, c0 + ch * 8, t.cols);
-        }
-        tile_put(tile, r, ch, v);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 512; i += 256) {
-        const int c = i >> 3, ch = i & 7;
-        if (c0 + c < t.cols_p && r0 + ch * 8 < t.rows_p[k])
-            *reinterpret_cast<typename vec8<T>::type*>(dst + (int64_t)(c0 + c) * t.ld_dst[k] + r0 + ch * 8) = tile_get_t(tile, c, ch);
-    }
-}
-
-// dg | du as rows [M, Kd] - dg from column 0, du from column S on, S = F rounded up to 8, zeros in the gaps and behind them
-// up to Kd - and as columns [2 S, Mp], zeros behind row M; colsum: the tile's column sums [row tile][2 S] (or null).
-// Grid (ceil(S / 64), Mp / 64).  One read of dh, g, u; two writes of dg and du.
+// dg | du as rows [M, 2 Fp] in K tiles of 64 - `whole` tiles of dg, as many of du, then the last of dg and of du if there is one
+// more, zeros behind column F - and as columns [2 F, Mp], zeros behind row M; colsum: the tile's column sums [row tile][2 Fp]
+// (or null).  Grid (Fp / 64, Mp / 64).  One read of dh, g, u; two writes of dg and du.
 template <typename T>
 __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh, int64_t ldh, const T* __restrict__ gate, int64_t ldg,
                                                        const T* __restrict__ up, int64_t ldu, T* __restrict__ dgu, T* __restrict__ dgut,
-                                                       float* __restrict__ colsum, int M, int F, int S, int Kd, int Mp, int act) {
+                                                       float* __restrict__ colsum, int M, int F, int Fp, int Mp, int whole, int act) {
     typedef typename vec8<T>::type V;
     __shared__ __attribute__((aligned(16))) T tg[64 * 64], tu[64 * 64];
     __shared__ float cs[2][4][64];
     const int64_t m0 = (int64_t)blockIdx.y * 64;
     const int f0 = blockIdx.x * 64, ch = threadIdx.x & 7, c = f0 + ch * 8;
-    const bool last = blockIdx.x == gridDim.x - 1;
     float sg[8] = {}, su[8] = {};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -301,12 +271,10 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh,
                 og[j] = (T)vg;
                 ou[j] = (T)vu;
             }
-            T* row = dgu + m * Kd;
-            if (c < S) {
-                *reinterpret_cast<V*>(row + c) = og;
-                *reinterpret_cast<V*>(row + S + c) = ou;
-            }
-            if (last && 2 * S + ch * 8 < Kd) *reinterpret_cast<V*>(row + 2 * S + ch * 8) = V{};
+            T* row = dgu + m * (2 * (int64_t)Fp) + ch * 8;
+            const int tile = blockIdx.x;
+            *reinterpret_cast<V*>(row + (tile < whole ? tile : 2 * whole) * 64) = og;
+            *reinterpret_cast<V*>(row + (tile < whole ? whole + tile : 2 * whole + 1) * 64) = ou;
         }
         tile_put(tg, r, ch, og);
         tile_put(tu, r, ch, ou);
@@ -329,19 +297,19 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh,
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int f = (threadIdx.x >> 3) + 32 * i;
-        if (f0 + f >= S) break;
+        if (f0 + f >= F) break;
         *reinterpret_cast<V*>(dgut + (int64_t)(f0 + f) * Mp + m0 + ch * 8) = tile_get_t(tg, f, ch);
-        *reinterpret_cast<V*>(dgut + (int64_t)(S + f0 + f) * Mp + m0 + ch * 8) = tile_get_t(tu, f, ch);
+        *reinterpret_cast<V*>(dgut + (int64_t)(F + f0 + f) * Mp + m0 + ch * 8) = tile_get_t(tu, f, ch);
     }
     if (colsum && threadIdx.x < 128) {
         const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
-        if (f0 + l < S)
-            colsum[(int64_t)blockIdx.y * (2 * S) + w * S + f0 + l] = (cs[w][0][l] + cs[w][1][l]) + (cs[w][2][l] + cs[w][3][l]);
+        colsum[(int64_t)blockIdx.y * (2 * Fp) + w * Fp + f0 + l] = (cs[w][0][l] + cs[w][1][l]) + (cs[w][2][l] + cs[w][3][l]);
     }
 }
 // out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns
 template <typename T>
-__global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, int splits, T* __restrict__ out, int64_t M, int N, int Np) {
+__global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, int splits, T* __restrict__ out, int64_t M, int N,
+                                                        int Np) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int per = Np / 4;
     if (i >= M * per) return;
@@ -349,37 +317,60 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict_
     const int n = (int)(i - m * per) * 4;
     f32x4 s = *reinterpret_cast<const f32x4*>(part + m * Np + n);
     for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + ((int64_t)k * M + m) * Np + n);
+    T* to = out + m * N + n;
+    typedef T A4 __attribute__((ext_vector_type(4), aligned(2)));
+    if (n + 4 <= N) {
+        *reinterpret_cast<A4*>(to) = A4{(T)s[0], (T)s[1], (T)s[2], (T)s[3]};
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (n + j < N) out[m * N + n + j] = (T)s[j];
+        for (int j = 0; j < 3; ++j)
+            if (n + j < N) to[j] = (T)s[j];
+    }
 }
+
 
 // How a product [M, N] over K (a multiple of 64) is cut: whole (0 parts: straight to 16 bits) where its 256 x 256 tiles fill
 // half the chip, else 256 x 128 tiles in parts of K of at least 8 tiles, as many as there are CUs.  N % 8 != 0: always
 // through 32 bits (the 16-bit stores are 16 bytes wide).
 struct Cut {
     int splits, ks_per;
+    bool narrow;
 };
 Cut cut(int64_t M, int N, int K) {
     const int64_t tm = (M + 255) / 256;
     const int nk = K / 64;
+    const bool narrow = tm * ((N + 255) / 256) < 128;
     int64_t s = 1;
-    if (tm * ((N + 255) / 256) < 128) {
+    if (narrow) {
         s = 256 / (tm * ((N + 127) / 128));
         if (s > nk / 8) s = nk / 8;
         if (s < 1) s = 1;
     }
     const int per = (int)((nk + s - 1) / s);
     const int splits = (nk + per - 1) / per;
-    return {splits == 1 && N % 8 == 0 ? 0 : splits, per};
+    return {splits == 1 && N % 8 == 0 ? 0 : splits, per, narrow};
 }
 int64_t cut_bytes(int64_t M, int N, int K) { return (int64_t)cut(M, N, K).splits * M * up8(N) * 4; }
 
+// Rows up to which the weights are streamed (glu_few_kernel).  [K, F] = [4096, 14336], streamed / matrix-core kernel, us:
+// bf16 45 / 70 at 1 row, 56 / 69 at 32, 64 / 71 at 48, 70 / 73 at 64; e4m3 21 / 30 at 1, 32 / 34 at 48, 37 / 35 at 64.
+constexpr int FEW = 48;
+constexpr int64_t FAR = int64_t(1) << 22;   // gemm_w4.h: 32-bit offsets within a tile
+constexpr int LIMIT = (1 << 20) - 64;      // M, F, K of the gradient: row strides of 2 F and 4 K stay below gemm_w4.h's limit of 2^22
+
+bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool wide_rows(const void* p, int64_t ld, int K) { return aligned16(p) && ld % 8 == 0 && ld < FAR && K % 64 == 0; }
+// rows that the gradient's products read as they lie (K is not contracted there); their last K tile's copy has their stride
+bool plain_rows(const void* p, int64_t ld, int K) { return aligned16(p) && ld % 8 == 0 && K % 8 == 0 && ld >= K && ld <= 4 * (int64_t)K; }
+
 struct GradSpace {                  // byte offsets in the workspace, each a multiple of 256
-    int64_t dgu, dgut, wt, xt, colsum, parts, end;
+    bool plain_x, plain_w;
+    int64_t ldx, ldw;               // row strides as the products see them
+    int64_t dgu, dgut, x, w, colsum, parts, end;         // x, w (gate, then up): the last K tile, or (not plain) all of it
 };
-GradSpace grad_space(int64_t M, int64_t F, int64_t K) {
-    const int64_t S = up8(F), Kd = up64(2 * S), Mp = up64(M), Kp = up8(K);
+GradSpace grad_space(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu, int64_t M, int64_t F, int K) {
+    const int64_t Fp = up64(F), Mp = up64(M), Kp = up8(K);
     GradSpace g;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -387,40 +378,50 @@ GradSpace grad_space(int64_t M, int64_t F, int64_t K) {
         at += (bytes + 255) & ~(int64_t)255;
         return o;
     };
-    g.dgu = take(M * Kd * 2);
-    g.dgut = take(2 * S * Mp * 2);
-    g.wt = take(Kp * Kd * 2);
-    g.xt = take(Kp * Mp * 2);
-    g.colsum = take(Mp / 64 * 2 * S * 4);
-    const int64_t a = cut_bytes(M, (int)K, (int)Kd), b = cut_bytes(F, (int)K, (int)Mp), c = cut_bytes(2 * F, (int)K, (int)Mp);
-    g.parts = take(a > b ? (a > c ? a : c) : (b > c ? b : c));
+    g.plain_x = plain_rows(x, ldx, K);
+    g.plain_w = plain_rows(wg, ldwg, K) && plain_rows(wu, ldwu, K) && ldwg == ldwu;
+    g.ldx = g.plain_x ? ldx : Kp;
+    g.ldw = g.plain_w ? ldwg : Kp;
+    g.dgu = take(M * 2 * Fp * 2);
+    g.dgut = take(2 * F * Mp * 2);
+    g.x = take((g.plain_x ? (M % 64 ? 64 : 0) : Mp) * g.ldx * 2);
+    g.w = take(2 * (g.plain_w ? (F % 64 ? 64 : 0) : Fp) * g.ldw * 2);
+    g.colsum = take(Mp / 64 * 2 * Fp * 4);
+    const int64_t a = cut_bytes(M, K, (int)(2 * Fp)), b = cut_bytes(2 * F, K, (int)Mp);
+    g.parts = take(a > b ? a : b);
     g.end = at;
     return g;
 }
 
-// out [M, N] = a [M, K] . w [up8(N), K]^T, K a multiple of 64 and everything in the workspace's layout
+// out [M, N] = the product, through fp32 parts where it is cut
 template <typename T>
-int product(const T* a, int64_t lda, const T* w, int64_t ldw, T* out, int M, int N, int K, float* parts, hipStream_t st) {
-    constexpr int type = sizeof(T) == 2 && __is_same(T, bf16) ? FF_BF16 : FF_F16;
-    const Cut c = cut(M, N, K);         // (splits > 1 means few tiles: the narrow tile)
-    if (c.splits == 0)
-        return (type == FF_BF16 ? fp_gemm_bf16 : fp_gemm_f16)(a, lda, nullptr, 0, w, ldw, nullptr, out, N, M, N, K, 0, 0, nullptr, 0, nullptr, st);
-    const int Np = (int)up8(N);
-    if (int rc = fpi_gemm_parts(type, c.splits > 1, a, lda, w, ldw, parts, M, Np, K, c.splits, c.ks_per, st)) return rc;
-    add_parts_kernel<T><<<dim3((unsigned)(((int64_t)M * (Np / 4) + 255) / 256)), dim3(256), 0, st>>>(parts, c.splits, out, M, N, Np);
+int product(GradProduct p, T* out, int N, float* parts, hipStream_t st) {
+    const Cut c = cut(p.M, N, p.K);
+    p.narrow = c.narrow;
+    p.splits = c.splits;
+    p.ks_per = c.ks_per;
+    p.N = (int)up8(N);
+    p.out = c.splits ? (void*)parts : (void*)out;
+    if (int rc = fpi_grad_product(__is_same(T, bf16) ? FF_BF16 : FF_F16, p, st)) return rc;
+    if (c.splits == 0) return 0;
+    const int64_t lanes = (int64_t)p.M * (p.N / 4);
+    add_parts_kernel<T><<<dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st>>>(parts, c.splits, out, p.M, N, p.N);
     FP_CHECK_LAUNCH();
     return 0;
 }
 
-// Rows up to which the weights are streamed (glu_few_kernel).  [K, F] = [4096, 14336], streamed / matrix-core kernel, us:
-// bf16 45 / 70 at 1 row, 56 / 69 at 32, 64 / 71 at 48, 70 / 73 at 64; e4m3 21 / 30 at 1, 32 / 34 at 48, 37 / 35 at 64.
-constexpr int FEW = 48;
-constexpr int64_t FAR = int64_t(1) << 22;   // gemm_w4.h: 32-bit offsets within a tile
-constexpr int LIMIT = (1 << 21) - 64;      // M, F, K of the gradient: Kd and Mp stay below gemm_w4.h's limit of 2^22 for a row stride
-
-bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-bool wide_rows(const void* p, int64_t ld, int K) { return aligned16(p) && ld % 8 == 0 && ld < FAR && K % 64 == 0; }
+template <typename T>
+int copy_rows(Copies c, int cols, int cols_p, hipStream_t st) {
+    c.cols = cols;
+    c.cols_p = cols_p;
+    c.chunks = ((int64_t)c.rows_p[0] + c.rows_p[1] + c.rows_p[2]) * (cols_p / 8);
+    c.blocks = (unsigned)(c.chunks < 2048 * 256 ? (c.chunks + 255) / 256 : 2048);
+    const unsigned sums = c.sums ? 2 * (unsigned)((c.F + 63) / 64) : 0;
+    if (c.blocks + sums == 0) return 0;
+    copy_rows_kernel<T><<<dim3(c.blocks + sums), dim3(256), 0, st>>>(c);
+    FP_CHECK_LAUNCH();
+    return 0;
+}
 
 template <typename TI, typename TO>
 int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64_t ldwg, const float* gs, const void* wu, int64_t ldwu,
@@ -462,10 +463,11 @@ int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64
             FP_REQUIRE(K <= LIMIT && F <= LIMIT && ws && aligned16(ws) &&
                        ws_bytes >= fp_gated_ff_workspace_bytes(x, ldx, wg, ldwg, wu, ldwu, M, F, K));
             TI *xp = (TI*)ws, *gp = xp + (x_fits ? 0 : M * Kp), *upk = gp + (g_fits ? 0 : F * Kp);
-            const Copies c{{x, wg, wu}, {xp, gp, upk}, {ldx, ldwg, ldwu}, {x_fits ? 0 : M, g_fits ? 0 : F, u_fits ? 0 : F}};
-            const int64_t chunks = ((int64_t)c.rows[0] + c.rows[1] + c.rows[2]) * (Kp / 8);
-            copy_rows_kernel<TI><<<dim3((unsigned)(chunks < 2048 * 256 ? (chunks + 255) / 256 : 2048)), dim3(256), 0, st>>>(c, K, (int)Kp);
-            FP_CHECK_LAUNCH();
+            Copies c{{x, wg, wu}, {xp, gp, upk}, {ldx, ldwg, ldwu}, {Kp, Kp, Kp}};
+            c.rows[0] = c.rows_p[0] = x_fits ? 0 : M;
+            c.rows[1] = c.rows_p[1] = g_fits ? 0 : F;
+            c.rows[2] = c.rows_p[2] = u_fits ? 0 : F;
+            if (int rc = copy_rows<TI>(c, K, (int)Kp, st)) return rc;
             return fpi_glu(type, x_fits ? x : xp, x_fits ? ldx : Kp, xs, g_fits ? wg : gp, g_fits ? ldwg : Kp, gs, u_fits ? wu : upk,
                            u_fits ? ldwu : Kp, us, bg, bu, h, ldh, gate, up, ldp, M, F, (int)Kp, act, st);
         }
@@ -475,34 +477,49 @@ int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64
 
 template <typename T>
 int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
-                   const void* gate, int64_t ldg, const void* up, int64_t ldu, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
-                   int M, int F, int K, int act, void* ws, int64_t ws_bytes, void* stream) {
-    FP_REQUIRE(dh && x && wg && wu && gate && up && dx && dwg && dwu && !dbg == !dbu && (act == 0 || act == 1));
-    FP_REQUIRE(aligned2(dh) && aligned2(x) && aligned2(wg) && aligned2(wu) && aligned2(gate) && aligned2(up) && aligned2(dbg) && aligned2(dbu));
-    FP_REQUIRE(aligned16(dx) && aligned16(dwg) && (K % 8 != 0 ? aligned2(dwu) : aligned16(dwu)));
+                   const void* gate, int64_t ldg, const void* up, int64_t ldu, void* dx, void* dw, void* db, int M, int F, int K, int act, void* ws, int64_t ws_bytes, void* stream) {
+    FP_REQUIRE(dh && x && wg && wu && gate && up && dx && dw && (act == 0 || act == 1));
+    FP_REQUIRE(aligned2(dh) && aligned2(x) && aligned2(wg) && aligned2(wu) && aligned2(gate) && aligned2(up) && aligned2(db));
+    FP_REQUIRE(aligned16(dx) && aligned16(dw));
     FP_REQUIRE(M > 0 && F > 0 && K > 0 && ldh >= 0 && ldx >= 0 && ldg >= 0 && ldu >= 0 && ldwg >= K && ldwu >= K);
     FP_REQUIRE(M <= LIMIT && F <= LIMIT && K <= LIMIT);
-    FP_REQUIRE(ws && aligned16(ws) && ws_bytes >= fp_gated_ff_backward_workspace_bytes(M, F, K));
+    const GradSpace g = grad_space(x, ldx, wg, ldwg, wu, ldwu, M, F, K);
+    FP_REQUIRE(ws && aligned16(ws) && ws_bytes >= g.end);
     hipStream_t st = (hipStream_t)stream;
-    const GradSpace g = grad_space(M, F, K);
-    const int S = (int)up8(F), Kd = (int)up64(2 * S), Mp = (int)up64(M), Kp = (int)up8(K), ktiles = (Kp + 63) / 64;
+    const int Fp = (int)up64(F), Mp = (int)up64(M), Kp = (int)up8(K);
     char* base = (char*)ws;
-    T *dgu = (T*)(base + g.dgu), *dgut = (T*)(base + g.dgut), *wt = (T*)(base + g.wt), *xt = (T*)(base + g.xt);
-    float *colsum = dbg ? (float*)(base + g.colsum) : nullptr, *parts = (float*)(base + g.parts);
-    glu_grad_kernel<T><<<dim3((unsigned)((S + 63) / 64), (unsigned)(Mp / 64)), dim3(256), 0, st>>>(
-        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, S, Kd, Mp, act);
+    T *dgu = (T*)(base + g.dgu), *dgut = (T*)(base + g.dgut), *xc = (T*)(base + g.x), *wc = (T*)(base + g.w);
+    float *colsum = db ? (float*)(base + g.colsum) : nullptr, *parts = (float*)(base + g.parts);
+    const int whole = g.plain_w ? F / 64 : Fp / 64, x_whole = g.plain_x ? M / 64 : Mp / 64, wc_rows = g.plain_w ? 64 : Fp;
+    glu_grad_kernel<T><<<dim3((unsigned)(Fp / 64), (unsigned)(Mp / 64)), dim3(256), 0, st>>>(
+        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, Fp, Mp, whole, act);
     FP_CHECK_LAUNCH();
-    const int up_rows = Kd - S;
-    const Transposes t{{wg, wu, x}, {wt, wt + S, xt}, {ldwg, ldwu, ldx}, {Kd, Kd, Mp}, {F, F, M}, {S, up_rows, Mp},
-                       {(S + 63) / 64 * ktiles, (up_rows + 63) / 64 * ktiles, Mp / 64 * ktiles}, K, Kp, ktiles};
-    const ColumnSums cs{colsum, Mp / 64, F, S, dbg, dbu};
-    transpose_kernel<T><<<dim3((unsigned)(t.tiles[0] + t.tiles[1] + t.tiles[2] + (dbg ? 2 * ((F + 63) / 64) : 0))), dim3(256), 0, st>>>(t, cs);
-    FP_CHECK_LAUNCH();
-    if (int rc = product<T>(dgu, Kd, wt, Kd, (T*)dx, M, K, Kd, parts, st)) return rc;
-    // (dWg over dWu in one product where they are the halves of one matrix)
-    if (S == F && (T*)dwu == (T*)dwg + (int64_t)F * K) return product<T>(dgut, Mp, xt, Mp, (T*)dwg, 2 * F, K, Mp, parts, st);
-    if (int rc = product<T>(dgut, Mp, xt, Mp, (T*)dwg, F, K, Mp, parts, st)) return rc;
-    return product<T>(dgut + (int64_t)S * Mp, Mp, xt, Mp, (T*)dwu, F, K, Mp, parts, st);
+    // what the products cannot read as it lies: all of it, or the rows of a partial last K tile
+    const int xr = M % 64, wr = F % 64;
+    Copies c{{x, wg, wu}, {xc, wc, wc + wc_rows * g.ldw}, {ldx, ldwg, ldwu}, {g.ldx, g.ldw, g.ldw}};
+    if (g.plain_x) c.src[0] = (const T*)x + (int64_t)(M - xr) * ldx;
+    if (g.plain_w) c.src[1] = (const T*)wg + (int64_t)(F - wr) * ldwg, c.src[2] = (const T*)wu + (int64_t)(F - wr) * ldwu;
+    c.rows[0] = g.plain_x ? xr : M;
+    c.rows_p[0] = g.plain_x ? (xr ? 64 : 0) : Mp;
+    c.rows[1] = c.rows[2] = g.plain_w ? wr : F;
+    c.rows_p[1] = c.rows_p[2] = g.plain_w ? (wr ? 64 : 0) : Fp;
+    c.sums = colsum;
+    c.tiles = Mp / 64, c.F = F, c.Fp = Fp, c.db = db;
+    if (int rc = copy_rows<T>(c, K, Kp, st)) return rc;
+    const T *w0 = g.plain_w ? (const T*)wg : wc, *w1 = g.plain_w ? (const T*)wu : wc + wc_rows * g.ldw, *x0 = g.plain_x ? (const T*)x : xc;
+    // where K tile t lies if one matrix went on: w0's tiles, w1's from tile `whole` on, the copies' from tile 2 whole on
+    auto jump = [](const T* to, const T* from, int64_t tiles, int64_t ld) { return ((intptr_t)to - (intptr_t)from) - tiles * 64 * ld * 2; };
+    GradProduct p{};
+    p.a = dgu, p.lda = 2 * Fp, p.w = w0, p.ldw = g.ldw;
+    p.s1 = whole, p.d1 = jump(w1, w0, whole, g.ldw);
+    p.s2 = 2 * whole, p.d2 = jump(wc, w0, 2 * whole, g.ldw) - p.d1;
+    p.M = M, p.K = 2 * Fp;
+    if (int rc = product<T>(p, (T*)dx, K, parts, st)) return rc;
+    p.a = dgut, p.lda = Mp, p.w = x0, p.ldw = g.ldx;
+    p.s1 = x_whole, p.d1 = jump(xc, x0, x_whole, g.ldx);
+    p.s2 = 1 << 30, p.d2 = 0;
+    p.M = 2 * F, p.K = Mp;
+    return product<T>(p, (T*)dw, K, parts, st);
 }
 
 }  // namespace
@@ -542,23 +559,24 @@ extern "C" int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, 
                                   (const float*)wu_scale, b_gate, b_up, h, ldh, nullptr, nullptr, 0, M, F, K, act, nullptr, 0, stream);
 }
 
-extern "C" int64_t fp_gated_ff_backward_workspace_bytes(int M, int F, int K) {
+extern "C" int64_t fp_gated_ff_backward_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up,
+                                                        int64_t ldwu, int M, int F, int K) {
     if (M <= 0 || F <= 0 || K <= 0 || M > LIMIT || F > LIMIT || K > LIMIT) return 0;
-    return grad_space(M, F, K).end;
+    return grad_space(x, ldx, w_gate, ldwg, w_up, ldwu, M, F, K).end;
 }
 
 extern "C" int fp_gated_ff_backward_bf16(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
                                          const void* w_up, int64_t ldwu, const void* gate, int64_t ldg, const void* up, int64_t ldu,
-                                         void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int F, int K, int act,
+                                         void* dx, void* dw, void* db, int M, int F, int K, int act,
                                          void* workspace, int64_t workspace_bytes, void* stream) {
-    return ff_grad_launch<bf16>(dh, ldh, x, ldx, w_gate, ldwg, w_up, ldwu, gate, ldg, up, ldu, dx, dw_gate, dw_up, db_gate, db_up, M, F, K,
+    return ff_grad_launch<bf16>(dh, ldh, x, ldx, w_gate, ldwg, w_up, ldwu, gate, ldg, up, ldu, dx, dw, db, M, F, K,
                                 act, workspace, workspace_bytes, stream);
 }
 
 extern "C" int fp_gated_ff_backward_f16(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
                                         const void* w_up, int64_t ldwu, const void* gate, int64_t ldg, const void* up, int64_t ldu,
-                                        void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int F, int K, int act,
+                                        void* dx, void* dw, void* db, int M, int F, int K, int act,
                                         void* workspace, int64_t workspace_bytes, void* stream) {
-    return ff_grad_launch<_Float16>(dh, ldh, x, ldx, w_gate, ldwg, w_up, ldwu, gate, ldg, up, ldu, dx, dw_gate, dw_up, db_gate, db_up, M,
+    return ff_grad_launch<_Float16>(dh, ldh, x, ldx, w_gate, ldwg, w_up, ldwu, gate, ldg, up, ldu, dx, dw, db, M,
                                     F, K, act, workspace, workspace_bytes, stream);
 }

@@ -1,0 +1,27 @@
+// K13's gradient products on the matrix cores: instances of gemm_w4.h (see TrArgs and SplitArgs there).
+#include "gated_ff.h"
+#include "gemm_w4.h"
+
+using namespace fp_gemm;
+
+template <typename T>
+static int run(const GradProduct& p, hipStream_t st) {
+    const TrArgs tr{p.s1, p.s2, p.d1, p.d2};
+    const SplitArgs sp{p.splits, p.ks_per};
+    ConvGeom cg{};
+    cg.gm = p.K >= 8192 ? -3 : 8;                       // tile walk (ConvGeom::gm)
+    FP_REQUIRE(p.K % BK == 0 && p.N % 8 == 0 && (int64_t)(p.M / 256 + 1) * (p.N / 128 + 1) * (p.splits > 0 ? p.splits : 1) < (1ll << 31));
+    FP_REQUIRE(p.splits == 0 || ((int64_t)(p.splits - 1) * p.ks_per < p.K / BK && (int64_t)p.splits * p.ks_per >= p.K / BK));
+#define FP_TR(TO, NT, SPLIT)                                                                                                         \
+    return launch_w4<T, 0, 0, TO, NT, 0, 0, 0, 0, 0, SPLIT, 1>(p.a, p.lda, 0, p.K, p.w, p.ldw, nullptr, p.out, p.N, p.M, p.N, p.K, 0, \
+                                                               nullptr, 0, nullptr, cg, st, nullptr, nullptr, QkNormArgs{}, Rows2{},  \
+                                                               GluArgs{}, sp, tr)
+    if (p.splits > 0) FP_TR(float, 4, 1);
+    if (p.narrow) FP_TR(T, 4, 0);
+    FP_TR(T, 8, 0);
+#undef FP_TR
+}
+
+int fpi_grad_product(int type, const GradProduct& p, hipStream_t st) {
+    return type == FF_BF16 ? run<bf16>(p, st) : run<_Float16>(p, st);
+}

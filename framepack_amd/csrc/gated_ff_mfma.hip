@@ -1,4 +1,4 @@
-// K13's products on the matrix cores: instances of gemm_w4.h (see GluArgs and SplitArgs there).
+// K13's forward product on the matrix cores: instances of gemm_w4.h (see GluArgs there).
 #include "gated_ff.h"
 #include "gemm_w4.h"
 
@@ -35,22 +35,4 @@ int fpi_glu(int type, const void* x, int64_t ldx, const float* xs, const void* w
     if (narrow) FP_GLU(_Float16, _Float16, 4, 0);
     FP_GLU(_Float16, _Float16, 8, 0);
 #undef FP_GLU
-}
-
-int fpi_gemm_parts(int type, bool narrow, const void* a, int64_t lda, const void* w, int64_t ldw, float* part, int M, int N, int K,
-                   int splits, int ks_per, hipStream_t st) {
-    const SplitArgs sp{splits, ks_per};
-    const ConvGeom cg{};
-    FP_REQUIRE(splits > 0 && ks_per > 0 && (int64_t)(splits - 1) * ks_per < K / BK && (int64_t)splits * ks_per >= K / BK);
-    FP_REQUIRE((int64_t)((M + BM - 1) / BM) * ((N + 127) / 128) * splits < (1ll << 31));
-#define FP_PARTS(T, NT)                                                                                                              \
-    return launch_w4<T, 0, 0, float, NT, 0, 0, 0, 0, 0, 1>(a, lda, 0, K, w, ldw, nullptr, part, N, M, N, K, 0, nullptr, 0, nullptr, cg, \
-                                                           st, nullptr, nullptr, QkNormArgs{}, Rows2{}, GluArgs{}, sp)
-    if (type == FF_BF16) {
-        if (narrow) FP_PARTS(bf16, 4);
-        FP_PARTS(bf16, 8);
-    }
-    if (narrow) FP_PARTS(_Float16, 4);
-    FP_PARTS(_Float16, 8);
-#undef FP_PARTS
 }

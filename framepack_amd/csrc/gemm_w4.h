@@ -74,6 +74,14 @@ template <int IDX> __device__ __forceinline__ f32x4 acc_read() {
     return f32x4{r0, r1, r2, r3};
 }
 
+// A fragment from an image whose rows are K: two transposing reads of 4 rows x 16 columns per 16 lanes (K = 8 g .. 8 g + 3
+// and 8 g + 4 .. + 7 for lane group g: the order of a row read from the ordinary image)
+template <int OFF> __device__ __forceinline__ void lds_read_tr(i32x4& dst, unsigned addr) {
+    u32x2 lo, hi;
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(lo) : "v"(addr), "n"(OFF));
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi) : "v"(addr), "n"(OFF + 1024));
+    dst = __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3));
+}
 template <int OFF> __device__ __forceinline__ void lds_read_b128(i32x4& dst, unsigned addr) {
     asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(dst) : "v"(addr), "n"(OFF));
 }
@@ -88,20 +96,21 @@ template <int OFF> __device__ __forceinline__ void lds_read_b128(i32x4& dst, uns
 #endif
 constexpr int A_AHEAD = FP_A_AHEAD;             // an A fragment is read this many groups (of 8 MFMAs) before its own
 constexpr int A_RING = A_AHEAD <= 2 ? 4 : 8;
-constexpr int lgkm_before(int P, int g, int NT) {
-    int issued = 0, idx_a[16] = {}, last_w1 = -1;
-    if (P == 0) issued += NT < 8 ? NT : 8;      // W(ks 0)
-    for (int i = 0; i < A_AHEAD; ++i) idx_a[i] = issued++;
+// RW: LDS reads per W fragment (2 where it is read transposed); the counter holds 15 at most.
+constexpr int lgkm_before(int P, int g, int NT, int RW = 1) {
+    int issued = 0, end_a[16] = {}, end_w1 = 0;  // reads issued up to and with the fragment's last
+    if (P == 0) issued += RW * (NT < 8 ? NT : 8);      // W(ks 0)
+    for (int i = 0; i < A_AHEAD; ++i) end_a[i] = ++issued;
     for (int j = 0; j < g; ++j) {               // what groups 0 .. g-1 issue
-        if (j + A_AHEAD < 8) idx_a[j + A_AHEAD] = issued++;
+        if (j + A_AHEAD < 8) end_a[j + A_AHEAD] = ++issued;
         if (P == 0 && j < 4) {
-            if (2 * j < NT) last_w1 = issued++;
-            if (2 * j + 1 < NT) last_w1 = issued++;
+            if (2 * j < NT) end_w1 = issued += RW;
+            if (2 * j + 1 < NT) end_w1 = issued += RW;
         }
     }
-    int need = idx_a[g];
-    if (P == 0 && g >= 4 && last_w1 > need) need = last_w1;
-    return issued - (need + 1);
+    int need = end_a[g];
+    if (P == 0 && g >= 4 && end_w1 > need) need = end_w1;
+    return issued - need < 15 ? issued - need : 15;
 }
 #if FP_A_AHEAD == 2
 static_assert(lgkm_before(0, 0, 8) == 1 && lgkm_before(0, 1, 8) == 3 && lgkm_before(0, 2, 8) == 5 &&
@@ -169,8 +178,19 @@ __device__ __forceinline__ float glu_c1(int act) { return act ? 1.44269504088896
 struct SplitArgs {
     int splits, ks_per;
 };
+// TRW (gated_ff.hip's gradient): W is given with K along its ROWS, [K, N] with unit stride in N, and read as it is: a K tile
+// is staged as rows of K and transposed on the way into registers (lds_read_tr).  LDS image of a wave column's half of W (all
+// of W at NT = 4): [64 K rows][256 B = 8 granules of 16 columns], the granule index XORed with (K & 3) | ((K >> 3) & 1) << 2,
+// so that the 16 rows a transposing read touches lie in all 8 bank groups; the XOR is applied to the DMA's source address, as
+// in the ordinary image.  K tile t lies t tiles behind W's first, plus d1 from tile s1 on, plus d2 from tile s2 on (bytes):
+// two matrices and the zero-padded last tiles of both are one operand without a branch in the loop (a choice between
+// pointers became one: 8 % of the kernel's time).  N % 8 == 0.
+struct TrArgs {
+    int s1, s2;
+    int64_t d1, d2;
+};
 template <typename T, typename TO, int EPI, int AMODE, int NT = 8, int QKN = 0, int TALL = 0, int GRP = 0, int GLU = 0,
-          int KEEP = 0, int SPLIT = 0>
+          int KEEP = 0, int SPLIT = 0, int TRW = 0>
 __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A, int64_t lda, int64_t a2_delta,
                                                          int k1, const T* __restrict__ W, int64_t ldw,
                                                          const TO* __restrict__ bias_, TO* __restrict__ C,
@@ -179,7 +199,9 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                                                          const TO* __restrict__ gate_, int ntm, int ntn, ConvGeom cg,
                                                          const float* __restrict__ a_scale,
                                                          const float* __restrict__ w_scale, QkNormArgs qk, Rows2 r2,
-                                                         GluArgs glu, SplitArgs sp) {
+                                                         GluArgs glu, SplitArgs sp, TrArgs tr) {
+    static_assert(!TRW || (AMODE == 0 && !TALL && !QKN && !GRP && !GLU && EPI == 0 && sizeof(T) == 2 && (NT == 8 || NT == 4)),
+                  "W by rows of K: the dense 16-bit tile");
     static_assert(!GLU || (AMODE == 0 && !TALL && !QKN && !GRP && EPI == 0 && sizeof(TO) == 2 && NT >= 4), "gated block: the dense tile");
     static_assert(!SPLIT || (AMODE == 0 && !TALL && !QKN && !GRP && !GLU && EPI == 0 && sizeof(TO) == 4), "parts of K: fp32 out");
     static_assert(!GRP || (AMODE == 0 && !TALL && !QKN && NT == 8 && sizeof(T) == 2), "row segments: the dense 16-bit 256 x 256 tile");
@@ -250,6 +272,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     constexpr int N_STORES = GLU ? 16 / RPI * 8 * (KEEP ? 3 : 1) : 32;
     int part = 0;                   // SPLIT: which run of K tiles
     int nk = K / BKE;
+    const int64_t w_tile = TRW ? (int64_t)BKE * (int)sizeof(T) * ldw : 0;      // bytes from a K tile of W to the next
     unsigned a_rd[2], w_rd[2];  // fragment read addresses (below)
     const int fr = lane & 15, fq = lane >> 4;
     constexpr unsigned SECOND = SCALED ? 16u : 64u;
@@ -321,6 +344,12 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int wrw = wrow0[j] + prow;
+            if constexpr (TRW) {
+                const int row = lane >> 4, c = lane & 15, i = wave * WPW + j, q = (c >> 1) ^ (row | ((j & 2) << 1));
+                const int col = (NT == 8 ? (i >> 4) * 128 : 0) + q * 16 + (c & 1) * 8;
+                pw[j] = (unsigned)((i & 15) * 4 + row) * (unsigned)(ldw * sizeof(T)) + (unsigned)min(col, N - 8 - n0) * (unsigned)sizeof(T);
+                continue;
+            }
             // GLU: the wave's WPW pieces are the rows of wave column wave >> 1 of one of the two matrices
             const int col = GLU ? (wave >> 1) * (CW / 2) + j * 8 + prow : wrw;
             pw[j] = (unsigned)(min(n0 + col, N - 1) - n0) * (unsigned)((GLU && (wave & 1) ? glu.ldw2 : ldw) * sizeof(T)) +
@@ -328,13 +357,13 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         }
         abase = AMODE == 1 ? reinterpret_cast<const char*>(A) + ((int64_t)lo_vox << (cg.lcin + LOG2_TB))
                            : reinterpret_cast<const char*>(A + (int64_t)m0 * lda);
-        wbase = reinterpret_cast<const char*>(w_seg + (int64_t)n0 * ldw);
+        wbase = reinterpret_cast<const char*>(w_seg + (TRW ? (int64_t)n0 : (int64_t)n0 * ldw));
         if constexpr (GLU) {
             if (wave & 1) wbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(glu.w2) + (int64_t)n0 * glu.ldw2);
         }
         if constexpr (SPLIT) {
             abase += (int64_t)part * sp.ks_per * 128;
-            wbase += (int64_t)part * sp.ks_per * 128;
+            if (!TRW) wbase += (int64_t)part * sp.ks_per * 128;
         }
     };
     // AMODE 1: a K tile is one tap x 64 or 128 channels, and with Cin >= 2 K tiles per tap (the launcher sends narrower
@@ -391,6 +420,10 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     };
     auto src_w = [&](int j, int t) __attribute__((always_inline)) -> const T* {
         asm volatile("" : "+v"(pw[j]));
+        if constexpr (TRW) {
+            const int tg = t + (SPLIT ? part * sp.ks_per : 0);
+            return reinterpret_cast<const T*>(wbase + (int64_t)tg * w_tile + (tg >= tr.s1 ? tr.d1 : 0) + (tg >= tr.s2 ? tr.d2 : 0) + pw[j]);
+        }
         return reinterpret_cast<const T*>(wbase + (int64_t)t * (BKE * (int)sizeof(T)) + pw[j]);
     };
     // EVEN: t is even before the clamp (clamped, an even and the odd call behind it both name tile nk - 1)
@@ -461,6 +494,17 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         w_rd[ks] = W_BASE + (unsigned)(wc * CW) * 128 + (ks ? (off_k0 ^ SECOND) : off_k0);
         asm volatile("" : "+v"(a_rd[ks]), "+v"(w_rd[ks]));
     }
+    // TRW: lane (g, r, c4) reads 8 bytes of K row 8 g + r at granule (index) ^ (r | (g & 1) << 2): one address per granule
+    unsigned w_tr[TRW ? 8 : 1];
+    {
+        const unsigned r = (unsigned)(lane & 15) >> 2, g = (unsigned)lane >> 4, sx = r | ((g & 1) << 2);
+        const unsigned in = (8 * g + r) * 256 + (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < (TRW ? NT : 0); ++i) {
+            w_tr[i] = W_BASE + in + (NT == 8 ? (unsigned)wc * (OP_BYTES / 2) + (((unsigned)i ^ sx) << 5) : (((unsigned)(wc * 4 + i) ^ sx) << 5));
+            asm volatile("" : "+v"(w_tr[i]));
+        }
+    }
 
     // The 64 accumulator tiles live in AGPRs a[0:255] that the compiler never sees: tile (mi, ni) = a[(mi*8+ni)*4 .. +3].
     // hipcc cannot keep 256 loop-carried accumulator registers in place once the MFMAs are interleaved with loads:
@@ -504,7 +548,11 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     };
     auto rd_w = [&](auto BUF, auto KS_, auto NI) __attribute__((always_inline)) {
         constexpr int off = BUF * (int)W_STEP + (NI * 16) * 128;
-        if constexpr (NI < NT) lds_read_b128<off>(wf[KS_][NI], w_rd[KS_]);
+        if constexpr (TRW) {
+            if constexpr (NI < NT) lds_read_tr<BUF * (int)W_STEP + KS_ * 8192>(wf[KS_][NI], w_tr[TRW ? (int)NI : 0]);
+        } else if constexpr (NI < NT) {
+            lds_read_b128<off>(wf[KS_][NI], w_rd[KS_]);
+        }
     };
     // MFMA ni of group G of phase P; ZC: first K step of the tile (C operand = 0); LGKM: wait in front (-1: none)
     auto mfma1 = [&](auto P, auto G, auto NI, auto ZC, auto LGKM) __attribute__((always_inline)) {
@@ -612,7 +660,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             fence();
             static_for<6>([&](auto g) __attribute__((always_inline)) {
                 static_for<8>([&](auto k) __attribute__((always_inline)) {
-                    mfma1(P, g, k, ZC, ic<(k == 0 ? lgkm_before(P, g, NT) : -1)>{});
+                    mfma1(P, g, k, ZC, ic<(k == 0 ? lgkm_before(P, g, NT, 1 + TRW) : -1)>{});
                     fence();
                     slot(BUF, P, t, g, k);
                     fence();
@@ -638,7 +686,9 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         return l;
     };
     // (GRP: the epilogue runs after the NEXT tile's setup, so the segment's terms are derived again from the tile's row)
-    auto seg_rows = [&](int em0) __attribute__((always_inline)) { return GRP ? (em0 >= r2.m_split ? M : r2.m_split) : M; };
+    auto seg_rows = [&](int em0) __attribute__((always_inline)) {
+        return GRP ? (em0 >= r2.m_split ? M : r2.m_split) : M;
+    };
     auto load_resid = [&](int em0, int en0, int ecw, int mi) __attribute__((always_inline)) {
         const int M = seg_rows(em0);            // shadows the kernel's
         const int el = opaque_lane();
@@ -731,6 +781,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         });
     };
     auto epilogue = [&](int em0, int en0, int ecw, int epart) __attribute__((always_inline)) {
+      const int64_t part0 = SPLIT ? (int64_t)epart * M : 0;      // (the whole M)
       const int M = seg_rows(em0);              // shadows the kernel's
       const bool second = GRP && em0 >= r2.m_split;
       const TO* const bias = second ? reinterpret_cast<const TO*>(r2.bias2) : bias_;
@@ -757,7 +808,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                 const int n = nb + ni * 16;
                 const f32x4 av = acc_read<(mi * 8 + ni) * 4>() + bv[ni];
                 if (mrow0 + fr < M && n < N)
-                    *reinterpret_cast<f32x4*>(C + ((SPLIT ? (int64_t)epart * M : 0) + mrow0 + fr) * ldc + n) = av;
+                    *reinterpret_cast<f32x4*>(C + (part0 + mrow0 + fr) * ldc + n) = av;
             });
         });
       } else {
@@ -988,12 +1039,12 @@ inline int persistent_grid() {
 }
 
 template <typename T, int EPI, int AMODE, typename TO = T, int NT = 8, int QKN = 0, int TALL = 0, int GRP = 0, int GLU = 0,
-          int KEEP = 0, int SPLIT = 0>
+          int KEEP = 0, int SPLIT = 0, int TRW = 0>
 int launch_w4(const void* a, int64_t lda, int64_t a2_delta, int k1, const void* w, int64_t ldw, const void* bias,
               void* c, int64_t ldc, int M, int N, int K, int gelu_from, const void* resid, int64_t ldr,
               const void* gate, const ConvGeom& cg, hipStream_t st, const float* a_scale = nullptr,
               const float* w_scale = nullptr, const QkNormArgs& qk = QkNormArgs{}, const Rows2& r2 = Rows2{},
-              const GluArgs& glu = GluArgs{}, const SplitArgs& sp = SplitArgs{}) {
+              const GluArgs& glu = GluArgs{}, const SplitArgs& sp = SplitArgs{}, const TrArgs& tr = TrArgs{}) {
     // lane offsets inside a tile are 32-bit: 255 rows x the row stride in bytes has to fit
     if (lda >= (int64_t(1) << 22) || ldw >= (int64_t(1) << 22) || glu.ldw2 >= (int64_t(1) << 22)) return (int)hipErrorInvalidValue;
     constexpr int TBM = TALL ? 2 * BM : BM, TBN = TALL || GLU ? 16 * NT : 32 * NT;
@@ -1001,13 +1052,13 @@ int launch_w4(const void* a, int64_t lda, int64_t a2_delta, int k1, const void* 
     const int ntn = (N + TBN - 1) / TBN;
     // operand buffers + the epilogue's row stage (TALL: all 160 KiB are operand buffers, the stage lies inside them)
     constexpr int smem = TALL ? 5 * OP_BYTES : 2 * BUF_BYTES + 4 * 8192;
-    auto kern = gemm_w4_kernel<T, TO, EPI, AMODE, NT, QKN, TALL, GRP, GLU, KEEP, SPLIT>;
+    auto kern = gemm_w4_kernel<T, TO, EPI, AMODE, NT, QKN, TALL, GRP, GLU, KEEP, SPLIT, TRW>;
     hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != hipSuccess) return (int)e;
     kern<<<dim3((unsigned)min(ntm * ntn * (SPLIT ? sp.splits : 1), persistent_grid())), dim3(256), smem, st>>>((const T*)a, lda, a2_delta, k1, (const T*)w, ldw,
                                                               (const TO*)bias, (TO*)c, ldc, M, N, K, gelu_from,
                                                               (const TO*)resid, ldr, (const TO*)gate, ntm, ntn, cg,
-                                                              a_scale, w_scale, qk, r2, glu, sp);
+                                                              a_scale, w_scale, qk, r2, glu, sp, tr);
     FP_CHECK_LAUNCH();
     return 0;
 }

@@ -948,15 +948,14 @@ def gated_ff_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w
     q2, _, _, ldq = _mat(up, "up", dt, M, F)
     new = x.new_empty if M > 0 else x.new_zeros
     dx, dw = new((M, K)), new((2 * F, K))
-    dwg, dwu = dw[:F], dw[F:]
-    dbg, dbu = new((2, F)) if bias else (None, None)
+    db = new((2 * F,)) if bias else None
     if M > 0:
         lib = _lib.load()
-        n = lib.fp_gated_ff_backward_workspace_bytes(M, F, K)
+        n = lib.fp_gated_ff_backward_workspace_bytes(x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, M, F, K)
         ws = x.new_empty((n,), dtype=torch.uint8)
         fn, name = ((lib.fp_gated_ff_backward_bf16, "fp_gated_ff_backward_bf16") if x.dtype == BF16 else
                     (lib.fp_gated_ff_backward_f16, "fp_gated_ff_backward_f16"))
         _lib.check(fn(d2.data_ptr(), ldd, x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, p2.data_ptr(), ldp,
-                      q2.data_ptr(), ldq, dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), _ptr(dbg), _ptr(dbu), M, F, K, act,
+                      q2.data_ptr(), ldq, dx.data_ptr(), dw.data_ptr(), _ptr(db), M, F, K, act,
                       ws.data_ptr(), n, _stream(x)), name)
-    return dx, dwg, dwu, dbg, dbu
+    return dx, dw[:F], dw[F:], None if db is None else db[:F], None if db is None else db[F:]

@@ -243,7 +243,7 @@ int fp_rmsnorm_residual_backward_f16(const void* dy, int64_t dy_row_stride, cons
  * neither, row stride ldp): receive g and u for the gradient.  No output may overlap an input.  workspace:
  * fp_gated_ff_workspace_bytes(...) bytes for these operands, 16-byte aligned, or NULL where that is 0: it is unless M > 48
  * and K % 64 != 0 or one of x, w_gate, w_up is not 16-byte aligned with a row stride of a multiple of 8 below 2^22 (such
- * operands are copied into rows that are; F, K <= 2^21 - 64 then). */
+ * operands are copied into rows that are; F, K <= 2^20 - 64 then). */
 int64_t fp_gated_ff_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up,
                                     int64_t ldwu, int M, int F, int K);
 int fp_gated_ff_bf16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
@@ -261,17 +261,17 @@ int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, const void*
                     int64_t ldh, int M, int F, int K, int act, void* stream);
 
 /* Gradient of K13 from dh and the kept g and u:  dg = dh u act'(g), du = dh act(g) (rounded to the type), then
- *   dx = dg . w_gate + du . w_up [M, K];  dw_gate = dg^T . x, dw_up = du^T . x [F, K];
- *   db_gate, db_up [F] = column sums of dg, du (both or neither NULL).
- * The outputs are contiguous, dx and dw_* 16-byte aligned (dw_up: where K % 8 == 0); dw_up right behind dw_gate saves a
- * launch.  M > 0; M, F, K <= 2^21 - 64.  Sums in fp32 in a fixed order.  workspace: fp_gated_ff_backward_workspace_bytes(M, F, K), 16-byte aligned. */
-int64_t fp_gated_ff_backward_workspace_bytes(int M, int F, int K);
+ *   dx = dg . w_gate + du . w_up [M, K];  dw [2 F, K] = dg^T . x over du^T . x;  db [2 F] (or NULL) = column sums of dg, du.
+ * The outputs are contiguous, dx and dw 16-byte aligned.  M > 0; M, F, K <= 2^20 - 64.  Sums in fp32 in a fixed order.
+ * workspace: fp_gated_ff_backward_workspace_bytes(...) bytes for these operands, 16-byte aligned. */
+int64_t fp_gated_ff_backward_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up,
+                                             int64_t ldwu, int M, int F, int K);
 int fp_gated_ff_backward_bf16(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
                               const void* w_up, int64_t ldwu, const void* gate, int64_t ldg, const void* up, int64_t ldu,
-                              void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
+                              void* dx, void* dw, void* db, int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
 int fp_gated_ff_backward_f16(const void* dh, int64_t ldh, const void* x, int64_t ldx, const void* w_gate, int64_t ldwg,
                              const void* w_up, int64_t ldwu, const void* gate, int64_t ldg, const void* up, int64_t ldu,
-                             void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
+                             void* dx, void* dw, void* db, int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- K11: causal-3D VAE decode (fp16, channels-last [T, H, W, C] volumes) -------------------------------
  * The reference's code for this path is diffusers_helper/hunyuan.py:93-103 (vae_decode); everything under its

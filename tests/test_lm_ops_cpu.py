@@ -133,7 +133,7 @@ def test_the_library_refuses_without_launching():
     ok = [p, m, p, m, p, m, p, p, m, p, n, m, 1e-6, p, 1 << 30, None]
     for i, v in ((0, None), (2, None), (6, None), (7, None), (9, None), (8, m - 1), (10, 0), (11, 0), (13, None), (13, p + 4), (14, 16)):
         refused("fp_rmsnorm_residual_backward_bf16", *[v if j == i else t for j, t in enumerate(ok)])
-    assert L.fp_rmsnorm_residual_backward_workspace_bytes(0, 8) == 0 and L.fp_gated_ff_backward_workspace_bytes(4, 0, 8) == 0
+    assert L.fp_rmsnorm_residual_backward_workspace_bytes(0, 8) == 0 and L.fp_gated_ff_backward_workspace_bytes(p, 8, p, 8, p, 8, 4, 0, 8) == 0
     F, K = 16, 128
     ok = [p, K, p, K, p, K, p, p, p, F, p, p, F, n, F, K, 0, None, 0, None]
     for i, v in ((0, None), (2, None), (4, None), (8, None), (6, None), (7, None), (10, None), (9, F - 1), (12, F - 1), (3, K - 1),
@@ -151,7 +151,7 @@ def test_the_library_refuses_without_launching():
     for i, v in ((0, None), (2, None), (5, None), (8, None), (1, K + 8), (4, K + 8), (7, K + 8), (0, p + 8), (3, p + 8), (6, p + 8),
                  (11, p + 8), (12, F + 4), (14, 12), (15, 64), (5, p + 4), (9, p + 2), (9, None), (16, -1)):
         refused("fp_gated_ff_fp8", *[v if j == i else t for j, t in enumerate(ok)])
-    ok = [p, F, p, K, p, K, p, K, p, F, p, F, p, p, p, p, p, n, F, K, 0, p, 1 << 30, None]
-    for i, v in ((0, None), (2, None), (4, None), (8, None), (12, None), (13, None), (15, None), (5, K - 1), (7, K - 1), (12, p + 8),
-                 (13, p + 2), (14, p + 2), (17, 0), (18, 0), (19, 0), (17, 1 << 21), (20, 3), (21, None), (21, p + 8), (22, 16)):
+    ok = [p, F, p, K, p, K, p, K, p, F, p, F, p, p, p, n, F, K, 0, p, 1 << 30, None]
+    for i, v in ((0, None), (2, None), (4, None), (8, None), (12, None), (13, None), (5, K - 1), (7, K - 1), (12, p + 8), (13, p + 2),
+                 (14, p + 1), (15, 0), (16, 0), (17, 0), (15, 1 << 20), (18, 3), (19, None), (19, p + 8), (20, 16)):
         refused("fp_gated_ff_backward_f16", *[v if j == i else t for j, t in enumerate(ok)])
