@@ -41,6 +41,20 @@ __device__ __forceinline__ float group16_sum(float v) {
     return v;
 }
 
+// K2's arithmetic between its rounding points (norm_kernels.hip and the GEMM epilogue that replaces it, gemm_w4.h, have to give
+// the same bits): what is fused and what is not is written out, so that no compiler option decides it for one of them alone.
+__device__ __forceinline__ float k2_sum_of_squares(const float (&f)[8]) {
+#pragma clang fp contract(off)
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+    return ss;
+}
+__device__ __forceinline__ float k2_rstd(float row_ss, float eps) { return rsqrtf(__builtin_fmaf(row_ss, 1.f / 128.f, eps)); }
+// the rotary pair (re, im): (re c0 - im s0, im c1 + re s1)
+__device__ __forceinline__ float k2_rot_re(float re, float im, float c0, float s0) { return __builtin_fmaf(re, c0, -(im * s0)); }
+__device__ __forceinline__ float k2_rot_im(float re, float im, float c1, float s1) { return __builtin_fmaf(im, c1, re * s1); }
+
 // Bijective XCD-aware remap (blocks b and b+8 share an XCD's L2): gives each XCD a contiguous run of
 // work items so that neighbours in work order share operands through one L2.
 __device__ __forceinline__ int xcd_remap(int bid, int nwg) {

@@ -915,13 +915,10 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                     if (qk_which >= 0) {
                         const bool is_txt = mrow0 + row >= qk.rope_rows;
                         const bf16x8 wv = is_txt ? qk_w_txt : qk_w_img;
-                        float f[8], ss = 0.f;
+                        float f[8];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            f[j] = (float)ov[j];
-                            ss += f[j] * f[j];
-                        }
-                        const float r = rsqrtf(group16_sum(ss) * (1.f / 128.f) + qk.eps);
+                        for (int j = 0; j < 8; ++j) f[j] = (float)ov[j];
+                        const float r = k2_rstd(group16_sum(k2_sum_of_squares(f)), qk.eps);
                         float nn[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -934,8 +931,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                             const float sn[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
 #pragma unroll
                             for (int p2 = 0; p2 < 4; ++p2) {
-                                ov[2 * p2] = (TO)(nn[2 * p2] * c[2 * p2] + (-nn[2 * p2 + 1]) * sn[2 * p2]);
-                                ov[2 * p2 + 1] = (TO)(nn[2 * p2 + 1] * c[2 * p2 + 1] + nn[2 * p2] * sn[2 * p2 + 1]);
+                                ov[2 * p2] = (TO)k2_rot_re(nn[2 * p2], nn[2 * p2 + 1], c[2 * p2], sn[2 * p2]);
+                                ov[2 * p2 + 1] = (TO)k2_rot_im(nn[2 * p2], nn[2 * p2 + 1], c[2 * p2 + 1], sn[2 * p2 + 1]);
                             }
                         } else {
 #pragma unroll

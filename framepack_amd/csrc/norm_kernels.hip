@@ -137,13 +137,9 @@ __global__ __launch_bounds__(256) void qk_rmsnorm_rope_kernel(bf16* __restrict__
 
     const bf16x8 xv = *reinterpret_cast<const bf16x8*>(base);
     float f[8];
-    float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        f[j] = (float)xv[j];
-        ss += f[j] * f[j];
-    }
-    const float r = rsqrtf(group16_sum(ss) * (1.f / 128.f) + eps);
+    for (int j = 0; j < 8; ++j) f[j] = (float)xv[j];
+    const float r = k2_rstd(group16_sum(k2_sum_of_squares(f)), eps);
     const bf16x8 wv = *reinterpret_cast<const bf16x8*>(w + sub * 8);
     float n[8];
 #pragma unroll
@@ -160,8 +156,8 @@ __global__ __launch_bounds__(256) void qk_rmsnorm_rope_kernel(bf16* __restrict__
         const float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
 #pragma unroll
         for (int p = 0; p < 4; ++p) {                        // pair (2p, 2p+1): rot = (-imag, real)
-            o[2 * p] = (bf16)(n[2 * p] * c[2 * p] + (-n[2 * p + 1]) * s[2 * p]);
-            o[2 * p + 1] = (bf16)(n[2 * p + 1] * c[2 * p + 1] + n[2 * p] * s[2 * p + 1]);
+            o[2 * p] = (bf16)k2_rot_re(n[2 * p], n[2 * p + 1], c[2 * p], s[2 * p]);
+            o[2 * p + 1] = (bf16)k2_rot_im(n[2 * p], n[2 * p + 1], c[2 * p + 1], s[2 * p + 1]);
         }
     } else {
 #pragma unroll
