@@ -470,8 +470,9 @@ def test_a_block_of_norm_gated_ff_and_residual_linear(M):
         n_ = h_ / torch.sqrt((h_ * h_).mean(1, keepdim=True) + EPS) * w_
         return (dy.double() * (h_ + (act64(n_ @ wg.double().t(), 0)[0] * (n_ @ wu.double().t())) @ wd.double().t())).sum()
 
-    p = x.double().requires_grad_(), w.double().requires_grad_()
-    want = torch.autograd.grad(loss(*p), p)
+    with torch.enable_grad():                              # (other test modules switch it off for the process)
+        p = x.double().requires_grad_(), w.double().requires_grad_()
+        want = torch.autograd.grad(loss(*p), p)
     # seven roundings between the loss and dx (n, gate and up, da, dg and du, dn, h, dx), of relative rms at most u / sqrt(3)
     assert rel_l2(dx, want[0]) < math.sqrt(9 / 3) * 2 * u_of(BF)
     assert rel_l2(dw, want[1]) < math.sqrt(9 / 3) * 2 * u_of(BF)
