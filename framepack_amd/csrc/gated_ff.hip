@@ -428,6 +428,7 @@ int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64
               const float* us, const void* bg, const void* bu, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M, int F,
               int K, int act, void* ws, int64_t ws_bytes, void* stream) {
     FP_REQUIRE(x && wg && wu && h && M >= 0 && F > 0 && K > 0 && (act == 0 || act == 1) && !bg == !bu && !gate == !up);
+    FP_REQUIRE(M <= 1 << 30 && F <= 1 << 30 && K <= 1 << 30);
     FP_REQUIRE(ldx >= 0 && ldwg >= K && ldwu >= K && ldh >= F && (!gate || ldp >= F));
     FP_REQUIRE(sizeof(TI) == 1 || (aligned2(x) && aligned2(wg) && aligned2(wu) && aligned2(h) && aligned2(bg) && aligned2(bu) &&
                                    aligned2(gate) && aligned2(up)));

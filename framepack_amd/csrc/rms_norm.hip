@@ -399,23 +399,17 @@ constexpr int WAVE_COLS = 4096, GROUP_COLS = 8192;
 constexpr int GRAD_COLS = 16384;     // the longest row of the gradient's one-pass form (512 lanes, 4 chunks each)
 int grad_parts(int rows, int cols) {
     if (cols > GRAD_COLS) return rows < 64 ? rows : 64;
-    const int rpb = cols <= 1024 ? 4 : 1, most = cols <= 2048 ? 1024 : cols <= 4096 ? 768 : cols <= 8192 ? 512 : 256;
-    const int groups = (rows + 2 * rpb - 1) / (2 * rpb);
-    return groups < most ? groups : most;
+    const int64_t rpb = cols <= 1024 ? 4 : 1, most = cols <= 2048 ? 1024 : cols <= 4096 ? 768 : cols <= 8192 ? 512 : 256;
+    const int64_t groups = (rows + 2 * rpb - 1) / (2 * rpb);
+    return (int)(groups < most ? groups : most);
 }
 
 template <typename T, bool Q8>
-int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, const void* w, void* y, int64_t y_rs,
-                void* q_scale, void* h, int64_t h_rs, int rows, int cols, float eps, void* stream) {
-    FP_REQUIRE(x && w && y && rows >= 0 && cols > 0 && x_rs >= 0 && y_rs >= cols);
-    FP_REQUIRE(!resid == !h && (!resid || (r_rs >= 0 && h_rs >= cols)) && eps >= 0.f);
-    FP_REQUIRE(aligned2(x) && aligned2(resid) && aligned2(w) && (Q8 || aligned2(y)) && aligned2(h));
-    FP_REQUIRE(!Q8 || (q_scale && ((uintptr_t)q_scale & 3) == 0));
-    if (rows == 0) return 0;
-    hipStream_t st = (hipStream_t)stream;
+int norm_rows(const T* x, int64_t x_rs, const T* resid, int64_t r_rs, const T* w, T* y, int64_t y_rs, float* q_scale, T* h, int64_t h_rs,
+              int rows, int cols, float eps, hipStream_t st) {
 #define FP_NORM(TPR, NCH)                                                                                                         \
     rmsnorm_kernel<T, Q8, TPR, NCH><<<dim3((unsigned)(TPR < 256 ? (rows + 3) / 4 : rows)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>( \
-        (const T*)x, x_rs, (const T*)resid, r_rs, (const T*)w, (T*)y, y_rs, (float*)q_scale, (T*)h, h_rs, rows, cols, eps)
+        x, x_rs, resid, r_rs, w, y, y_rs, q_scale, h, h_rs, rows, cols, eps)
     const int nch = (cols + 7) / 8;
     if (cols <= 512 || (cols <= WAVE_COLS && rows >= 2048)) {
         if (nch <= 64) FP_NORM(64, 1);
@@ -431,17 +425,38 @@ int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, co
         else if (nch <= 4096) FP_NORM(1024, 4);
         else FP_NORM(1024, 8);
     } else {
-        rmsnorm_rows_kernel<T, Q8><<<dim3((unsigned)rows), dim3(256), 0, st>>>((const T*)x, x_rs, (const T*)resid, r_rs, (const T*)w,
-                                                                              (T*)y, y_rs, (float*)q_scale, (T*)h, h_rs, cols, eps);
+        rmsnorm_rows_kernel<T, Q8><<<dim3((unsigned)rows), dim3(256), 0, st>>>(x, x_rs, resid, r_rs, w, y, y_rs, q_scale, h, h_rs, cols, eps);
     }
 #undef FP_NORM
     FP_CHECK_LAUNCH();
     return 0;
 }
 
+template <typename T, bool Q8>
+int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, const void* w, void* y, int64_t y_rs,
+                void* q_scale, void* h, int64_t h_rs, int rows, int cols, float eps, void* stream) {
+    FP_REQUIRE(x && w && y && rows >= 0 && cols > 0 && x_rs >= 0 && y_rs >= cols);
+    FP_REQUIRE(!resid == !h && (!resid || (r_rs >= 0 && h_rs >= cols)) && eps >= 0.f);
+    FP_REQUIRE(aligned2(x) && aligned2(resid) && aligned2(w) && (Q8 || aligned2(y)) && aligned2(h));
+    FP_REQUIRE(!Q8 || (q_scale && ((uintptr_t)q_scale & 3) == 0));
+    if (rows == 0) return 0;
+    hipStream_t st = (hipStream_t)stream;
+    constexpr int MOST = 1 << 21;      // rows a launch: its lanes have to stay below 2^32
+    for (int64_t r = 0; r < rows; r += MOST) {
+        // (y_rs counts bytes where y is e4m3)
+        T* yr = Q8 ? (T*)((unsigned char*)y + r * y_rs) : (T*)y + r * y_rs;
+        if (int rc = norm_rows<T, Q8>((const T*)x + r * x_rs, x_rs, resid ? (const T*)resid + r * r_rs : nullptr, r_rs, (const T*)w, yr, y_rs,
+                                      Q8 ? (float*)q_scale + r : nullptr, h ? (T*)h + r * h_rs : nullptr, h_rs,
+                                      rows - r < MOST ? (int)(rows - r) : MOST, cols, eps, st))
+            return rc;
+    }
+    return 0;
+}
+
 template <typename T>
 int grad_launch(const void* dy, int64_t dy_rs, const void* h, int64_t h_rs, const void* dh, int64_t dh_rs, const void* w,
                 void* dx, int64_t dx_rs, void* dw, int rows, int cols, float eps, void* ws, int64_t ws_bytes, void* stream) {
+    FP_REQUIRE(cols <= GRAD_COLS || rows <= 1 << 21);           // (a workgroup per row there)
     FP_REQUIRE(dy && h && w && dx && dw && rows > 0 && cols > 0 && dy_rs >= 0 && h_rs >= 0 && dx_rs >= cols && eps >= 0.f);
     FP_REQUIRE(!dh || dh_rs >= 0);
     FP_REQUIRE(aligned2(dy) && aligned2(h) && aligned2(dh) && aligned2(w) && aligned2(dx) && aligned2(dw));

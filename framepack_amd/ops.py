@@ -690,6 +690,9 @@ def attention_framecausal(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, q_
 ACT_SILU, ACT_GELU = 0, 1          # GELU: the tanh form, as in EPI_GELU
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
 def _mat(t: torch.Tensor, what: str, dtypes, rows: int = -1, cols: int = -1):
     """(tensor, rows, cols, row stride) of a matrix argument of K12 / K13: [.., rows, cols] as `_rows2d` takes it, of one
     of `dtypes`, of `rows` and `cols` if given.  A single row's stride says nothing and is replaced by the row's length."""
@@ -703,6 +706,8 @@ def _mat(t: torch.Tensor, what: str, dtypes, rows: int = -1, cols: int = -1):
             raise ValueError(f"{what}: expected a [rows, cols] tensor, got {tuple(t.shape)} / {t.stride()}")
     r, c = t.shape
     rs, cs = t.stride()
+    if r > _INT_MAX or c > _INT_MAX:                   # (the library's sizes are C ints)
+        raise ValueError(f"{what}: more than {_INT_MAX} rows or columns, got {[r, c]}")
     if c == 0 or (rows >= 0 and r != rows) or (cols >= 0 and c != cols):
         raise ValueError(f"{what}: expected [{rows if rows >= 0 else 'rows'}, {cols if cols >= 0 else 'at least one column'}], "
                          f"got {[r, c]}")

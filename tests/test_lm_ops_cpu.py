@@ -46,6 +46,7 @@ def test_norm_refusals(no_device_check):
         (lambda: ops.rmsnorm_residual(torch.zeros(4, 128, dtype=BF)[:, ::2], w), "unit inner stride"),
         (lambda: ops.rmsnorm_residual(torch.zeros(4, 0, dtype=BF), w[:0]), "column"),
         (lambda: ops.rmsnorm_residual(x, w, eps=-1.0), "eps"),
+        (lambda: ops.rmsnorm_residual(x[:1].expand(2 ** 32 + 4, 64), w), "more than"),
         (lambda: ops.rmsnorm_residual(x, w, eps=float("nan")), "eps"),
         (lambda: ops.rmsnorm_residual(x, w, resid_out=r), "without resid"),
         (lambda: ops.rmsnorm_residual(x, w, r, out=torch.zeros(4, 32, dtype=BF)), "out"),
@@ -155,3 +156,52 @@ def test_the_library_refuses_without_launching():
     for i, v in ((0, None), (2, None), (4, None), (8, None), (12, None), (13, None), (5, K - 1), (7, K - 1), (12, p + 8), (13, p + 2),
                  (14, p + 1), (15, 0), (16, 0), (17, 0), (15, 1 << 20), (18, 3), (19, None), (19, p + 8), (20, 16)):
         refused("fp_gated_ff_backward_f16", *[v if j == i else t for j, t in enumerate(ok)])
+
+
+def test_fragment_reads_of_the_gated_blocks_products_all_feed_an_mfma(tmp_path):
+    """The 16-bit instances of the 4-wave kernel read their MFMA fragments with inline asm - K13's gradient with pairs of
+    transposing reads - whose results the compiler takes for written at once.  Compile K13's products to assembly with the
+    Makefile's flags and check, per kernel: no register of a read in flight is touched by a compiler instruction or written
+    by another read before an MFMA has taken it, every read is taken, nothing goes to scratch memory."""
+    import os
+    import re
+    import subprocess
+    hipcc = "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("needs hipcc")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "framepack_amd", "csrc")
+    mk = open(os.path.join(csrc, "Makefile")).read()
+    flags = re.search(r"^CXXFLAGS = (.*)$", mk, re.M).group(1).replace("$(ARCH)", "gfx950").replace("-fPIC", "").split()
+    files = ("gated_ff_mfma", "gated_ff_grad_mfma")
+    procs = [subprocess.Popen([hipcc, *flags, "-S", "--cuda-device-only", os.path.join(csrc, f + ".hip"), "-o", str(tmp_path / (f + ".s"))],
+                              stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL) for f in files]
+    seen = transposing = 0
+    for f, pr in zip(files, procs):
+        assert pr.wait() == 0, f
+        text = (tmp_path / (f + ".s")).read_text()
+        for m in re.finditer(r"^(_ZN7fp_gemm14gemm_w4_kernel\S*):[^\n]*\n(.*?)^\s*\.amdhsa_kernel \1", text, re.S | re.M):
+            name, body = m.group(1), m.group(2)
+            seen += 1
+            pending, in_asm = {}, False                     # register -> the read that is on its way into it
+            for line in body.splitlines():
+                t = line.strip()
+                if "#ASMSTART" in t or "#ASMEND" in t:
+                    in_asm = "#ASMSTART" in t
+                    continue
+                regs = {int(r) for r in re.findall(r"\bv(\d+)\b", t)}
+                for lo, hi in re.findall(r"\bv\[(\d+):(\d+)\]", t):
+                    regs |= set(range(int(lo), int(hi) + 1))
+                rd = re.match(r"ds_read_(b128|b64_tr_b16) v\[(\d+):(\d+)\], v(\d+)", t) if in_asm else None
+                if rd:
+                    assert not regs & set(pending), (name, "a fragment read is overwritten before any MFMA used it", t)
+                    transposing += rd.group(1) != "b128"
+                    pending.update({r: t for r in range(int(rd.group(2)), int(rd.group(3)) + 1)})
+                elif t.startswith("v_mfma"):
+                    for r in regs:
+                        pending.pop(r, None)
+                elif not in_asm:
+                    assert not regs & set(pending), (name, "register of an in-flight fragment read touched", t)
+            assert not pending, (name, "fragment reads that no MFMA takes", pending)
+            assert int(re.search(re.escape(name) + r"\.num_vgpr, (\d+)", text).group(1)) <= 256
+            assert int(re.search(re.escape(name) + r"\.private_seg_size, (\d+)", text).group(1)) == 0
+    assert seen >= 16 and transposing > 0

@@ -536,16 +536,37 @@ def test_empty_batches():
     assert dx.shape == (0, 64) and all((t == 0).all() for t in (dwg, dwu, dbg, dbu)) and dwg.shape == (16, 64)
 
 
-def test_matrices_past_two_gigabytes():
-    rows, cols = 70000, 16384                              # 2.3 GB a matrix: byte offsets past 2^31, elements past 2^30
+def test_matrices_past_four_gigabytes():
+    rows, cols = 140000, 16384                             # 4.6 GB a matrix: byte offsets past 2^32, elements past 2^31
     x = torch.randn(64, cols, device=DEV).to(BF).repeat(rows // 64 + 1, 1)[:rows]
     w = randn(cols, seed=1, dtype=BF)
     y, h = ops.rmsnorm_residual(x, w, x)
     want, _ = ops.rmsnorm_residual(x[:64].contiguous(), w, x[:64].contiguous())
     assert torch.equal(y[rows // 64 * 64 - 64:rows // 64 * 64], want) and torch.equal(y[:64], want)
-    del y, h
+    dx, _ = ops.rmsnorm_residual_backward(y, x, w, dh=x)
+    want, _ = ops.rmsnorm_residual_backward(y[:64], x[:64], w, dh=x[:64])
+    assert torch.equal(dx[rows // 64 * 64 - 64:rows // 64 * 64], want)
+    del y, h, dx
     wg = randn(64, cols, seed=2, scale=cols ** -0.5, dtype=BF)
     a = ops.gated_ff(x, wg, wg)
     want = ops.gated_ff(x[:256].contiguous(), wg, wg)
     k = rows // 256 * 256
     assert torch.equal(a[:256], want) and torch.equal(a[k - 256:k], want)
+    dh = a[:64].repeat(rows // 64 + 1, 1)[:rows]
+    dx, _, _, _, _ = ops.gated_ff_backward(dh, x, wg, wg, a, a)
+    want, _, _, _, _ = ops.gated_ff_backward(dh[:256], x[:256], wg, wg, a[:256], a[:256])
+    # (a product of another size may be cut into other parts of K: the same sums in another order, rounded once)
+    within(dx[k - 256:k], want, want.double().abs() * 2 * u_of(BF) + 1e-3 * want.double().abs().max())
+
+
+def test_norm_of_more_rows_than_a_launch_takes():
+    rows = (1 << 22) + 77
+    x = torch.randn(rows, 8, device=DEV).to(BF)
+    w = randn(8, seed=1, dtype=BF)
+    y, h = ops.rmsnorm_residual(x, w, x)
+    h64, y64 = norm64(x, x, w)
+    within(y, y64, norm_tol(y64, BF, 8))
+    within(h, h64, h64.abs() * (u_of(BF) + 2 * E32))
+    q, s, _ = ops.rmsnorm_residual_fp8(x, w, x)
+    within(s, y64.abs().amax(1) / 448, y64.abs().amax(1) / 448 * 16 * E32)
+    within(q.double() * s.double()[:, None], y64, y64.abs() * 2.0 ** -4 * 1.001 + s.double()[:, None] * 2.0 ** -10)
