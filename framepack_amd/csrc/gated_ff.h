@@ -11,6 +11,12 @@ __attribute__((visibility("hidden"))) int fpi_glu(int type, const void* x, int64
                                                   const void* bu, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M,
                                                   int F, int K, int act, hipStream_t st);
 
+// The same in fp32 parts of K, without scales, biases and activation: part[s] [M, 2 Fp], x . wg^T from column 0, x . wu^T from
+// column Fp = F rounded up to 8 on, over the K tiles (128 bytes) of part s: ks_per each, the last part the rest.
+__attribute__((visibility("hidden"))) int fpi_glu_parts(int type, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu,
+                                                        int64_t ldwu, float* part, int M, int F, int K, int splits, int ks_per,
+                                                        hipStream_t st);
+
 // The gradient's products: out [M, N] = a [M, K] . w with w's K tiles as they lie, 64 rows of N each; tile t at w + t tiles,
 // + d1 bytes from tile s1 on, + d2 from tile s2 on (gemm_w4.h, TrArgs).  out in 16 bits (splits = 0; row stride N, 16-byte
 // aligned) or fp32 parts [splits][M, N] over ks_per K tiles each.  narrow: 256 x 128 tiles instead of 256 x 256 (as the

@@ -3,6 +3,7 @@
 // include/framepack_hip.h.
 //
 //   dg = dh u act'(g)   du = dh act(g)   dx = dg . Wg + du . Wu   dWg = dg^T . x   dWu = du^T . x   db = column sums
+#include <algorithm>
 #include <type_traits>
 #include "gated_ff.h"
 #include "gemm_pipeline.h"
@@ -72,8 +73,9 @@ __device__ __forceinline__ f32x4 mma(fp8e4, const u32x4& w, const u32x4& x, f32x
     c = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(a[0], b[0], c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(a[1], b[1], c, 0, 0, 0);
 }
-template <typename TI, typename TO, int MT, int NC, int STEPS>
-__global__ __launch_bounds__(256) void glu_few_kernel(GluCall q) {
+// PARTS: blockIdx.y takes per_part steps of K and leaves both projections' sums, [part][M][2 Fp] (see glu_finish_kernel).
+template <typename TI, typename TO, int MT, int NC, int STEPS, bool PARTS>
+__global__ __launch_bounds__(256) void glu_few_kernel(GluCall q, float* __restrict__ parts, int per_part) {
     constexpr int NW = 4;
     typedef u32x4 Q __attribute__((aligned(1)));
     constexpr int STEP = 128 / (int)sizeof(TI), E = 16 / (int)sizeof(TI);      // elements of a step, of a 16-byte load
@@ -82,15 +84,15 @@ __global__ __launch_bounds__(256) void glu_few_kernel(GluCall q) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = lane & 15, ch = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * (16 * NC);
-    const int m0 = blockIdx.y * (MT * 16);
     const TI *pw[G], *px[MT];
 #pragma unroll
     for (int g = 0; g < G; ++g)
         pw[g] = reinterpret_cast<const TI*>(q.w[g & 1]) + min(n0 + (g >> 1) * 16 + row, (int64_t)q.F - 1) * q.ldw[g & 1] + ch * E;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) px[t] = reinterpret_cast<const TI*>(q.x) + (int64_t)min(m0 + t * 16 + row, q.M - 1) * q.ldx + ch * E;
+    for (int t = 0; t < MT; ++t) px[t] = reinterpret_cast<const TI*>(q.x) + (int64_t)min(t * 16 + row, q.M - 1) * q.ldx + ch * E;
     f32x4 acc[G][MT] = {};
-    const int steps = q.K / STEP;
+    const int steps = q.K / STEP;                              // whole ones
+    const int first = PARTS ? (int)blockIdx.y * per_part : 0, end = PARTS ? min(steps, first + per_part) : steps;
     auto run = [&](auto U_, int s) {                           // the loads of U steps go out together
         constexpr int U = decltype(U_)::value;
         u32x4 w[U][G][2], x[U][MT][2];
@@ -114,11 +116,11 @@ __global__ __launch_bounds__(256) void glu_few_kernel(GluCall q) {
 #pragma unroll
                     for (int t = 0; t < MT; ++t) acc[g][t] = mma(TI{}, w[i][g][c], x[i][t][c], acc[g][t]);
     };
-    int s = wave;
+    int s = first + wave;
     if constexpr (STEPS > 1)
-        for (; s + (STEPS - 1) * NW < steps; s += STEPS * NW) run(std::integral_constant<int, STEPS>{}, s);
-    for (; s < steps; s += NW) run(std::integral_constant<int, 1>{}, s);
-    if (steps * STEP < q.K && wave == steps % NW) {
+        for (; s + (STEPS - 1) * NW < end; s += STEPS * NW) run(std::integral_constant<int, STEPS>{}, s);
+    for (; s < end; s += NW) run(std::integral_constant<int, 1>{}, s);
+    if (steps * STEP < q.K && end == steps && wave == steps % NW && (!PARTS || blockIdx.y == gridDim.y - 1)) {
         auto part = [&](const TI* p, int c) {                  // 16 bytes of the step, zeros past the end of the row
             TI v[E];
 #pragma unroll
@@ -153,7 +155,7 @@ __global__ __launch_bounds__(256) void glu_few_kernel(GluCall q) {
     __syncthreads();
     for (int i = tid; i < NC * MT * 256; i += NW * 64) {
         const int col = i & 15, nc = (i >> 4) % NC, tok = (i / (16 * NC)) & 15, t = i / (256 * NC);
-        const int64_t m = m0 + t * 16 + tok, nn = n0 + nc * 16 + col;
+        const int64_t m = t * 16 + tok, nn = n0 + nc * 16 + col;
         if (m >= q.M || nn >= q.F) continue;
         float v[2];
 #pragma unroll
@@ -161,12 +163,56 @@ __global__ __launch_bounds__(256) void glu_few_kernel(GluCall q) {
             v[g] = red[0][2 * nc + g][t][col * 17 + tok];
 #pragma unroll
             for (int w = 1; w < NW; ++w) v[g] += red[w][2 * nc + g][t][col * 17 + tok];
+            if constexpr (PARTS) {
+                const int64_t Fp = (q.F + 7) & ~7;
+                parts[((int64_t)blockIdx.y * q.M + m) * (2 * Fp) + g * Fp + nn] = v[g];
+                continue;
+            }
             if (sizeof(TI) == 1) v[g] *= q.xs[m] * q.ws[g][nn];
             if (q.b[g]) v[g] += (float)reinterpret_cast<const TO*>(q.b[g])[nn];
             if (q.pre[g]) reinterpret_cast<TO*>(q.pre[g])[m * q.ldp + nn] = (TO)v[g];
         }
-        reinterpret_cast<TO*>(q.h)[m * q.ldh + nn] = (TO)(act_of(v[0], q.act) * v[1]);
+        if constexpr (!PARTS) reinterpret_cast<TO*>(q.h)[m * q.ldh + nn] = (TO)(act_of(v[0], q.act) * v[1]);
     }
+}
+
+// h (and the projections) from the parts of K [splits][M][2 Fp], Fp = F rounded up to 8: added up in their order, then what the
+// one-pass kernels do at their ends.  A lane takes four columns.
+template <typename TO, bool SCALED>
+__global__ __launch_bounds__(256) void glu_finish_kernel(GluCall q, const float* __restrict__ parts, int splits) {
+    typedef TO A4 __attribute__((ext_vector_type(4), aligned(2)));
+    const int64_t Fp = (q.F + 7) & ~7, per = Fp / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= q.M * per) return;
+    const int64_t m = i / per;
+    const int n = (int)(i - m * per) * 4;
+    f32x4 v[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const float* p = parts + m * (2 * Fp) + g * Fp + n;
+        v[g] = *reinterpret_cast<const f32x4*>(p);
+        for (int s = 1; s < splits; ++s) v[g] += *reinterpret_cast<const f32x4*>(p + (int64_t)s * q.M * (2 * Fp));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (n + j >= q.F) continue;
+            if (SCALED) v[g][j] *= q.xs[m] * q.ws[g][n + j];
+            if (q.b[g]) v[g][j] += (float)reinterpret_cast<const TO*>(q.b[g])[n + j];
+        }
+    }
+    const A4 o = {(TO)(act_of(v[0][0], q.act) * v[1][0]), (TO)(act_of(v[0][1], q.act) * v[1][1]), (TO)(act_of(v[0][2], q.act) * v[1][2]),
+                  (TO)(act_of(v[0][3], q.act) * v[1][3])};
+    auto put = [&](TO* to, const A4& a) {
+        if (n + 4 <= q.F) {
+            *reinterpret_cast<A4*>(to) = a;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (n + j < q.F) to[j] = a[j];
+        }
+    };
+    put(reinterpret_cast<TO*>(q.h) + m * q.ldh + n, o);
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+        if (q.pre[g]) put(reinterpret_cast<TO*>(q.pre[g]) + m * q.ldp + n, A4{(TO)v[g][0], (TO)v[g][1], (TO)v[g][2], (TO)v[g][3]});
 }
 
 // ---- the gradient -------------------------------------------------------------------------------------------------
@@ -410,6 +456,34 @@ int product(GradProduct p, T* out, int N, float* parts, hipStream_t st) {
     return 0;
 }
 
+// How a forward call runs.  e: bytes of an operand's element.
+struct Plan {
+    bool few, two;                  // stream the weights; two column tiles a workgroup
+    bool x_fits, g_fits, u_fits;    // (not few) what the matrix-core kernel can read as it lies
+    int splits, per;                // parts of K, steps (few) or K tiles of each; 1: no parts
+    int64_t parts, bytes;           // where the parts begin in the workspace, and its end
+};
+Plan plan(int e, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu, int64_t M, int64_t F, int K) {
+    Plan p{};
+    p.few = M <= FEW;
+    // two column tiles where that leaves a workgroup per CU; one for the fewest tokens in 16 bits
+    p.two = F >= 8192 && (M > 8 || e == 1);
+    p.x_fits = p.g_fits = p.u_fits = true;
+    if (!p.few && e == 2) p.x_fits = wide_rows(x, ldx, K), p.g_fits = wide_rows(wg, ldwg, K), p.u_fits = wide_rows(wu, ldwu, K);
+    // Parts of K where the output's tiles leave CUs idle and K is long enough to pay for the second launch: as many as there are
+    // CUs, of at least 8 steps.  One launch / in parts, us: rows, [K, F] = 128, [4096, 4096] 49 / 28; 87, [6784, 120] 62 / 18;
+    // 300, [2048, 1024] 24 / 20; 300, [1024, 1024] 15.3 / 16.4; streamed: 16, [8192, 1024] 24 / 14; 1, [2048, 1024] 6.4 / 7.4.
+    const int64_t nk = (p.few ? (int64_t)K : up64(K)) * e / 128, tiles = p.few ? (F + 15) / 16 : (M + 255) / 256 * ((F + 63) / 64);
+    int64_t s = 1;
+    if (p.few ? tiles <= 64 && nk >= 64 : tiles <= 128 && nk >= 24) s = std::min(256 / tiles, nk / 8);
+    p.per = (int)((nk + s - 1) / s);
+    p.splits = p.per > 0 ? (int)((nk + p.per - 1) / p.per) : 1;
+    const int64_t copied = (p.x_fits ? 0 : M) + (p.g_fits ? 0 : F) + (p.u_fits ? 0 : F);
+    p.parts = (copied * up64(K) * 2 + 255) & ~(int64_t)255;
+    p.bytes = p.splits > 1 ? p.parts + (int64_t)p.splits * M * 2 * up8(F) * 4 : copied * up64(K) * 2;
+    return p;
+}
+
 template <typename T>
 int copy_rows(Copies c, int cols, int cols_p, hipStream_t st) {
     c.cols = cols;
@@ -436,44 +510,59 @@ int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64
     hipStream_t st = (hipStream_t)stream;
     constexpr int type = sizeof(TI) == 1 ? FF_E4M3 : __is_same(TI, bf16) ? FF_BF16 : FF_F16;
     const GluCall q{x, ldx, xs, {wg, wu}, {ldwg, ldwu}, {gs, us}, {bg, bu}, h, ldh, {gate, up}, ldp, M, F, K, act};
-    if (M <= FEW) {
+    const Plan p = plan(sizeof(TI), x, ldx, wg, ldwg, wu, ldwu, M, F, K);
+    FP_REQUIRE(p.bytes == 0 || (ws && aligned16(ws) && ws_bytes >= p.bytes));
+    float* parts = (float*)((char*)ws + p.parts);
+    if (p.few) {
         const int mt = (M + 15) / 16;
-        // two column tiles a workgroup where that leaves a workgroup per CU; one for the fewest tokens in 16 bits
-        const bool two = F >= 8192 && (M > 8 || sizeof(TI) == 1);
-#define FP_FEW(MT, NC, STEPS) glu_few_kernel<TI, TO, MT, NC, STEPS><<<dim3((unsigned)((F + 16 * NC - 1) / (16 * NC))), dim3(256), 0, st>>>(q)
-        if (mt == 1) {
-            if (two) FP_FEW(1, 2, 1);
-            else FP_FEW(1, 1, 2);
+#define FP_FEW(MT, NC, STEPS, PARTS)                                                                                                        \
+    glu_few_kernel<TI, TO, MT, NC, STEPS, PARTS><<<dim3((unsigned)((F + 16 * NC - 1) / (16 * NC)), PARTS ? p.splits : 1), dim3(256), 0, st>>>( \
+        q, parts, p.per)
+        if (p.splits > 1) {
+            if (mt == 1) FP_FEW(1, 1, 2, true);
+            else if (mt == 2) FP_FEW(2, 1, 1, true);
+            else FP_FEW(3, 1, 1, true);
+        } else if (mt == 1) {
+            if (p.two) FP_FEW(1, 2, 1, false);
+            else FP_FEW(1, 1, 2, false);
         } else if (mt == 2) {
-            if (two) FP_FEW(2, 2, 1);
-            else FP_FEW(2, 1, 1);
+            if (p.two) FP_FEW(2, 2, 1, false);
+            else FP_FEW(2, 1, 1, false);
         } else {
-            if (two) FP_FEW(3, 2, 1);
-            else FP_FEW(3, 1, 1);
+            if (p.two) FP_FEW(3, 2, 1, false);
+            else FP_FEW(3, 1, 1, false);
         }
 #undef FP_FEW
         FP_CHECK_LAUNCH();
-        return 0;
-    }
-    // The matrix-core kernel stages its operands 16 bytes a lane and in whole K tiles, with 32-bit offsets inside a tile: what
-    // does not fit that is copied into rows that do.
-    if constexpr (sizeof(TI) == 2) {
-        const bool x_fits = wide_rows(x, ldx, K), g_fits = wide_rows(wg, ldwg, K), u_fits = wide_rows(wu, ldwu, K);
-        if (!x_fits || !g_fits || !u_fits) {
-            const int64_t Kp = up64(K);
-            FP_REQUIRE(K <= LIMIT && F <= LIMIT && ws && aligned16(ws) &&
-                       ws_bytes >= fp_gated_ff_workspace_bytes(x, ldx, wg, ldwg, wu, ldwu, M, F, K));
-            TI *xp = (TI*)ws, *gp = xp + (x_fits ? 0 : M * Kp), *upk = gp + (g_fits ? 0 : F * Kp);
-            Copies c{{x, wg, wu}, {xp, gp, upk}, {ldx, ldwg, ldwu}, {Kp, Kp, Kp}};
-            c.rows[0] = c.rows_p[0] = x_fits ? 0 : M;
-            c.rows[1] = c.rows_p[1] = g_fits ? 0 : F;
-            c.rows[2] = c.rows_p[2] = u_fits ? 0 : F;
-            if (int rc = copy_rows<TI>(c, K, (int)Kp, st)) return rc;
-            return fpi_glu(type, x_fits ? x : xp, x_fits ? ldx : Kp, xs, g_fits ? wg : gp, g_fits ? ldwg : Kp, gs, u_fits ? wu : upk,
-                           u_fits ? ldwu : Kp, us, bg, bu, h, ldh, gate, up, ldp, M, F, (int)Kp, act, st);
+    } else {
+        // The matrix-core kernel stages its operands 16 bytes a lane and in whole K tiles, with 32-bit offsets inside a tile:
+        // what does not fit that is copied into rows that do.
+        int Kp = K;
+        if constexpr (sizeof(TI) == 2) {
+            if (!p.x_fits || !p.g_fits || !p.u_fits) {
+                FP_REQUIRE(K <= LIMIT && F <= LIMIT);
+                Kp = (int)up64(K);
+                TI *xp = (TI*)ws, *gp = xp + (p.x_fits ? 0 : (int64_t)M * Kp), *upk = gp + (p.g_fits ? 0 : (int64_t)F * Kp);
+                Copies c{{x, wg, wu}, {xp, gp, upk}, {ldx, ldwg, ldwu}, {Kp, Kp, Kp}};
+                c.rows[0] = c.rows_p[0] = p.x_fits ? 0 : M;
+                c.rows[1] = c.rows_p[1] = p.g_fits ? 0 : F;
+                c.rows[2] = c.rows_p[2] = p.u_fits ? 0 : F;
+                if (int rc = copy_rows<TI>(c, K, Kp, st)) return rc;
+                if (!p.x_fits) x = xp, ldx = Kp;
+                if (!p.g_fits) wg = gp, ldwg = Kp;
+                if (!p.u_fits) wu = upk, ldwu = Kp;
+            }
         }
+        if (p.splits == 1)
+            return fpi_glu(type, x, ldx, xs, wg, ldwg, gs, wu, ldwu, us, bg, bu, h, ldh, gate, up, ldp, M, F, Kp, act, st);
+        if (int rc = fpi_glu_parts(type, x, ldx, wg, ldwg, wu, ldwu, parts, M, F, Kp, p.splits, p.per, st)) return rc;
     }
-    return fpi_glu(type, x, ldx, xs, wg, ldwg, gs, wu, ldwu, us, bg, bu, h, ldh, gate, up, ldp, M, F, K, act, st);
+    if (p.splits > 1) {
+        const int64_t lanes = (int64_t)M * (up8(F) / 4);
+        glu_finish_kernel<TO, sizeof(TI) == 1><<<dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st>>>(q, parts, p.splits);
+        FP_CHECK_LAUNCH();
+    }
+    return 0;
 }
 
 template <typename T>
@@ -527,10 +616,13 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
 
 extern "C" int64_t fp_gated_ff_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
                                                int M, int F, int K) {
-    if (M <= FEW || F <= 0 || K <= 0 || F > LIMIT || K > LIMIT) return 0;
-    const int64_t rows = (wide_rows(x, ldx, K) ? 0 : (int64_t)M) + (wide_rows(w_gate, ldwg, K) ? 0 : (int64_t)F) +
-                         (wide_rows(w_up, ldwu, K) ? 0 : (int64_t)F);
-    return rows * up64(K) * 2;
+    if (M <= 0 || F <= 0 || K <= 0 || M > 1 << 30 || F > 1 << 30 || K > 1 << 30) return 0;
+    return plan(2, x, ldx, w_gate, ldwg, w_up, ldwu, M, F, K).bytes;
+}
+
+extern "C" int64_t fp_gated_ff_fp8_workspace_bytes(int M, int F, int K) {
+    if (M <= 0 || F <= 0 || K <= 0 || M > 1 << 30 || F > 1 << 30 || K > 1 << 30) return 0;
+    return plan(1, nullptr, 0, nullptr, 0, nullptr, 0, M, F, K).bytes;
 }
 
 extern "C" int fp_gated_ff_bf16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
@@ -551,13 +643,13 @@ extern "C" int fp_gated_ff_f16(const void* x, int64_t ldx, const void* w_gate, i
 
 extern "C" int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, const void* w_gate, int64_t ldwg, const void* wg_scale,
                                const void* w_up, int64_t ldwu, const void* wu_scale, const void* b_gate, const void* b_up, void* h,
-                               int64_t ldh, int M, int F, int K, int act, void* stream) {
+                               int64_t ldh, int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream) {
     FP_REQUIRE(x_scale && wg_scale && wu_scale && K > 0 && K % 128 == 0 && F > 0 && F % 8 == 0);
     FP_REQUIRE(aligned16(x) && aligned16(w_gate) && aligned16(w_up) && aligned16(h) && ldx % 16 == 0 && ldwg % 16 == 0 &&
                ldwu % 16 == 0 && ldh % 8 == 0 && ldx >= 0);
     FP_REQUIRE(((uintptr_t)x_scale & 3) == 0 && aligned16(wg_scale) && aligned16(wu_scale) && aligned16(b_gate) && aligned16(b_up));
     return ff_launch<fp8e4, bf16>(x, ldx, (const float*)x_scale, w_gate, ldwg, (const float*)wg_scale, w_up, ldwu,
-                                  (const float*)wu_scale, b_gate, b_up, h, ldh, nullptr, nullptr, 0, M, F, K, act, nullptr, 0, stream);
+                                  (const float*)wu_scale, b_gate, b_up, h, ldh, nullptr, nullptr, 0, M, F, K, act, workspace, workspace_bytes, stream);
 }
 
 extern "C" int64_t fp_gated_ff_backward_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up,

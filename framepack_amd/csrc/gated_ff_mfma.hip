@@ -36,3 +36,21 @@ int fpi_glu(int type, const void* x, int64_t ldx, const float* xs, const void* w
     FP_GLU(_Float16, _Float16, 8, 0);
 #undef FP_GLU
 }
+
+int fpi_glu_parts(int type, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu, float* part, int M, int F,
+                  int K, int splits, int ks_per, hipStream_t st) {
+    const int64_t Fp = (F + 7) & ~7;
+    const GluArgs glu{wu, nullptr, ldwu, nullptr, nullptr, nullptr, Fp, 0};
+    const SplitArgs sp{splits, ks_per};
+    const ConvGeom cg{};
+    const int nk = K / (type == FF_E4M3 ? 128 : 64);
+    FP_REQUIRE((int64_t)((M + BM - 1) / BM) * ((F + 63) / 64) * splits < (1ll << 31));
+    FP_REQUIRE(splits > 0 && (int64_t)(splits - 1) * ks_per < nk && (int64_t)splits * ks_per >= nk);
+#define FP_PARTS(T)                                                                                                                     \
+    return launch_w4<T, 0, 0, float, 4, 0, 0, 0, 1, 0, 1>(x, ldx, 0, K, wg, ldwg, nullptr, part, 2 * Fp, M, F, K, 0, nullptr, 0, nullptr, cg, \
+                                                          st, nullptr, nullptr, QkNormArgs{}, Rows2{}, glu, sp)
+    if (type == FF_E4M3) FP_PARTS(fp8e4);
+    if (type == FF_BF16) FP_PARTS(bf16);
+    FP_PARTS(_Float16);
+#undef FP_PARTS
+}

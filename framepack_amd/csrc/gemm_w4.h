@@ -173,8 +173,9 @@ __device__ __forceinline__ float glu_act(float v, float c0, float c1) {
 }
 __device__ __forceinline__ float glu_c0(int act) { return 1.4426950408889634f * (act ? 2.f * 0.7978845608028654f : 1.f); }
 __device__ __forceinline__ float glu_c1(int act) { return act ? 1.4426950408889634f * 2.f * 0.7978845608028654f * 0.044715f : 0.f; }
-// SPLIT > 0 (gated_ff.hip's dx: few output tiles, a long K): the K tiles are dealt to `splits` workgroups per output tile in
-// runs of ks_per, and part s goes to rows [s M, (s + 1) M) of the fp32 output; the caller adds them up.
+// SPLIT > 0 (gated_ff.hip: few output tiles, a long K): the K tiles are dealt to `splits` workgroups per output tile in runs of
+// ks_per, and part s goes to rows [s M, (s + 1) M) of the fp32 output; the caller adds them up.  With GLU, both projections'
+// sums: the first from column 0 on, the second from column ldp on (ldp >= N a multiple of 4; columns up to it are written).
 struct SplitArgs {
     int splits, ks_per;
 };
@@ -202,8 +203,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                                                          GluArgs glu, SplitArgs sp, TrArgs tr) {
     static_assert(!TRW || (AMODE == 0 && !TALL && !QKN && !GRP && !GLU && EPI == 0 && sizeof(T) == 2 && (NT == 8 || NT == 4)),
                   "W by rows of K: the dense 16-bit tile");
-    static_assert(!GLU || (AMODE == 0 && !TALL && !QKN && !GRP && EPI == 0 && sizeof(TO) == 2 && NT >= 4), "gated block: the dense tile");
-    static_assert(!SPLIT || (AMODE == 0 && !TALL && !QKN && !GRP && !GLU && EPI == 0 && sizeof(TO) == 4), "parts of K: fp32 out");
+    static_assert(!GLU || (AMODE == 0 && !TALL && !QKN && !GRP && EPI == 0 && sizeof(TO) == (SPLIT ? 4 : 2) && NT >= 4), "gated block: the dense tile");
+    static_assert(!SPLIT || (AMODE == 0 && !TALL && !QKN && !GRP && !KEEP && EPI == 0 && sizeof(TO) == 4), "parts of K: fp32 out");
     static_assert(!GRP || (AMODE == 0 && !TALL && !QKN && NT == 8 && sizeof(T) == 2), "row segments: the dense 16-bit 256 x 256 tile");
     typedef i32x4 frag_t;
     typedef TO Tx4 __attribute__((ext_vector_type(4)));
@@ -780,6 +781,27 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             }
         });
     };
+    auto glu_parts = [&](int em0, int en0, int epart) __attribute__((always_inline)) {
+        const int el = opaque_lane();
+        const int fr = el & 15;
+        const int nb = en0 + wc * OCW + 4 * (el >> 4);
+        static_for<8>([&](auto MI_) __attribute__((always_inline)) {
+            constexpr int mi = MI_;
+            const int mrow0 = em0 + wr * 128 + mi * 16;
+            if (mrow0 >= M) return;                            // wave-uniform
+            static_for<NT / 2>([&](auto NI_) __attribute__((always_inline)) {
+                constexpr int ni = NI_;
+                const int n = nb + ni * 16;
+                const f32x4 ag = acc_read<(mi * 8 + ni) * 4>();
+                const f32x4 au = acc_read<(mi * 8 + ni + NT / 2) * 4>();
+                if (mrow0 + fr < M && n < glu.ldp) {
+                    TO* to = C + ((int64_t)epart * M + mrow0 + fr) * ldc + n;
+                    *reinterpret_cast<f32x4*>(to) = ag;
+                    *reinterpret_cast<f32x4*>(to + glu.ldp) = au;
+                }
+            });
+        });
+    };
     auto epilogue = [&](int em0, int en0, int ecw, int epart) __attribute__((always_inline)) {
       const int64_t part0 = SPLIT ? (int64_t)epart * M : 0;      // (the whole M)
       const int M = seg_rows(em0);              // shadows the kernel's
@@ -1002,7 +1024,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         }
         fence();
         asm volatile("s_nop 15\ns_nop 15" ::: "memory");        // the last MFMAs retire before their tiles are read
-        if constexpr (GLU) glu_epilogue(em0, en0);
+        if constexpr (GLU && SPLIT) glu_parts(em0, en0, epart);
+        else if constexpr (GLU) glu_epilogue(em0, en0);
         else epilogue(em0, en0, ecw, epart);
 #if defined(FP_PROBE_REG_LOAD)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

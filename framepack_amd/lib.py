@@ -40,7 +40,8 @@ SIGNATURES = {
     "fp_gated_ff_workspace_bytes": [P, L, P, L, P, L, I, I, I],
     "fp_gated_ff_bf16": [P, L, P, L, P, L, P, P, P, L, P, P, L, I, I, I, I, P, L, P],
     "fp_gated_ff_f16": [P, L, P, L, P, L, P, P, P, L, P, P, L, I, I, I, I, P, L, P],
-    "fp_gated_ff_fp8": [P, L, P, P, L, P, P, L, P, P, P, P, L, I, I, I, I, P],
+    "fp_gated_ff_fp8_workspace_bytes": [I, I, I],
+    "fp_gated_ff_fp8": [P, L, P, P, L, P, P, L, P, P, P, P, L, I, I, I, I, P, L, P],
     "fp_gated_ff_backward_workspace_bytes": [P, L, P, L, P, L, I, I, I],
     "fp_gated_ff_backward_bf16": [P, L, P, L, P, L, P, L, P, L, P, L, P, P, P, I, I, I, I, P, L, P],
     "fp_gated_ff_backward_f16": [P, L, P, L, P, L, P, L, P, L, P, L, P, P, P, I, I, I, I, P, L, P],

@@ -933,9 +933,12 @@ def gated_ff_fp8(x_q: torch.Tensor, x_scale: torch.Tensor, wg_q: torch.Tensor, w
                                ("b_gate", bg), ("b_up", bu)])
     if M == 0:
         return h
-    _lib.check(_lib.load().fp_gated_ff_fp8(x2.data_ptr(), ldx, xs.data_ptr(), g2.data_ptr(), ldg, gs.data_ptr(), u2.data_ptr(),
-                                           ldu, us.data_ptr(), _ptr(bg), _ptr(bu), h2.data_ptr(), ldh, M, F, K, act,
-                                           _stream(x_q)), "fp_gated_ff_fp8")
+    lib = _lib.load()
+    n = lib.fp_gated_ff_fp8_workspace_bytes(M, F, K)
+    ws = x_q.new_empty((n,), dtype=torch.uint8) if n else None
+    _lib.check(lib.fp_gated_ff_fp8(x2.data_ptr(), ldx, xs.data_ptr(), g2.data_ptr(), ldg, gs.data_ptr(), u2.data_ptr(), ldu,
+                                   us.data_ptr(), _ptr(bg), _ptr(bu), h2.data_ptr(), ldh, M, F, K, act, _ptr(ws), n,
+                                   _stream(x_q)), "fp_gated_ff_fp8")
     return h
 
 

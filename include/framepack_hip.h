@@ -241,9 +241,10 @@ int fp_rmsnorm_residual_backward_f16(const void* dy, int64_t dy_row_stride, cons
 /* K13  h = act(g) * u,  g = x . w_gate^T + b_gate,  u = x . w_up^T + b_up;  act: 0 = SiLU, 1 = tanh-GELU.
  * x: [M, K], w_gate, w_up: [F, K] (nn.Linear layout), biases [F] (both or neither), h: [M, F].  gate, up (both or
  * neither, row stride ldp): receive g and u for the gradient.  No output may overlap an input.  workspace:
- * fp_gated_ff_workspace_bytes(...) bytes for these operands, 16-byte aligned, or NULL where that is 0: it is unless M > 48
+ * fp_gated_ff_workspace_bytes(...) bytes for these operands, 16-byte aligned, or NULL where that is 0.  It is not 0 where M > 48
  * and K % 64 != 0 or one of x, w_gate, w_up is not 16-byte aligned with a row stride of a multiple of 8 below 2^22 (such
- * operands are copied into rows that are; F, K <= 2^20 - 64 then). */
+ * operands are copied into rows that are; F, K <= 2^20 - 64 then), and where the output has few tiles and K is long (fp32
+ * parts of K).  M, F, K <= 2^30. */
 int64_t fp_gated_ff_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up,
                                     int64_t ldwu, int M, int F, int K);
 int fp_gated_ff_bf16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
@@ -255,10 +256,12 @@ int fp_gated_ff_f16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg
 
 /* K13 on e4m3 operands: g = x_scale[m] * wg_scale[n] * (x . w_gate^T) + b_gate and u alike; h and the biases bf16, the
  * scales fp32.  K % 128 == 0, F % 8 == 0, the matrices 16-byte aligned with row strides of multiples of 16 elements
- * (h: of 8), scales and biases 16-byte aligned. */
+ * (h: of 8), scales and biases 16-byte aligned; x's and the weights' row strides below 2^22.  workspace:
+ * fp_gated_ff_fp8_workspace_bytes(M, F, K) bytes, 16-byte aligned, or NULL where that is 0. */
+int64_t fp_gated_ff_fp8_workspace_bytes(int M, int F, int K);
 int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, const void* w_gate, int64_t ldwg, const void* wg_scale,
                     const void* w_up, int64_t ldwu, const void* wu_scale, const void* b_gate, const void* b_up, void* h,
-                    int64_t ldh, int M, int F, int K, int act, void* stream);
+                    int64_t ldh, int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Gradient of K13 from dh and the kept g and u:  dg = dh u act'(g), du = dh act(g) (rounded to the type), then
  *   dx = dg . w_gate + du . w_up [M, K];  dw [2 F, K] = dg^T . x over du^T . x;  db [2 F] (or NULL) = column sums of dg, du.

@@ -148,10 +148,16 @@ def test_the_library_refuses_without_launching():
     refused("fp_gated_ff_bf16", *ok)
     refused("fp_gated_ff_f16", *[p + 8 if j == 17 else 1 << 30 if j == 18 else t for j, t in enumerate(ok)])
     refused("fp_gated_ff_f16", *[p if j == 17 else (49 + 2 * F) * K * 2 - 1 if j == 18 else t for j, t in enumerate(ok)])
-    ok = [p, K, p, p, K, p, p, K, p, p, p, p, F, n, F, K, 0, None]
+    ok = [p, K, p, p, K, p, p, K, p, p, p, p, F, n, F, K, 0, None, 0, None]
     for i, v in ((0, None), (2, None), (5, None), (8, None), (1, K + 8), (4, K + 8), (7, K + 8), (0, p + 8), (3, p + 8), (6, p + 8),
                  (11, p + 8), (12, F + 4), (14, 12), (15, 64), (5, p + 4), (9, p + 2), (9, None), (16, -1)):
         refused("fp_gated_ff_fp8", *[v if j == i else t for j, t in enumerate(ok)])
+    assert L.fp_gated_ff_fp8_workspace_bytes(4, 16, 128) == 0 and L.fp_gated_ff_fp8_workspace_bytes(4, 14336, 4096) == 0
+    need = L.fp_gated_ff_fp8_workspace_bytes(4, 16, 8192)                          # few columns, a long K: parts of it
+    assert need > 0 and need % (4 * 2 * 16 * 4) == 0
+    ok[1] = ok[4] = ok[7] = ok[15] = 8192
+    for i, v in ((17, None), (17, p + 8), (18, need - 1)):
+        refused("fp_gated_ff_fp8", *[v if j == i else p if j == 17 else need if j == 18 else t for j, t in enumerate(ok)])
     ok = [p, F, p, K, p, K, p, K, p, F, p, F, p, p, p, n, F, K, 0, p, 1 << 30, None]
     for i, v in ((0, None), (2, None), (4, None), (8, None), (12, None), (13, None), (5, K - 1), (7, K - 1), (12, p + 8), (13, p + 2),
                  (14, p + 1), (15, 0), (16, 0), (17, 0), (15, 1 << 20), (18, 3), (19, None), (19, p + 8), (20, 16)):
