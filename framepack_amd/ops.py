@@ -22,6 +22,8 @@ ATTN_EVENTS: Optional[list] = None
 
 # (the handle alone: building torch's Stream object around it takes 2 us, as long as a small kernel)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# (a tensor on a GPU means that torch has its context: no check for that, and a third of the time)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -43,7 +45,7 @@ def _dev(*ts: Optional[torch.Tensor]) -> None:
         if not t.is_cuda:
             raise RuntimeError("framepack_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
         if cur is None:
-            cur = torch.cuda.current_device()
+            cur = _current_device()
         if d != cur:
             raise RuntimeError(f"tensor on cuda:{d} but the current device is cuda:{cur}: "
                                f"wrap the call in `with torch.cuda.device({d}):`")
@@ -723,12 +725,12 @@ def _vec(t: torch.Tensor, what: str, dtype, n: int) -> torch.Tensor:
     return t if t.is_contiguous() else t.reshape(-1).contiguous()
 
 
-def _out(t: Optional[torch.Tensor], what: str, dtype, rows: int, cols: int, like: torch.Tensor):
-    """An output matrix (as returned, 2-d view, row stride): allocated if None, else of this type and size with rows that do
-    not overlap each other."""
+def _out(t: Optional[torch.Tensor], what: str, dtype, rows: int, cols: int, like: torch.Tensor, same: bool = False):
+    """An output matrix (as returned, 2-d view, row stride): allocated if None (on like's device; `same`: like is a
+    contiguous [rows, cols] itself), else of this type and size with rows that do not overlap each other."""
     if t is None:
-        # (empty_like of a contiguous tensor of this very shape is the quickest to come by)
-        if like.dtype is dtype and like.shape == (rows, cols) and like.is_contiguous():
+        # (empty_like of a contiguous tensor of this very shape and type is the quickest to come by)
+        if same and like.dtype is dtype:
             t = torch.empty_like(like)
         else:
             t = like.new_empty((rows, cols), dtype=dtype)
@@ -791,7 +793,7 @@ def _rmsnorm_args(x, weight, resid, resid_out, dtypes, eps):
             raise ValueError("resid_out without resid")
         return x2, rows, cols, xs, w, None, 0, x, None, 0
     r2, _, _, rs = _mat(resid, "resid", (x.dtype,), rows, cols)
-    h, h2, hs = _out(resid_out, "resid_out", x.dtype, rows, cols, x)
+    h, h2, hs = _out(resid_out, "resid_out", x.dtype, rows, cols, x, x2 is x and x.is_contiguous())
     return x2, rows, cols, xs, w, r2, rs, h, h2, hs
 
 
@@ -804,7 +806,7 @@ def rmsnorm_residual(x: torch.Tensor, weight: torch.Tensor, resid: Optional[torc
     x, resid [rows, cols] (row-strided ok, any cols), weight [cols], one type: bf16 or f16.  The norm is taken of the
     32-bit sum; h is that sum rounded to the type.  out and resid_out may each be x or resid itself."""
     x2, rows, cols, xs, w, r2, rs, h, h2, hs = _rmsnorm_args(x, weight, resid, resid_out, (BF16, F16), eps)
-    y, y2, ys = _out(out, "out", x.dtype, rows, cols, x)
+    y, y2, ys = _out(out, "out", x.dtype, rows, cols, x, x2 is x and x.is_contiguous())
     if out is not None or resid_out is not None:
         _dev(x, out)
         _apart(_given(("out", out, y2), ("resid_out", resid_out, h2)), [("x", x2), ("resid", r2), ("weight", w)], _NORM_SAME)
@@ -858,7 +860,7 @@ def rmsnorm_residual_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.T
     d2, ds = None, 0
     if dh is not None:
         d2, _, _, ds = _mat(dh, "dh", (h.dtype,), rows, cols)
-    got, dx2, dxs = _out(dx, "dx", h.dtype, rows, cols, h)
+    got, dx2, dxs = _out(dx, "dx", h.dtype, rows, cols, h, h2 is h and h.is_contiguous())
     if dx is not None:
         _apart([("dx", dx2)], [("dy", y2), ("h", h2), ("dh", d2), ("weight", w)], {("dx", "dh")})
     if rows == 0:
