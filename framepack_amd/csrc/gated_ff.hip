@@ -352,11 +352,11 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh,
         colsum[(int64_t)blockIdx.y * (2 * Fp) + w * Fp + f0 + l] = (cs[w][0][l] + cs[w][1][l]) + (cs[w][2][l] + cs[w][3][l]);
     }
 }
-// out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns
+// out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns, from chunk i0 on
 template <typename T>
 __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, int splits, T* __restrict__ out, int64_t M, int N,
-                                                        int Np) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                                                        int Np, int64_t i0) {
+    const int64_t i = i0 + (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int per = Np / 4;
     if (i >= M * per) return;
     const int64_t m = i / per;
@@ -373,7 +373,6 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict_
             if (n + j < N) to[j] = (T)s[j];
     }
 }
-
 
 // How a product [M, N] over K (a multiple of 64) is cut: whole (0 parts: straight to 16 bits) where its 256 x 256 tiles fill
 // half the chip, else 256 x 128 tiles in parts of K of at least 8 tiles, as many as there are CUs.  N % 8 != 0: always
@@ -402,6 +401,7 @@ int64_t cut_bytes(int64_t M, int N, int K) { return (int64_t)cut(M, N, K).splits
 // bf16 45 / 70 at 1 row, 56 / 69 at 32, 64 / 71 at 48, 70 / 73 at 64; e4m3 21 / 30 at 1, 32 / 34 at 48, 37 / 35 at 64.
 constexpr int FEW = 48;
 constexpr int64_t FAR = int64_t(1) << 22;   // gemm_w4.h: 32-bit offsets within a tile
+constexpr int MOST_F = 1 << 27;             // glu_few_kernel's lanes, 16 a column, have to stay below 2^32
 constexpr int LIMIT = (1 << 20) - 64;      // M, F, K of the gradient: row strides of 2 F and 4 K stay below gemm_w4.h's limit of 2^22
 
 bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
@@ -450,9 +450,12 @@ int product(GradProduct p, T* out, int N, float* parts, hipStream_t st) {
     p.out = c.splits ? (void*)parts : (void*)out;
     if (int rc = fpi_grad_product(__is_same(T, bf16) ? FF_BF16 : FF_F16, p, st)) return rc;
     if (c.splits == 0) return 0;
-    const int64_t lanes = (int64_t)p.M * (p.N / 4);
-    add_parts_kernel<T><<<dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, st>>>(parts, c.splits, out, p.M, N, p.N);
-    FP_CHECK_LAUNCH();
+    const int64_t lanes = (int64_t)p.M * (p.N / 4), most = int64_t(1) << 31;         // (a launch's lanes have to stay below 2^32)
+    for (int64_t i = 0; i < lanes; i += most) {
+        add_parts_kernel<T><<<dim3((unsigned)((std::min(most, lanes - i) + 255) / 256)), dim3(256), 0, st>>>(parts, c.splits, out, p.M, N,
+                                                                                                            p.N, i);
+        FP_CHECK_LAUNCH();
+    }
     return 0;
 }
 
@@ -502,7 +505,7 @@ int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64
               const float* us, const void* bg, const void* bu, void* h, int64_t ldh, void* gate, void* up, int64_t ldp, int M, int F,
               int K, int act, void* ws, int64_t ws_bytes, void* stream) {
     FP_REQUIRE(x && wg && wu && h && M >= 0 && F > 0 && K > 0 && (act == 0 || act == 1) && !bg == !bu && !gate == !up);
-    FP_REQUIRE(M <= 1 << 30 && F <= 1 << 30 && K <= 1 << 30);
+    FP_REQUIRE(M <= 1 << 30 && F <= MOST_F && K <= 1 << 30);
     FP_REQUIRE(ldx >= 0 && ldwg >= K && ldwu >= K && ldh >= F && (!gate || ldp >= F));
     FP_REQUIRE(sizeof(TI) == 1 || (aligned2(x) && aligned2(wg) && aligned2(wu) && aligned2(h) && aligned2(bg) && aligned2(bu) &&
                                    aligned2(gate) && aligned2(up)));
@@ -540,7 +543,7 @@ int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64
         int Kp = K;
         if constexpr (sizeof(TI) == 2) {
             if (!p.x_fits || !p.g_fits || !p.u_fits) {
-                FP_REQUIRE(K <= LIMIT && F <= LIMIT);
+                FP_REQUIRE(K <= LIMIT);
                 Kp = (int)up64(K);
                 TI *xp = (TI*)ws, *gp = xp + (p.x_fits ? 0 : (int64_t)M * Kp), *upk = gp + (p.g_fits ? 0 : (int64_t)F * Kp);
                 Copies c{{x, wg, wu}, {xp, gp, upk}, {ldx, ldwg, ldwu}, {Kp, Kp, Kp}};
@@ -616,12 +619,12 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
 
 extern "C" int64_t fp_gated_ff_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,
                                                int M, int F, int K) {
-    if (M <= 0 || F <= 0 || K <= 0 || M > 1 << 30 || F > 1 << 30 || K > 1 << 30) return 0;
+    if (M <= 0 || F <= 0 || K <= 0 || M > 1 << 30 || F > MOST_F || K > 1 << 30) return 0;
     return plan(2, x, ldx, w_gate, ldwg, w_up, ldwu, M, F, K).bytes;
 }
 
 extern "C" int64_t fp_gated_ff_fp8_workspace_bytes(int M, int F, int K) {
-    if (M <= 0 || F <= 0 || K <= 0 || M > 1 << 30 || F > 1 << 30 || K > 1 << 30) return 0;
+    if (M <= 0 || F <= 0 || K <= 0 || M > 1 << 30 || F > MOST_F || K > 1 << 30) return 0;
     return plan(1, nullptr, 0, nullptr, 0, nullptr, 0, M, F, K).bytes;
 }
 

@@ -399,6 +399,7 @@ __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(const float* __res
 
 bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
 
+constexpr int MOST_COLS = 1 << 28;   // 32-bit columns, and a launch's lanes below 2^32 (rmsnorm_dweight_kernel: 8 a column)
 constexpr int REG_COLS = 65536;      // the longest row that is held in registers (1024 lanes, 8 chunks each)
 // Lanes per row: a wave where half of a workgroup's would have nothing to do and the rows alone fill the chip, else a workgroup
 // (us, wave / workgroup: 20000 x 1024 29 / 34; 19385 x 4096 118 / 114; 1 x 4096 4.4 / 2.6), of 1024 lanes where 256 would hold
@@ -445,7 +446,7 @@ int norm_rows(const T* x, int64_t x_rs, const T* resid, int64_t r_rs, const T* w
 template <typename T, bool Q8>
 int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, const void* w, void* y, int64_t y_rs,
                 void* q_scale, void* h, int64_t h_rs, int rows, int cols, float eps, void* stream) {
-    FP_REQUIRE(x && w && y && rows >= 0 && cols > 0 && x_rs >= 0 && y_rs >= cols);
+    FP_REQUIRE(x && w && y && rows >= 0 && cols > 0 && cols <= MOST_COLS && x_rs >= 0 && y_rs >= cols);
     FP_REQUIRE(!resid == !h && (!resid || (r_rs >= 0 && h_rs >= cols)) && eps >= 0.f);
     FP_REQUIRE(aligned2(x) && aligned2(resid) && aligned2(w) && (Q8 || aligned2(y)) && aligned2(h));
     FP_REQUIRE(!Q8 || (q_scale && ((uintptr_t)q_scale & 3) == 0));
@@ -466,7 +467,7 @@ int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, co
 template <typename T>
 int grad_launch(const void* dy, int64_t dy_rs, const void* h, int64_t h_rs, const void* dh, int64_t dh_rs, const void* w,
                 void* dx, int64_t dx_rs, void* dw, int rows, int cols, float eps, void* ws, int64_t ws_bytes, void* stream) {
-    FP_REQUIRE(cols <= GRAD_COLS || rows <= 1 << 21);           // (a workgroup per row there)
+    FP_REQUIRE(cols <= MOST_COLS && (cols <= GRAD_COLS || rows <= 1 << 21));           // (a workgroup per row there)
     FP_REQUIRE(dy && h && w && dx && dw && rows > 0 && cols > 0 && dy_rs >= 0 && h_rs >= 0 && dx_rs >= cols && eps >= 0.f);
     FP_REQUIRE(!dh || dh_rs >= 0);
     FP_REQUIRE(aligned2(dy) && aligned2(h) && aligned2(dh) && aligned2(w) && aligned2(dx) && aligned2(dw));
@@ -524,7 +525,7 @@ extern "C" int fp_rmsnorm_residual_fp8(const void* x, int64_t x_row_stride, cons
 }
 
 extern "C" int64_t fp_rmsnorm_residual_backward_workspace_bytes(int rows, int cols) {
-    if (rows <= 0 || cols <= 0) return 0;
+    if (rows <= 0 || cols <= 0 || cols > MOST_COLS) return 0;
     return ((int64_t)grad_parts(rows, cols) * (((int64_t)cols + 7) & ~7) + (cols > GRAD_COLS ? (int64_t)rows : 0)) * 4;
 }
 

@@ -898,8 +898,8 @@ def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: 
              b_up: Optional[torch.Tensor] = None, act: int = ACT_SILU, out: Optional[torch.Tensor] = None, keep: bool = False):
     """K13: h = act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up) in one kernel, act = ACT_SILU or ACT_GELU; returns h
     [M, inner], with keep (h, gate, up): the two projections before the activation, as `gated_ff_backward` takes them.
-    x [M, K], w_gate, w_up [inner, K] (nn.Linear layout; row-strided ok, slices of one fused weight too), any sizes; one
-    type, bf16 or f16.  The block's second linear is `gemm`, with the residual in its epilogue (EPI_RESIDUAL)."""
+    x [M, K], w_gate, w_up [inner, K] (nn.Linear layout; row-strided ok, slices of one fused weight too), any sizes (K
+    below 2^20 for more than 48 rows); one type, bf16 or f16.  The block's second linear is `gemm`, with the residual in its epilogue (EPI_RESIDUAL)."""
     _dev(x, w_gate, w_up, b_gate, b_up, out)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, (BF16, F16), x.dtype)
     h, h2, ldh = _out(out, "out", x.dtype, M, F, x)
@@ -923,8 +923,8 @@ def gated_ff_fp8(x_q: torch.Tensor, x_scale: torch.Tensor, wg_q: torch.Tensor, w
                  act: int = ACT_SILU, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """K13 on e4m3 operands: bf16 h = act(g) * u with g = x_scale[m] * wg_scale[n] * (x_q @ wg_q.T) + b_gate and u alike.
     x_q [M, K] with x_scale [M] as `rmsnorm_residual_fp8` and `quantize_rows_fp8` return them, weights [inner, K] with
-    scales [inner] as `quantize_weight_fp8` prepares them; biases bf16.  K a multiple of 128, inner of 8, matrices 16-byte
-    aligned with row strides of multiples of 16, as `gemm_fp8`."""
+    scales [inner] as `quantize_weight_fp8` prepares them; biases bf16.  K a multiple of 128, inner of 8, all 16-byte
+    aligned, matrices with row strides of multiples of 16, as `gemm_fp8`."""
     _dev(x_q, x_scale, wg_q, wg_scale, wu_q, wu_scale, b_gate, b_up, out)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x_q, wg_q, wu_q, b_gate, b_up, act, (FP8,), BF16)
     xs, gs, us = (_vec(t, n, torch.float32, k) for t, n, k in ((x_scale, "x_scale", M), (wg_scale, "wg_scale", F),

@@ -209,7 +209,8 @@ int fp_gemm_fp8_bf16(const void* a, int64_t lda, const void* a_scale, const void
 
 /* K12  h = resid + x;  y = h / sqrt(mean(h^2) + eps) * weight,  x, resid, y, h: [rows, cols], weight: [cols].
  * The norm is taken of the 32-bit sum, h receives it rounded.  resid and h may both be NULL: h = x, nothing but y is
- * written.  y and h may each be the very matrix x or resid (same pointer and stride).  cols is any positive number. */
+ * written.  y and h may each be the very matrix x or resid (same pointer and stride).  0 < cols <= 2^28.
+ * The squares are summed in fp32: entries past 2^63 overflow the row's norm, entries below 2^-74 count as 0. */
 int fp_rmsnorm_residual_bf16(const void* x, int64_t x_row_stride, const void* resid, int64_t resid_row_stride,
                              const void* weight, void* y, int64_t y_row_stride, void* h, int64_t h_row_stride, int rows,
                              int cols, float eps, void* stream);
@@ -243,8 +244,8 @@ int fp_rmsnorm_residual_backward_f16(const void* dy, int64_t dy_row_stride, cons
  * neither, row stride ldp): receive g and u for the gradient.  No output may overlap an input.  workspace:
  * fp_gated_ff_workspace_bytes(...) bytes for these operands, 16-byte aligned, or NULL where that is 0.  It is not 0 where M > 48
  * and K % 64 != 0 or one of x, w_gate, w_up is not 16-byte aligned with a row stride of a multiple of 8 below 2^22 (such
- * operands are copied into rows that are; F, K <= 2^20 - 64 then), and where the output has few tiles and K is long (fp32
- * parts of K).  M, F, K <= 2^30. */
+ * operands are copied into rows that are; K <= 2^20 - 64 then), and where the output has few tiles and K is long (fp32
+ * parts of K).  M, K <= 2^30, F <= 2^27. */
 int64_t fp_gated_ff_workspace_bytes(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up,
                                     int64_t ldwu, int M, int F, int K);
 int fp_gated_ff_bf16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg, const void* w_up, int64_t ldwu,

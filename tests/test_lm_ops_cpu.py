@@ -164,6 +164,20 @@ def test_the_library_refuses_without_launching():
         refused("fp_gated_ff_backward_f16", *[v if j == i else t for j, t in enumerate(ok)])
 
 
+def test_the_library_refuses_sizes_whose_launches_would_not_fit():
+    L = fplib.load()
+    p, big = 1 << 20, 1 << 28
+    ok = [p, big, None, 0, p, p, big, None, 0, 1, big + 1, 1e-6, None]
+    ok[1] = ok[6] = big + 8
+    assert L.fp_rmsnorm_residual_bf16(*ok) == 1 and L.fp_rmsnorm_residual_f16(*ok) == 1
+    assert L.fp_rmsnorm_residual_backward_workspace_bytes(1, big + 1) == 0
+    ld = big + 8
+    assert L.fp_rmsnorm_residual_backward_bf16(p, ld, p, ld, None, 0, p, p, ld, p, 1, big + 1, 1e-6, p, 1 << 60, None) == 1
+    F = (1 << 27) + 1
+    assert L.fp_gated_ff_workspace_bytes(p, 8, p, 8, p, 8, 1, F, 8) == 0
+    assert L.fp_gated_ff_bf16(p, 8, p, 8, p, 8, None, None, p, F, None, None, 0, 1, F, 8, 0, None, 0, None) == 1
+
+
 def test_fragment_reads_of_the_gated_blocks_products_all_feed_an_mfma(tmp_path):
     """The 16-bit instances of the 4-wave kernel read their MFMA fragments with inline asm - K13's gradient with pairs of
     transposing reads - whose results the compiler takes for written at once.  Compile K13's products to assembly with the

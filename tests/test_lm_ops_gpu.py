@@ -573,3 +573,88 @@ def test_norm_of_more_rows_than_a_launch_takes():
     q, s, _ = ops.rmsnorm_residual_fp8(x, w, x)
     within(s, y64.abs().amax(1) / 448, y64.abs().amax(1) / 448 * 16 * E32)
     within(q.double() * s.double()[:, None], y64, y64.abs() * 2.0 ** -4 * 1.001 + s.double()[:, None] * 2.0 ** -10)
+
+
+def test_norm_without_eps_and_of_sums_past_the_types_range():
+    x, r = randn(5, 520, seed=1, dtype=HF), randn(5, 520, seed=2, dtype=HF)
+    w = randn(520, seed=3, dtype=HF)
+    h64, y64 = norm64(x, r, w, eps=0.0)
+    y, _ = ops.rmsnorm_residual(x, w, r, eps=0.0)
+    within(y, y64, norm_tol(y64, HF, 520))
+    x[2], r[2] = x[2] * 0 + 60000, r[2] * 0 + 60000          # h is inf in 16 bits; the norm is taken of the 32-bit sum
+    h64, y64 = norm64(x, r, w)
+    y, h = ops.rmsnorm_residual(x, w, r)
+    assert torch.isinf(h[2]).all() and torch.isfinite(h[[0, 1, 3, 4]]).all()
+    within(y, y64, norm_tol(y64, HF, 520))
+    z = torch.zeros(3, 520, dtype=HF, device=DEV)            # 0 / 0: NaN, as the formula has it, and only there
+    z[1] = x[0]
+    y, _ = ops.rmsnorm_residual(z, w, eps=0.0)
+    assert torch.isnan(y[0]).all() and torch.isnan(y[2]).all() and torch.isfinite(y[1]).all()
+
+
+@pytest.mark.parametrize("M,F,K", [(70, 136, 192), (64, 130, 100)])
+def test_gated_ff_gradient_of_a_fused_weight_and_of_repeated_rows(M, F, K):
+    dh, w = randn(M, F, seed=1, dtype=BF), randn(2 * F, K, seed=2, scale=K ** -0.5, dtype=BF)
+    g, u = randn(M, F, seed=3, dtype=BF), randn(M, F, seed=4, dtype=BF)
+    x = randn(1, K, seed=5, dtype=BF).expand(M, K)           # one row for all: the gradient of each copy
+    gu = torch.cat([g, u], 1)                                # the two projections side by side, as one product leaves them
+    got = ops.gated_ff_backward(dh, x, w[:F], w[F:], gu[:, :F], gu[:, F:], bias=True)
+    check_ff_grad(got, dh, x, w[:F], w[F:], g, u, ops.ACT_SILU, BF)
+    # the same matrix for two arguments, and the same row of it in every place
+    got = ops.gated_ff_backward(g, x, w[:F], w[:F], g, g)
+    check_ff_grad(got, g, x, w[:F], w[:F], g, g, ops.ACT_SILU, BF)
+
+
+@pytest.mark.parametrize("M", [3, 130])
+def test_calls_that_overlap_on_two_streams(M):
+    D, F = 1024, 520                                         # (forward in parts of K, both products of the gradient too)
+    sets = []
+    for k in range(2):
+        x, r, w, wg, wu, _ = layer_inputs(M, D, F)
+        sets.append(((x * (k + 1)).contiguous(), r, w, wg, wu, randn(M, F, seed=20 + k, dtype=BF)))
+
+    def step(x, r, w, wg, wu, dh):
+        n, h = ops.rmsnorm_residual(x, w, r)
+        a, g, u = ops.gated_ff(n, wg, wu, keep=True)
+        dn, dwg, dwu, dbg, dbu = ops.gated_ff_backward(dh, n, wg, wu, g, u, bias=True)
+        return [n, h, a, g, u, dn, dwg, dwu, dbg, dbu, *ops.rmsnorm_residual_backward(dn, h, w, dh=h)]
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(8):                                       # in turn, so that both streams' calls are in flight together
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(step(*sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for o in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(o, want[k]))
+
+
+def test_leading_dimensions_of_one_and_batches():
+    x, r = randn(2, 3, 64, seed=1, dtype=BF), randn(2, 3, 64, seed=2, dtype=BF)
+    w, wg = randn(64, seed=3, dtype=BF), randn(24, 64, seed=4, scale=0.125, dtype=BF)
+    y, h = ops.rmsnorm_residual(x, w, r)                     # [.., rows, cols] in, [rows, cols] out, as the other norms
+    y2, h2 = ops.rmsnorm_residual(x.reshape(6, 64), w, r.reshape(6, 64))
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+    assert torch.equal(ops.gated_ff(x, wg, wg), ops.gated_ff(x.reshape(6, 64), wg, wg))
+    a, g, u = ops.gated_ff(x[:1], wg, wg, keep=True)
+    got = ops.gated_ff_backward(a[None], x[:1], wg, wg, g, u)
+    assert all(torch.equal(p, q) for p, q in zip(got[:3], ops.gated_ff_backward(a, x[0], wg, wg, g, u)[:3]))
+
+
+def test_the_widest_blocks():
+    F = (1 << 22) + 24                                       # row strides of the output past 2^22
+    x, wg = randn(50, 8, seed=1, dtype=BF), randn(F, 8, seed=2, dtype=BF)
+    for M in (3, 50):
+        h64, g, u, eg, eu = ff64(x[:M], wg, wg, None, None, ops.ACT_SILU)
+        within(ops.gated_ff(x[:M], wg, wg), h64, ff_tol(h64, g, u, eg, eu, ops.ACT_SILU, BF))
+    cols = (1 << 24) + 9                                     # 32-bit column offsets in the long rows' kernels
+    x, w = randn(2, cols, seed=3, dtype=BF), randn(cols, seed=4, dtype=BF)
+    h64, y64 = norm64(x, x, w)
+    y, h = ops.rmsnorm_residual(x, w, x)
+    within(h, h64, h64.abs() * (u_of(BF) + 2 * E32))
+    # each lane adds 65537 squares up, then the lanes' sums: half of (65537 + 8) 2^-24 relative, by the root
+    within(y, y64, y64.abs() * (u_of(BF) + (65545 / 2 + 8) * E32))
