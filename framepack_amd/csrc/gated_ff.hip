@@ -227,8 +227,7 @@ __global__ __launch_bounds__(256) void glu_finish_kernel(GluCall q, const float*
 constexpr int64_t up64(int64_t v) { return (v + 63) & ~(int64_t)63; }
 constexpr int64_t up8(int64_t v) { return (v + 7) & ~(int64_t)7; }
 
-// Up to three matrices of the same width into zero-padded rows of their own stride; behind them (if wanted) the biases'
-// gradients: db = sum of the row tiles' column sums, 64 columns a block.
+// Up to three matrices of the same width into zero-padded rows of their own stride.
 struct Copies {
     const void* src[3];
     void* dst[3];
@@ -236,28 +235,11 @@ struct Copies {
     int rows[3], rows_p[3];         // rows of the source, rows written (0: not this one)
     int cols, cols_p;               // columns of the source, columns written (a multiple of 8)
     int64_t chunks;                 // of all of them: 8 columns each
-    unsigned blocks;                // that copy; the others add up column sums
-    const float* sums;              // [tiles][2 Fp]
-    int tiles, F, Fp;
-    void* db;                       // [2 F]
 };
-template <typename T>
-__global__ __launch_bounds__(256) void copy_rows_kernel(Copies q) {
-    if (blockIdx.x >= q.blocks) {
-        __shared__ float red[4][64];
-        const int b = blockIdx.x - q.blocks, per = (q.F + 63) / 64, half = b / per, l = threadIdx.x & 63, c = (b - half * per) * 64 + l,
-                  w = threadIdx.x >> 6;
-        float s = 0.f;
-        if (c < q.F)
-            for (int i = w; i < q.tiles; i += 4) s += q.sums[(int64_t)i * (2 * q.Fp) + half * q.Fp + c];
-        red[w][l] = s;
-        __syncthreads();
-        if (w == 0 && c < q.F) reinterpret_cast<T*>(q.db)[half * q.F + c] = (T)((red[0][l] + red[1][l]) + (red[2][l] + red[3][l]));
-        return;
-    }
+template <typename T> __device__ __forceinline__ void copy_rows_of(const Copies& q, int64_t block, int64_t blocks) {
     const int per = q.cols_p / 8;
     const int64_t n0 = (int64_t)q.rows_p[0] * per, n1 = n0 + (int64_t)q.rows_p[1] * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < q.chunks; i += (int64_t)q.blocks * 256) {
+    for (int64_t i = block * 256 + threadIdx.x; i < q.chunks; i += blocks * 256) {
         const int k = i < n0 ? 0 : i < n1 ? 1 : 2;
         const int64_t at = i - (k == 0 ? 0 : k == 1 ? n0 : n1), r = at / per;
         const int c = (int)(at - r * per) * 8;
@@ -268,6 +250,39 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(Copies q) {
         }
         *reinterpret_cast<typename vec8<T>::type*>(reinterpret_cast<T*>(q.dst[k]) + r * q.ld_dst[k] + c) = v;
     }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void copy_rows_kernel(Copies q) {
+    copy_rows_of<T>(q, blockIdx.x, gridDim.x);
+}
+constexpr int64_t COPY_BLOCKS = 2048;       // at most
+void count(Copies& c, int cols, int cols_p) {
+    c.cols = cols;
+    c.cols_p = cols_p;
+    c.chunks = ((int64_t)c.rows_p[0] + c.rows_p[1] + c.rows_p[2]) * (cols_p / 8);
+}
+
+// The biases' gradients: db [2 F] = sum of the row tiles' column sums [tiles][2 Fp], 64 columns a block.
+struct ColumnSums {
+    const float* sums;
+    int tiles, F, Fp;
+    void* db;
+    __host__ unsigned blocks() const { return sums ? 2 * (unsigned)((F + 63) / 64) : 0; }
+};
+template <typename T> __device__ __forceinline__ void column_sums_of(const ColumnSums& q, int b) {
+    __shared__ float red[4][64];
+    const int per = (q.F + 63) / 64, half = b / per, l = threadIdx.x & 63, c = (b - half * per) * 64 + l, w = threadIdx.x >> 6;
+    float s = 0.f;
+    if (c < q.F)
+        for (int i = w; i < q.tiles; i += 4) s += q.sums[(int64_t)i * (2 * q.Fp) + half * q.Fp + c];
+    red[w][l] = s;
+    __syncthreads();
+    if (w == 0 && c < q.F) reinterpret_cast<T*>(q.db)[half * q.F + c] = (T)((red[0][l] + red[1][l]) + (red[2][l] + red[3][l]));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void column_sums_kernel(ColumnSums q) {
+    column_sums_of<T>(q, blockIdx.x);
 }
 
 // A 64 x 64 tile in LDS, written by rows and read by columns: 16-byte chunks, the chunk index XORed with row / 8 so that the
@@ -286,24 +301,38 @@ __device__ __forceinline__ typename vec8<T>::type tile_get_t(const T* t, int col
 
 // dg | du as rows [M, 2 Fp] in K tiles of 64 - `whole` tiles of dg, as many of du, then the last of dg and of du if there is one
 // more, zeros behind column F - and as columns [2 F, Mp], zeros behind row M; colsum: the tile's column sums [row tile][2 Fp]
-// (or null).  Grid (Fp / 64, Mp / 64).  One read of dh, g, u; two writes of dg and du.
+// (or null).  Grid (Fp / 64, Mp / 64 + rows of blocks for the copies).  One read of dh, g, u; two writes of dg and du.
 template <typename T>
 __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh, int64_t ldh, const T* __restrict__ gate, int64_t ldg,
                                                        const T* __restrict__ up, int64_t ldu, T* __restrict__ dgu, T* __restrict__ dgut,
-                                                       float* __restrict__ colsum, int M, int F, int Fp, int Mp, int whole, int act) {
+                                                       float* __restrict__ colsum, int M, int F, int Fp, int Mp, int whole, int act,
+                                                       Copies copies) {
     typedef typename vec8<T>::type V;
     __shared__ __attribute__((aligned(16))) T tg[64 * 64], tu[64 * 64];
     __shared__ float cs[2][4][64];
+    const int row_tiles = Mp / 64;
+    if ((int)blockIdx.y >= row_tiles) {
+        copy_rows_of<T>(copies, (int64_t)(blockIdx.y - row_tiles) * gridDim.x + blockIdx.x, (int64_t)(gridDim.y - row_tiles) * gridDim.x);
+        return;
+    }
     const int64_t m0 = (int64_t)blockIdx.y * 64;
     const int f0 = blockIdx.x * 64, ch = threadIdx.x & 7, c = f0 + ch * 8;
     float sg[8] = {}, su[8] = {};
+    V dv[2], gv[2], uv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {                           // all loads first
+        const int64_t m = min(m0 + (threadIdx.x >> 3) + 32 * i, (int64_t)M - 1);
+        dv[i] = load8(dh + m * ldh, c, F);
+        gv[i] = load8(gate + m * ldg, c, F);
+        uv[i] = load8(up + m * ldu, c, F);
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r = (threadIdx.x >> 3) + 32 * i;
         const int64_t m = m0 + r;
         V og = {}, ou = {};
         if (m < M) {
-            V d = load8(dh + m * ldh, c, F), g = load8(gate + m * ldg, c, F), u = load8(up + m * ldu, c, F);
+            V &d = dv[i], &g = gv[i], &u = uv[i];
             fit(d, c, F);
             fit(g, c, F);
             fit(u, c, F);
@@ -352,10 +381,15 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh,
         colsum[(int64_t)blockIdx.y * (2 * Fp) + w * Fp + f0 + l] = (cs[w][0][l] + cs[w][1][l]) + (cs[w][2][l] + cs[w][3][l]);
     }
 }
-// out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns, from chunk i0 on
+// out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns, from chunk i0 on.  The
+// last cs.blocks() blocks add up column sums instead.
 template <typename T>
 __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, int splits, T* __restrict__ out, int64_t M, int N,
-                                                        int Np, int64_t i0) {
+                                                        int Np, int64_t i0, ColumnSums cs, unsigned cs_blocks) {
+    if (blockIdx.x >= gridDim.x - cs_blocks) {
+        column_sums_of<T>(cs, (int)(blockIdx.x - (gridDim.x - cs_blocks)));
+        return;
+    }
     const int64_t i = i0 + (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int per = Np / 4;
     if (i >= M * per) return;
@@ -439,9 +473,10 @@ GradSpace grad_space(const void* x, int64_t ldx, const void* wg, int64_t ldwg, c
     return g;
 }
 
-// out [M, N] = the product, through fp32 parts where it is cut
+// out [M, N] = the product, through fp32 parts where it is cut.  sums: taken along by the launch that adds the parts up, if
+// there is one (`sums.sums` is null from then on).
 template <typename T>
-int product(GradProduct p, T* out, int N, float* parts, hipStream_t st) {
+int product(GradProduct p, T* out, int N, float* parts, ColumnSums& sums, hipStream_t st) {
     const Cut c = cut(p.M, N, p.K);
     p.narrow = c.narrow;
     p.splits = c.splits;
@@ -452,9 +487,11 @@ int product(GradProduct p, T* out, int N, float* parts, hipStream_t st) {
     if (c.splits == 0) return 0;
     const int64_t lanes = (int64_t)p.M * (p.N / 4), most = int64_t(1) << 31;         // (a launch's lanes have to stay below 2^32)
     for (int64_t i = 0; i < lanes; i += most) {
-        add_parts_kernel<T><<<dim3((unsigned)((std::min(most, lanes - i) + 255) / 256)), dim3(256), 0, st>>>(parts, c.splits, out, p.M, N,
-                                                                                                            p.N, i);
+        const unsigned b = sums.blocks();
+        add_parts_kernel<T><<<dim3((unsigned)((std::min(most, lanes - i) + 255) / 256) + b), dim3(256), 0, st>>>(parts, c.splits, out, p.M, N,
+                                                                                                                p.N, i, sums, b);
         FP_CHECK_LAUNCH();
+        sums.sums = nullptr;
     }
     return 0;
 }
@@ -485,19 +522,6 @@ Plan plan(int e, const void* x, int64_t ldx, const void* wg, int64_t ldwg, const
     p.parts = (copied * up64(K) * 2 + 255) & ~(int64_t)255;
     p.bytes = p.splits > 1 ? p.parts + (int64_t)p.splits * M * 2 * up8(F) * 4 : copied * up64(K) * 2;
     return p;
-}
-
-template <typename T>
-int copy_rows(Copies c, int cols, int cols_p, hipStream_t st) {
-    c.cols = cols;
-    c.cols_p = cols_p;
-    c.chunks = ((int64_t)c.rows_p[0] + c.rows_p[1] + c.rows_p[2]) * (cols_p / 8);
-    c.blocks = (unsigned)(c.chunks < 2048 * 256 ? (c.chunks + 255) / 256 : 2048);
-    const unsigned sums = c.sums ? 2 * (unsigned)((c.F + 63) / 64) : 0;
-    if (c.blocks + sums == 0) return 0;
-    copy_rows_kernel<T><<<dim3(c.blocks + sums), dim3(256), 0, st>>>(c);
-    FP_CHECK_LAUNCH();
-    return 0;
 }
 
 template <typename TI, typename TO>
@@ -550,7 +574,9 @@ int ff_launch(const void* x, int64_t ldx, const float* xs, const void* wg, int64
                 c.rows[0] = c.rows_p[0] = p.x_fits ? 0 : M;
                 c.rows[1] = c.rows_p[1] = p.g_fits ? 0 : F;
                 c.rows[2] = c.rows_p[2] = p.u_fits ? 0 : F;
-                if (int rc = copy_rows<TI>(c, K, Kp, st)) return rc;
+                count(c, K, Kp);
+                copy_rows_kernel<TI><<<dim3((unsigned)std::min((c.chunks + 255) / 256, COPY_BLOCKS)), dim3(256), 0, st>>>(c);
+                FP_CHECK_LAUNCH();
                 if (!p.x_fits) x = xp, ldx = Kp;
                 if (!p.g_fits) wg = gp, ldwg = Kp;
                 if (!p.u_fits) wu = upk, ldwu = Kp;
@@ -584,9 +610,6 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
     T *dgu = (T*)(base + g.dgu), *dgut = (T*)(base + g.dgut), *xc = (T*)(base + g.x), *wc = (T*)(base + g.w);
     float *colsum = db ? (float*)(base + g.colsum) : nullptr, *parts = (float*)(base + g.parts);
     const int whole = g.plain_w ? F / 64 : Fp / 64, x_whole = g.plain_x ? M / 64 : Mp / 64, wc_rows = g.plain_w ? 64 : Fp;
-    glu_grad_kernel<T><<<dim3((unsigned)(Fp / 64), (unsigned)(Mp / 64)), dim3(256), 0, st>>>(
-        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, Fp, Mp, whole, act);
-    FP_CHECK_LAUNCH();
     // what the products cannot read as it lies: all of it, or the rows of a partial last K tile
     const int xr = M % 64, wr = F % 64;
     Copies c{{x, wg, wu}, {xc, wc, wc + wc_rows * g.ldw}, {ldx, ldwg, ldwu}, {g.ldx, g.ldw, g.ldw}};
@@ -596,9 +619,12 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
     c.rows_p[0] = g.plain_x ? (xr ? 64 : 0) : Mp;
     c.rows[1] = c.rows[2] = g.plain_w ? wr : F;
     c.rows_p[1] = c.rows_p[2] = g.plain_w ? (wr ? 64 : 0) : Fp;
-    c.sums = colsum;
-    c.tiles = Mp / 64, c.F = F, c.Fp = Fp, c.db = db;
-    if (int rc = copy_rows<T>(c, K, Kp, st)) return rc;
+    count(c, K, Kp);
+    const int64_t copy_rows = (std::min((c.chunks + 255) / 256, COPY_BLOCKS) + Fp / 64 - 1) / (Fp / 64);       // of blocks
+    glu_grad_kernel<T><<<dim3((unsigned)(Fp / 64), (unsigned)(Mp / 64 + copy_rows)), dim3(256), 0, st>>>(
+        (const T*)dh, ldh, (const T*)gate, ldg, (const T*)up, ldu, dgu, dgut, colsum, M, F, Fp, Mp, whole, act, c);
+    FP_CHECK_LAUNCH();
+    ColumnSums sums{colsum, Mp / 64, F, Fp, db};
     const T *w0 = g.plain_w ? (const T*)wg : wc, *w1 = g.plain_w ? (const T*)wu : wc + wc_rows * g.ldw, *x0 = g.plain_x ? (const T*)x : xc;
     // where K tile t lies if one matrix went on: w0's tiles, w1's from tile `whole` on, the copies' from tile 2 whole on
     auto jump = [](const T* to, const T* from, int64_t tiles, int64_t ld) { return ((intptr_t)to - (intptr_t)from) - tiles * 64 * ld * 2; };
@@ -607,12 +633,17 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
     p.s1 = whole, p.d1 = jump(w1, w0, whole, g.ldw);
     p.s2 = 2 * whole, p.d2 = jump(wc, w0, 2 * whole, g.ldw) - p.d1;
     p.M = M, p.K = 2 * Fp;
-    if (int rc = product<T>(p, (T*)dx, K, parts, st)) return rc;
+    if (int rc = product<T>(p, (T*)dx, K, parts, sums, st)) return rc;
     p.a = dgut, p.lda = Mp, p.w = x0, p.ldw = g.ldx;
     p.s1 = x_whole, p.d1 = jump(xc, x0, x_whole, g.ldx);
     p.s2 = 1 << 30, p.d2 = 0;
     p.M = 2 * F, p.K = Mp;
-    return product<T>(p, (T*)dw, K, parts, st);
+    if (int rc = product<T>(p, (T*)dw, K, parts, sums, st)) return rc;
+    if (sums.sums) {
+        column_sums_kernel<T><<<dim3(sums.blocks()), dim3(256), 0, st>>>(sums);
+        FP_CHECK_LAUNCH();
+    }
+    return 0;
 }
 
 }  // namespace
