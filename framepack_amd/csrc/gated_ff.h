@@ -29,3 +29,5 @@ struct GradProduct {
     void* out;
 };
 __attribute__((visibility("hidden"))) int fpi_grad_product(int type, const GradProduct& p, hipStream_t st);
+// Two in one launch of 256 x 128 tiles: `first` (splits > 0), then `second`.
+__attribute__((visibility("hidden"))) int fpi_grad_pair(int type, const GradProduct& first, const GradProduct& second, hipStream_t st);

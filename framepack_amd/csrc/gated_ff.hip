@@ -431,6 +431,43 @@ Cut cut(int64_t M, int N, int K) {
 }
 int64_t cut_bytes(int64_t M, int N, int K) { return (int64_t)cut(M, N, K).splits * M * up8(N) * 4; }
 
+// Both products of the gradient in one launch (fpi_grad_pair): dx in parts of K first, then dw, in parts too if dw.splits > 0.
+// Workgroup i takes items i, i + 256, .. of 256 x 128 tiles: the cuts are those that leave the longest workgroup the fewest K
+// tiles of about 0.7 us; an item counts 3 more (its first loads, its stores), what goes through 32 bits its traffic and launch.
+// Taken where dx's 256 x 256 tiles fill less than half the chip and dw's are no more than 384: the whole gradient, one launch /
+// two launches, us: 129 rows, [K, F] = [256, 512] 17 / 28; 729, [1152, 4304] (170 tiles) 62 / 71; 8000, [256, 1024] 66 / 80; 512,
+// [2048, 5504] (344) 82 / 86; 1024, [2048, 8192] (512) 189 / 177: there 256 x 256 tiles, which stage less a product, win.
+struct Pair {
+    Cut dx, dw;                     // dx.splits == 0: not this way
+};
+Pair pair(int M, int F, int K) {
+    const int nk = (int)up64(F) / 32, nk_w = (int)up64(M) / 64, tn = (K + 127) / 128;
+    const int64_t t = (int64_t)((M + 255) / 256) * tn, t_w = (2 * (int64_t)F + 255) / 256 * tn;
+    Pair best{{0, nk, true}, {0, nk_w, true}};
+    if (K % 8 != 0 || !cut(M, K, 64 * nk).narrow || (2 * (int64_t)F + 255) / 256 * ((K + 255) / 256) > 384) return best;
+    double least = 1e30;
+    auto trial = [&](int s, int s_w) {
+        const int per = (nk + s - 1) / s, per_w = (nk_w + s_w - 1) / s_w;
+        const unsigned n = (unsigned)(t * ((nk + per - 1) / per)), n_w = (unsigned)(t_w * ((nk_w + per_w - 1) / per_w));
+        const unsigned all = (n + n_w + 255) / 256, up = (n + 255) / 256, down = n / 256, rest = (n + n_w - n % 256 + 255) / 256;
+        // workgroup 0, and the first with an item of dx less
+        const unsigned most = std::max(up * (per + 3) + (all - up) * (per_w + 3), down * (per + 3) + (rest - down) * (per_w + 3));
+        const double cost = most + (2.3e-6 * s * M * K) + (s_w > 1 ? 6 + 2.3e-6 * s_w * 2 * F * K : 0);
+        if (cost < least) {
+            least = cost;
+            best.dx = {(nk + per - 1) / per, per, true};
+            best.dw = {s_w > 1 ? (nk_w + per_w - 1) / per_w : 0, per_w, true};
+        }
+    };
+    const int most_w = (int)std::min<int64_t>(nk_w / 8, 256 / t_w);
+    for (int s = 1; s <= 32 && (s == 1 || nk / s >= 8); ++s) {
+        trial(s, 1);
+        if (most_w > 1) trial(s, most_w);
+        if (most_w > 3) trial(s, most_w / 2);
+    }
+    return best;
+}
+
 // Rows up to which the weights are streamed (glu_few_kernel).  [K, F] = [4096, 14336], streamed / matrix-core kernel, us:
 // bf16 45 / 70 at 1 row, 56 / 69 at 32, 64 / 71 at 48, 70 / 73 at 64; e4m3 21 / 30 at 1, 32 / 34 at 48, 37 / 35 at 64.
 constexpr int FEW = 48;
@@ -467,14 +504,28 @@ GradSpace grad_space(const void* x, int64_t ldx, const void* wg, int64_t ldwg, c
     g.x = take((g.plain_x ? (M % 64 ? 64 : 0) : Mp) * g.ldx * 2);
     g.w = take(2 * (g.plain_w ? (F % 64 ? 64 : 0) : Fp) * g.ldw * 2);
     g.colsum = take(Mp / 64 * 2 * Fp * 4);
-    const int64_t a = cut_bytes(M, K, (int)(2 * Fp)), b = cut_bytes(2 * F, K, (int)Mp);
-    g.parts = take(a > b ? a : b);
+    const Pair both = pair((int)M, (int)F, K);
+    g.parts = take(both.dx.splits > 0 ? (both.dx.splits * M + both.dw.splits * 2 * F) * K * 4
+                                      : std::max(cut_bytes(M, K, (int)(2 * Fp)), cut_bytes(2 * F, K, (int)Mp)));
     g.end = at;
     return g;
 }
 
-// out [M, N] = the product, through fp32 parts where it is cut.  sums: taken along by the launch that adds the parts up, if
-// there is one (`sums.sums` is null from then on).
+// out [M, N] = sum of the parts [splits][M, up8(N)]; sums: taken along by the (first) launch, `sums.sums` is null from then on
+template <typename T>
+int add_parts(const float* parts, int splits, T* out, int64_t M, int N, ColumnSums& sums, hipStream_t st) {
+    const int64_t Np = up8(N), lanes = M * (Np / 4), most = int64_t(1) << 31;        // (a launch's lanes have to stay below 2^32)
+    for (int64_t i = 0; i < lanes; i += most) {
+        const unsigned b = sums.blocks();
+        add_parts_kernel<T><<<dim3((unsigned)((std::min(most, lanes - i) + 255) / 256) + b), dim3(256), 0, st>>>(parts, splits, out, M, N,
+                                                                                                                (int)Np, i, sums, b);
+        FP_CHECK_LAUNCH();
+        sums.sums = nullptr;
+    }
+    return 0;
+}
+
+// out [M, N] = the product, through fp32 parts where it is cut
 template <typename T>
 int product(GradProduct p, T* out, int N, float* parts, ColumnSums& sums, hipStream_t st) {
     const Cut c = cut(p.M, N, p.K);
@@ -484,16 +535,7 @@ int product(GradProduct p, T* out, int N, float* parts, ColumnSums& sums, hipStr
     p.N = (int)up8(N);
     p.out = c.splits ? (void*)parts : (void*)out;
     if (int rc = fpi_grad_product(__is_same(T, bf16) ? FF_BF16 : FF_F16, p, st)) return rc;
-    if (c.splits == 0) return 0;
-    const int64_t lanes = (int64_t)p.M * (p.N / 4), most = int64_t(1) << 31;         // (a launch's lanes have to stay below 2^32)
-    for (int64_t i = 0; i < lanes; i += most) {
-        const unsigned b = sums.blocks();
-        add_parts_kernel<T><<<dim3((unsigned)((std::min(most, lanes - i) + 255) / 256) + b), dim3(256), 0, st>>>(parts, c.splits, out, p.M, N,
-                                                                                                                p.N, i, sums, b);
-        FP_CHECK_LAUNCH();
-        sums.sums = nullptr;
-    }
-    return 0;
+    return c.splits == 0 ? 0 : add_parts<T>(parts, c.splits, out, p.M, N, sums, st);
 }
 
 // How a forward call runs.  e: bytes of an operand's element.
@@ -628,17 +670,27 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
     const T *w0 = g.plain_w ? (const T*)wg : wc, *w1 = g.plain_w ? (const T*)wu : wc + wc_rows * g.ldw, *x0 = g.plain_x ? (const T*)x : xc;
     // where K tile t lies if one matrix went on: w0's tiles, w1's from tile `whole` on, the copies' from tile 2 whole on
     auto jump = [](const T* to, const T* from, int64_t tiles, int64_t ld) { return ((intptr_t)to - (intptr_t)from) - tiles * 64 * ld * 2; };
-    GradProduct p{};
+    GradProduct p{}, q{};
     p.a = dgu, p.lda = 2 * Fp, p.w = w0, p.ldw = g.ldw;
     p.s1 = whole, p.d1 = jump(w1, w0, whole, g.ldw);
     p.s2 = 2 * whole, p.d2 = jump(wc, w0, 2 * whole, g.ldw) - p.d1;
     p.M = M, p.K = 2 * Fp;
+    q.a = dgut, q.lda = Mp, q.w = x0, q.ldw = g.ldx;
+    q.s1 = x_whole, q.d1 = jump(xc, x0, x_whole, g.ldx);
+    q.s2 = 1 << 30, q.d2 = 0;
+    q.M = 2 * F, q.K = Mp;
+    if (const Pair both = pair(M, F, K); both.dx.splits > 0) {
+        float* parts_w = parts + (int64_t)both.dx.splits * M * K;
+        p.splits = both.dx.splits, p.ks_per = both.dx.ks_per, p.out = parts;
+        q.splits = both.dw.splits, q.ks_per = both.dw.ks_per, q.out = both.dw.splits > 0 ? (void*)parts_w : dw;
+        p.N = q.N = K;
+        if (int rc = fpi_grad_pair(__is_same(T, bf16) ? FF_BF16 : FF_F16, p, q, st)) return rc;
+        if (both.dw.splits > 0)
+            if (int rc = add_parts<T>(parts_w, both.dw.splits, (T*)dw, 2 * F, K, sums, st)) return rc;
+        return add_parts<T>(parts, both.dx.splits, (T*)dx, M, K, sums, st);
+    }
     if (int rc = product<T>(p, (T*)dx, K, parts, sums, st)) return rc;
-    p.a = dgut, p.lda = Mp, p.w = x0, p.ldw = g.ldx;
-    p.s1 = x_whole, p.d1 = jump(xc, x0, x_whole, g.ldx);
-    p.s2 = 1 << 30, p.d2 = 0;
-    p.M = 2 * F, p.K = Mp;
-    if (int rc = product<T>(p, (T*)dw, K, parts, sums, st)) return rc;
+    if (int rc = product<T>(q, (T*)dw, K, parts, sums, st)) return rc;
     if (sums.sums) {
         column_sums_kernel<T><<<dim3(sums.blocks()), dim3(256), 0, st>>>(sums);
         FP_CHECK_LAUNCH();

@@ -190,8 +190,19 @@ struct TrArgs {
     int s1, s2;
     int64_t d1, d2;
 };
+// DUAL (TRW): one launch for two products, so that the second's tiles follow where the first's leave CUs idle: the tiles of
+// a product in fp32 parts of K (all of it described here: c [splits][M, N], N % 8 == 0), then those of the kernel's ordinary
+// arguments (with SPLIT in parts too).  Workgroup i takes tiles i, i + gridDim.x, .. of that row.
+struct PartsArgs {
+    const void *a, *w;
+    float* c;
+    int64_t lda, ldw;
+    TrArgs tr;
+    int M, N, K, ntm, ntn, gm;
+    SplitArgs sp;
+};
 template <typename T, typename TO, int EPI, int AMODE, int NT = 8, int QKN = 0, int TALL = 0, int GRP = 0, int GLU = 0,
-          int KEEP = 0, int SPLIT = 0, int TRW = 0>
+          int KEEP = 0, int SPLIT = 0, int TRW = 0, int DUAL = 0>
 __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A, int64_t lda, int64_t a2_delta,
                                                          int k1, const T* __restrict__ W, int64_t ldw,
                                                          const TO* __restrict__ bias_, TO* __restrict__ C,
@@ -200,7 +211,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                                                          const TO* __restrict__ gate_, int ntm, int ntn, ConvGeom cg,
                                                          const float* __restrict__ a_scale,
                                                          const float* __restrict__ w_scale, QkNormArgs qk, Rows2 r2,
-                                                         GluArgs glu, SplitArgs sp, TrArgs tr) {
+                                                         GluArgs glu, SplitArgs sp, TrArgs tr, PartsArgs pp) {
+    static_assert(!DUAL || (TRW && NT == 4), "two products: the narrow tile of W by rows of K");
     static_assert(!TRW || (AMODE == 0 && !TALL && !QKN && !GRP && !GLU && EPI == 0 && sizeof(T) == 2 && (NT == 8 || NT == 4)),
                   "W by rows of K: the dense 16-bit tile");
     static_assert(!GLU || (AMODE == 0 && !TALL && !QKN && !GRP && EPI == 0 && sizeof(TO) == (SPLIT ? 4 : 2) && NT >= 4), "gated block: the dense tile");
@@ -265,36 +277,65 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     // tile order: XCD-contiguous, grouped 8 row-tiles tall so that co-running tiles share A and W panels.  The
     // workgroup is persistent: it takes tiles vb = blockIdx.x, + gridDim.x, ... (gridDim.x is a multiple of 8 or
     // the whole tile count, so vb & 7 stays this workgroup's XCD).
-    const int ntiles = ntm * ntn * (SPLIT ? sp.splits : 1);
+    const int n_parts = DUAL ? pp.ntm * pp.ntn * pp.sp.splits : 0;
+    const int ntiles = n_parts + ntm * ntn * (SPLIT ? sp.splits : 1);
+    bool parts_ = false;            // DUAL: the tile is one of the product in parts
     constexpr int CW = NT * 16;     // W rows per wave column
     constexpr int TBN = TALL || GLU ? CW : 2 * CW;                   // output columns of a tile
     // GLU: output columns of a wave, 16-B chunks of its rows, rows per store instruction; the epilogue's stores of a tile
     constexpr int OCW = CW / 2, CPR = OCW / 8, RPI = CPR > 0 ? 64 / CPR : 64;
     constexpr int N_STORES = GLU ? 16 / RPI * 8 * (KEEP ? 3 : 1) : 32;
-    int part = 0;                   // SPLIT: which run of K tiles
+    int part = 0, k_first = 0;      // SPLIT: which run of K tiles, and its first
     int nk = K / BKE;
-    const int64_t w_tile = TRW ? (int64_t)BKE * (int)sizeof(T) * ldw : 0;      // bytes from a K tile of W to the next
+    int64_t w_tile = TRW ? (int64_t)BKE * (int)sizeof(T) * ldw : 0;            // bytes from a K tile of W to the next
+    TrArgs trc = tr;
     unsigned a_rd[2], w_rd[2];  // fragment read addresses (below)
     const int fr = lane & 15, fq = lane >> 4;
     constexpr unsigned SECOND = SCALED ? 16u : 64u;
     const unsigned off_k0 = (unsigned)(fr * 128 + (((SCALED ? 2 * fq : fq) ^ (fr >> 1)) << 4));
     auto setup = [&](int vb) __attribute__((always_inline)) {
         // ConvGeom::gm: gm > 0: gm row tiles x all column tiles per group; gm < 0: -gm column tiles x all row tiles
-        const int GM = cg.gm != 0 ? abs(cg.gm) : 8;
         int wid = xcd_remap(vb, ntiles);
         if constexpr (SPLIT) {
+            if (DUAL) wid = vb < n_parts ? 0 : xcd_remap(vb - n_parts, ntiles - n_parts);
             part = wid / (ntm * ntn);
             wid -= part * (ntm * ntn);
-            nk = min(sp.ks_per, K / BKE - part * sp.ks_per);
+            k_first = part * sp.ks_per;
+            nk = min(sp.ks_per, K / BKE - k_first);
         }
-        const int nmaj = cg.gm < 0 ? ntn : ntm, nmin = cg.gm < 0 ? ntm : ntn;
+        const T *A_ = A, *W_ = W;
+        int64_t lda_ = lda, ldw_ = ldw;
+        int N_ = N, ntm_ = ntm, ntn_ = ntn, gm = cg.gm;
+        if constexpr (DUAL) {
+            parts_ = vb < n_parts;
+            m_end = M;
+            trc = tr;
+            if (!SPLIT) {
+                wid = xcd_remap(vb - n_parts, ntiles - n_parts);
+                k_first = 0;
+                nk = K / BKE;
+            }
+            if (parts_) {
+                wid = xcd_remap(vb, n_parts);
+                A_ = reinterpret_cast<const T*>(pp.a), W_ = reinterpret_cast<const T*>(pp.w);
+                lda_ = pp.lda, ldw_ = pp.ldw, trc = pp.tr;
+                m_end = pp.M, N_ = pp.N, ntm_ = pp.ntm, ntn_ = pp.ntn, gm = pp.gm;
+                part = wid / (ntm_ * ntn_);
+                wid -= part * (ntm_ * ntn_);
+                k_first = part * pp.sp.ks_per;
+                nk = min(pp.sp.ks_per, pp.K / BKE - k_first);
+            }
+            w_tile = (int64_t)BKE * (int)sizeof(T) * ldw_;
+        }
+        const int GM = gm != 0 ? abs(gm) : 8;
+        const int nmaj = gm < 0 ? ntn_ : ntm_, nmin = gm < 0 ? ntm_ : ntn_;
         const int per_group = GM * nmin;
         const int group = wid / per_group, in_group = wid % per_group;
         const int first = group * GM;
         const int gsz = min(nmaj - first, GM);
         const int tmaj = first + in_group % gsz, tmin = in_group / gsz;
-        int tm = cg.gm < 0 ? tmin : tmaj;
-        const int tn = cg.gm < 0 ? tmaj : tmin;
+        int tm = gm < 0 ? tmin : tmaj;
+        const int tn = gm < 0 ? tmaj : tmin;
         if (AMODE == 1 && cg.band > 0) {               // band-major walk (ConvGeom::band): position -> (band, frame, tile)
             const int per = cg.band * cg.To, bnd = tm / per, rem = tm - bnd * per;
             const int t = rem / cg.band;
@@ -320,7 +361,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             for (int j = 0; j < APW; ++j) {
                 const int ar = arow0[h][j] + prow;
                 if (AMODE == 0) {
-                    pa[h][j] = (unsigned)(min(m0 + ar, m_end - 1) - m0) * (unsigned)(lda * sizeof(T)) + (pch ^ ((ar >> 1) & 7)) * 16;
+                    pa[h][j] = (unsigned)(min(m0 + ar, m_end - 1) - m0) * (unsigned)(lda_ * sizeof(T)) + (pch ^ ((ar >> 1) & 7)) * 16;
                 } else {
                     const int m = min(m0 + ar, M - 1);
                     const int wc = (m % cg.Wo) << cg.dw, hc = ((m / cg.Wo) % cg.Ho) << cg.dh,
@@ -348,7 +389,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             if constexpr (TRW) {
                 const int row = lane >> 4, c = lane & 15, i = wave * WPW + j, q = (c >> 1) ^ (row | ((j & 2) << 1));
                 const int col = (NT == 8 ? (i >> 4) * 128 : 0) + q * 16 + (c & 1) * 8;
-                pw[j] = (unsigned)((i & 15) * 4 + row) * (unsigned)(ldw * sizeof(T)) + (unsigned)min(col, N - 8 - n0) * (unsigned)sizeof(T);
+                pw[j] = (unsigned)((i & 15) * 4 + row) * (unsigned)(ldw_ * sizeof(T)) + (unsigned)min(col, N_ - 8 - n0) * (unsigned)sizeof(T);
                 continue;
             }
             // GLU: the wave's WPW pieces are the rows of wave column wave >> 1 of one of the two matrices
@@ -357,14 +398,15 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                     (pch ^ ((wrw >> 1) & 7)) * 16;
         }
         abase = AMODE == 1 ? reinterpret_cast<const char*>(A) + ((int64_t)lo_vox << (cg.lcin + LOG2_TB))
-                           : reinterpret_cast<const char*>(A + (int64_t)m0 * lda);
+                           : reinterpret_cast<const char*>(A_ + (int64_t)m0 * lda_);
+        if constexpr (DUAL) w_seg = W_;
         wbase = reinterpret_cast<const char*>(w_seg + (TRW ? (int64_t)n0 : (int64_t)n0 * ldw));
         if constexpr (GLU) {
             if (wave & 1) wbase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(glu.w2) + (int64_t)n0 * glu.ldw2);
         }
-        if constexpr (SPLIT) {
-            abase += (int64_t)part * sp.ks_per * 128;
-            if (!TRW) wbase += (int64_t)part * sp.ks_per * 128;
+        if constexpr (SPLIT || DUAL) {
+            abase += (int64_t)k_first * 128;
+            if (!TRW) wbase += (int64_t)k_first * 128;
         }
     };
     // AMODE 1: a K tile is one tap x 64 or 128 channels, and with Cin >= 2 K tiles per tap (the launcher sends narrower
@@ -422,8 +464,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     auto src_w = [&](int j, int t) __attribute__((always_inline)) -> const T* {
         asm volatile("" : "+v"(pw[j]));
         if constexpr (TRW) {
-            const int tg = t + (SPLIT ? part * sp.ks_per : 0);
-            return reinterpret_cast<const T*>(wbase + (int64_t)tg * w_tile + (tg >= tr.s1 ? tr.d1 : 0) + (tg >= tr.s2 ? tr.d2 : 0) + pw[j]);
+            const int tg = t + (SPLIT || DUAL ? k_first : 0);
+            return reinterpret_cast<const T*>(wbase + (int64_t)tg * w_tile + (tg >= trc.s1 ? trc.d1 : 0) + (tg >= trc.s2 ? trc.d2 : 0) + pw[j]);
         }
         return reinterpret_cast<const T*>(wbase + (int64_t)t * (BKE * (int)sizeof(T)) + pw[j]);
     };
@@ -802,6 +844,21 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             });
         });
     };
+    auto dual_parts = [&](int em0, int en0, int epart) __attribute__((always_inline)) {
+        const int el = opaque_lane();
+        const int fr = el & 15, nb = en0 + wc * CW + 4 * (el >> 4);
+        static_for<8>([&](auto MI_) __attribute__((always_inline)) {
+            constexpr int mi = MI_;
+            const int mrow0 = em0 + wr * 128 + mi * 16;
+            if (mrow0 >= pp.M) return;                         // wave-uniform
+            static_for<NT>([&](auto NI_) __attribute__((always_inline)) {
+                constexpr int ni = NI_;
+                const f32x4 av = acc_read<(mi * 8 + ni) * 4>();
+                if (mrow0 + fr < pp.M && nb + ni * 16 < pp.N)
+                    *reinterpret_cast<f32x4*>(pp.c + ((int64_t)epart * pp.M + mrow0 + fr) * pp.N + nb + ni * 16) = av;
+            });
+        });
+    };
     auto epilogue = [&](int em0, int en0, int ecw, int epart) __attribute__((always_inline)) {
       const int64_t part0 = SPLIT ? (int64_t)epart * M : 0;      // (the whole M)
       const int M = seg_rows(em0);              // shadows the kernel's
@@ -975,6 +1032,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     bool relaxed = false;
     for (;;) {
         const int em0 = m0, en0 = n0, epart = part;
+        const bool eparts = DUAL && parts_;
         constexpr int ecw = CW;
         phase(ic<0>{}, ic<0>{}, 0, ic<0>{}, ic<1>{}, relaxed, ic<0>{});
         phase(ic<0>{}, ic<1>{}, 0, ic<1>{}, ic<1>{}, relaxed, ic<1>{});
@@ -1026,6 +1084,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         asm volatile("s_nop 15\ns_nop 15" ::: "memory");        // the last MFMAs retire before their tiles are read
         if constexpr (GLU && SPLIT) glu_parts(em0, en0, epart);
         else if constexpr (GLU) glu_epilogue(em0, en0);
+        else if (eparts) dual_parts(em0, en0, epart);
         else epilogue(em0, en0, ecw, epart);
 #if defined(FP_PROBE_REG_LOAD)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1040,7 +1099,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
             for (int j = 0; j < APW; ++j) poff[1][j] = tap_off(1, j, 0);
         }
         // a ragged tile skips stores, so the relaxed count would not cover the loads: drain instead
-        if (em0 + TBM > seg_rows(em0) || en0 + TBN > N) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (em0 + TBM > (eparts ? pp.M : seg_rows(em0)) || en0 + TBN > (eparts ? pp.N : N)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         relaxed = true;
     }
 }
@@ -1059,26 +1118,29 @@ inline int persistent_grid() {
 }
 
 template <typename T, int EPI, int AMODE, typename TO = T, int NT = 8, int QKN = 0, int TALL = 0, int GRP = 0, int GLU = 0,
-          int KEEP = 0, int SPLIT = 0, int TRW = 0>
+          int KEEP = 0, int SPLIT = 0, int TRW = 0, int DUAL = 0>
 int launch_w4(const void* a, int64_t lda, int64_t a2_delta, int k1, const void* w, int64_t ldw, const void* bias,
               void* c, int64_t ldc, int M, int N, int K, int gelu_from, const void* resid, int64_t ldr,
               const void* gate, const ConvGeom& cg, hipStream_t st, const float* a_scale = nullptr,
               const float* w_scale = nullptr, const QkNormArgs& qk = QkNormArgs{}, const Rows2& r2 = Rows2{},
-              const GluArgs& glu = GluArgs{}, const SplitArgs& sp = SplitArgs{}, const TrArgs& tr = TrArgs{}) {
+              const GluArgs& glu = GluArgs{}, const SplitArgs& sp = SplitArgs{}, const TrArgs& tr = TrArgs{},
+              const PartsArgs& pp = PartsArgs{}) {
     // lane offsets inside a tile are 32-bit: 255 rows x the row stride in bytes has to fit
-    if (lda >= (int64_t(1) << 22) || ldw >= (int64_t(1) << 22) || glu.ldw2 >= (int64_t(1) << 22)) return (int)hipErrorInvalidValue;
+    if (lda >= (int64_t(1) << 22) || ldw >= (int64_t(1) << 22) || glu.ldw2 >= (int64_t(1) << 22) ||
+        pp.lda >= (int64_t(1) << 22) || pp.ldw >= (int64_t(1) << 22))
+        return (int)hipErrorInvalidValue;
     constexpr int TBM = TALL ? 2 * BM : BM, TBN = TALL || GLU ? 16 * NT : 32 * NT;
     const int ntm = GRP ? (r2.m_split + TBM - 1) / TBM + (M - r2.m_split + TBM - 1) / TBM : (M + TBM - 1) / TBM;
     const int ntn = (N + TBN - 1) / TBN;
     // operand buffers + the epilogue's row stage (TALL: all 160 KiB are operand buffers, the stage lies inside them)
     constexpr int smem = TALL ? 5 * OP_BYTES : 2 * BUF_BYTES + 4 * 8192;
-    auto kern = gemm_w4_kernel<T, TO, EPI, AMODE, NT, QKN, TALL, GRP, GLU, KEEP, SPLIT, TRW>;
+    auto kern = gemm_w4_kernel<T, TO, EPI, AMODE, NT, QKN, TALL, GRP, GLU, KEEP, SPLIT, TRW, DUAL>;
     hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != hipSuccess) return (int)e;
-    kern<<<dim3((unsigned)min(ntm * ntn * (SPLIT ? sp.splits : 1), persistent_grid())), dim3(256), smem, st>>>((const T*)a, lda, a2_delta, k1, (const T*)w, ldw,
+    kern<<<dim3((unsigned)min(ntm * ntn * (SPLIT ? sp.splits : 1) + pp.ntm * pp.ntn * pp.sp.splits, persistent_grid())), dim3(256), smem, st>>>((const T*)a, lda, a2_delta, k1, (const T*)w, ldw,
                                                               (const TO*)bias, (TO*)c, ldc, M, N, K, gelu_from,
                                                               (const TO*)resid, ldr, (const TO*)gate, ntm, ntn, cg,
-                                                              a_scale, w_scale, qk, r2, glu, sp, tr);
+                                                              a_scale, w_scale, qk, r2, glu, sp, tr, pp);
     FP_CHECK_LAUNCH();
     return 0;
 }

@@ -658,3 +658,15 @@ def test_the_widest_blocks():
     within(h, h64, h64.abs() * (u_of(BF) + 2 * E32))
     # each lane adds 65537 squares up, then the lanes' sums: half of (65537 + 8) 2^-24 relative, by the root
     within(y, y64, y64.abs() * (u_of(BF) + (65545 / 2 + 8) * E32))
+
+
+# both products in one launch with dw whole / in parts of K; two launches, dx in parts of K / whole 256 x 128 / 256 x 256 tiles
+@pytest.mark.parametrize("M,F,K", [(700, 1400, 392), (2100, 136, 264), (130, 4104, 4096), (1300, 4104, 4096), (2100, 4104, 4096)])
+def test_gated_ff_gradient_each_way_its_products_are_cut(M, F, K):
+    dh, x = randn(M, F, seed=1, dtype=BF), randn(M, K, seed=2, dtype=BF)
+    wg, wu = randn(F, K, seed=3, scale=K ** -0.5, dtype=BF), randn(F, K, seed=4, scale=K ** -0.5, dtype=BF)
+    g, u = randn(M, F, seed=5, scale=2.0, dtype=BF), randn(M, F, seed=6, dtype=BF)
+    got = ops.gated_ff_backward(dh, x, wg, wu, g, u, bias=True)
+    check_ff_grad(got, dh, x, wg, wu, g, u, ops.ACT_SILU, BF)
+    again = ops.gated_ff_backward(dh, x, wg, wu, g, u, bias=True)
+    assert all(torch.equal(a, b) for a, b in zip(again, got))
