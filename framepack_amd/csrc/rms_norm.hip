@@ -39,14 +39,21 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     return v;
 }
 
-// y / scale by one Newton step on y * (1 / scale), so that it rounds as a division does
-__device__ __forceinline__ float divide(float y, float scale, float inv) {
-    const float q = y * inv;
-    return __builtin_fmaf(__builtin_fmaf(-q, scale, y), inv, q);
+// e4m3: q = 448 t / top with t = h w, top = max|t|, and the row's scale r top / 448.  The norm's factor r is one of the scale
+// alone (in q it would cancel, but for its roundings), unless it is 0, infinite or NaN: then t has it and the scale has not.
+// A row of zeros has top = 448, scale 1; between the bounds neither top / 448 nor its reciprocal is infinite.
+__device__ __forceinline__ float in_q(float r) { return r > 0.f && r < __builtin_inff() ? 1.f : r; }
+__device__ __forceinline__ float row_top(float amax) {
+    return amax > 0.f ? fminf(fmaxf(amax, FP8_MAX * 0x1p-126f), 0x1.fffffep127f) : FP8_MAX;
 }
-// The row's scale.  A row of zeros gets 1; between the bounds neither scale nor 1 / scale is infinite.
-__device__ __forceinline__ float row_scale(float amax) {
-    return amax > 0.f ? fminf(fmaxf(amax / FP8_MAX, 0x1p-126f), 0x1p127f) : 1.f;
+__device__ __forceinline__ float row_scale(float amax, float top, float r) {
+    return top / FP8_MAX * (amax > 0.f && in_q(r) == 1.f ? r : 1.f);
+}
+// 448 t / top = 7 t / m with m = top / 64 (exact), inv = 1 / m: the remainder 7 t - q m, taken as (8 t - q m) - t, corrects the
+// first quotient, so that one rounding is left in front of that to 8 bits.
+__device__ __forceinline__ float quotient(float t, float m, float inv) {
+    const float q = t * (7.f * inv);
+    return __builtin_fmaf(__builtin_fmaf(-q, m, 8.f * t) - t, inv, q);
 }
 
 typedef unsigned int any_u32x2 __attribute__((ext_vector_type(2), aligned(1)));
@@ -131,20 +138,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(const T*
         }
     }
     float m = 0.f;
+    const float f = Q8 ? in_q(r) : r;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         V o;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[i][j] = v[i][j] * r * (float)wv[i][j];
+            v[i][j] = v[i][j] * f * (float)wv[i][j];
             if constexpr (Q8) m = fmaxf(m, fabsf(v[i][j]));
             else o[j] = (T)v[i][j];
         }
         if constexpr (!Q8) store8(y + row * y_rs, (i * TPR + lane) * 8, cols, o);
     }
     if constexpr (Q8) {
-        const float scale = row_scale(row_max<TPR>(m, red[1])), inv = 1.f / scale;
-        if (lane == 0) q_scale[row] = scale;
+        const float amax = row_max<TPR>(m, red[1]), top = row_top(amax), m64 = top * 0x1p-6f, inv = 1.f / m64;
+        if (lane == 0) q_scale[row] = row_scale(amax, top, r);
         unsigned char* qr = reinterpret_cast<unsigned char*>(y) + row * y_rs;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
@@ -153,8 +161,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(const T*
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 int p = 0;
-                p = __builtin_amdgcn_cvt_pk_fp8_f32(divide(v[i][4 * k], scale, inv), divide(v[i][4 * k + 1], scale, inv), p, false);
-                p = __builtin_amdgcn_cvt_pk_fp8_f32(divide(v[i][4 * k + 2], scale, inv), divide(v[i][4 * k + 3], scale, inv), p, true);
+                p = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[i][4 * k], m64, inv), quotient(v[i][4 * k + 1], m64, inv), p, false);
+                p = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(v[i][4 * k + 2], m64, inv), quotient(v[i][4 * k + 3], m64, inv), p, true);
                 o[k] = (unsigned)p;
             }
             if (c + 8 <= cols) {
@@ -187,17 +195,20 @@ __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(const T* x, int64_t x
         ss += v * v;
     }
     const float r = 1.f / sqrtf(block_sum(ss, red) / (float)cols + eps);
-    float scale = 1.f, inv = 1.f;
+    const float f = Q8 ? in_q(r) : r;
+    float m64 = 1.f, inv = 1.f;
     if constexpr (Q8) {
         float m = 0.f;
-        for (int c = threadIdx.x; c < cols; c += 256) m = fmaxf(m, fabsf(at(c) * r * (float)w[c]));
-        scale = row_scale(block_max(m, red));
-        inv = 1.f / scale;
-        if (threadIdx.x == 0) q_scale[row] = scale;
+        for (int c = threadIdx.x; c < cols; c += 256) m = fmaxf(m, fabsf(at(c) * f * (float)w[c]));
+        const float amax = block_max(m, red);
+        const float top = row_top(amax);
+        m64 = top * 0x1p-6f;
+        inv = 1.f / m64;
+        if (threadIdx.x == 0) q_scale[row] = row_scale(amax, top, r);
     }
     for (int c = threadIdx.x; c < cols; c += 256) {
-        const float v = at(c), o = v * r * (float)w[c];
-        if constexpr (Q8) reinterpret_cast<unsigned char*>(y)[row * y_rs + c] = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(divide(o, scale, inv), 0.f, 0, false) & 0xff);
+        const float v = at(c), o = v * f * (float)w[c];
+        if constexpr (Q8) reinterpret_cast<unsigned char*>(y)[row * y_rs + c] = (unsigned char)(__builtin_amdgcn_cvt_pk_fp8_f32(quotient(o, m64, inv), 0.f, 0, false) & 0xff);
         else y[row * y_rs + c] = (T)o;
         if (rr) h[row * h_rs + c] = (T)v;
     }

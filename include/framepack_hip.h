@@ -220,7 +220,8 @@ int fp_rmsnorm_residual_f16(const void* x, int64_t x_row_stride, const void* res
 
 /* K12 into 8 bits: x, resid, weight, h bf16 as above, q: e4m3 [rows, cols] (row stride ldq bytes) and q_scale: fp32
  * [rows] with y ~ q_scale * q, q_scale = max|y| / 448 (1 for a row of zeros): the A operand of fp_gemm_fp8_bf16 and
- * fp_gated_ff_fp8.  q is rounded once, from the 32-bit y.  A NaN is left out of the row's maximum and stays a NaN. */
+ * fp_gated_ff_fp8.  q is rounded once, from 32 bits.  A NaN is left out of the row's maximum and stays a NaN.  A row of which
+ * no |h weight| reaches 2^-117 loses resolution. */
 int fp_rmsnorm_residual_fp8(const void* x, int64_t x_row_stride, const void* resid, int64_t resid_row_stride,
                             const void* weight, void* q, int64_t ldq, void* q_scale, void* h, int64_t h_row_stride,
                             int rows, int cols, float eps, void* stream);
