@@ -1,4 +1,6 @@
-// K13's gradient products on the matrix cores: instances of gemm_w4.h (see TrArgs and SplitArgs there).
+// K13's gradient products on the matrix cores: instances of gemm_w4.h (see TrArgs, SplitArgs and PartsArgs there; figures in
+// gated_ff.hip).  W by rows of K is read as it lies: transposed copies of Wg, Wu and x would move 213 MB each way at 4096 rows
+// of [4096, 11008], where either product takes 535 us.
 #include "gated_ff.h"
 #include "gemm_w4.h"
 
@@ -8,14 +10,12 @@ static bool fits(const GradProduct& p) {
     return p.K % BK == 0 && p.N % 8 == 0 && (int64_t)(p.M / 256 + 1) * (p.N / 128 + 1) * (p.splits > 0 ? p.splits : 1) < (1ll << 30) &&
            (p.splits == 0 || ((int64_t)(p.splits - 1) * p.ks_per < p.K / BK && (int64_t)p.splits * p.ks_per >= p.K / BK));
 }
-static int walk(const GradProduct& p) { return p.K >= 8192 ? -3 : 8; }         // the tiles' order (ConvGeom::gm)
 
 template <typename T>
 static int run(const GradProduct& p, hipStream_t st) {
     const TrArgs tr{p.s1, p.s2, p.d1, p.d2};
     const SplitArgs sp{p.splits, p.ks_per};
-    ConvGeom cg{};
-    cg.gm = walk(p);
+    const ConvGeom cg{};
     FP_REQUIRE(fits(p));
 #define FP_TR(TO, NT, SPLIT)                                                                                                         \
     return launch_w4<T, 0, 0, TO, NT, 0, 0, 0, 0, 0, SPLIT, 1>(p.a, p.lda, 0, p.K, p.w, p.ldw, nullptr, p.out, p.N, p.M, p.N, p.K, 0, \
@@ -30,10 +30,9 @@ static int run(const GradProduct& p, hipStream_t st) {
 template <typename T>
 static int run_pair(const GradProduct& q, const GradProduct& p, hipStream_t st) {
     FP_REQUIRE(fits(q) && fits(p) && q.splits > 0);
-    ConvGeom cg{};
-    cg.gm = walk(p);
+    const ConvGeom cg{};
     const PartsArgs pp{q.a, q.w, (float*)q.out, q.lda, q.ldw, {q.s1, q.s2, q.d1, q.d2}, q.M, q.N, q.K, (q.M + BM - 1) / BM, (q.N + 127) / 128,
-                       walk(q), {q.splits, q.ks_per}};
+                       {q.splits, q.ks_per}};
 #define FP_PAIR(TO, SPLIT)                                                                                                          \
     return launch_w4<T, 0, 0, TO, 4, 0, 0, 0, 0, 0, SPLIT, 1, 1>(p.a, p.lda, 0, p.K, p.w, p.ldw, nullptr, p.out, p.N, p.M, p.N, p.K, 0, \
                                                                 nullptr, 0, nullptr, cg, st, nullptr, nullptr, QkNormArgs{}, Rows2{}, \

@@ -1,4 +1,4 @@
-// K13's forward product on the matrix cores: instances of gemm_w4.h (see GluArgs there).
+// K13's forward product on the matrix cores: instances of gemm_w4.h (see GluArgs there; figures in gated_ff.hip).
 #include "gated_ff.h"
 #include "gemm_w4.h"
 

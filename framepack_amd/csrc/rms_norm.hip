@@ -7,11 +7,11 @@
 // All of it is bound by HBM: the row stays in registers between its sums and its last use, so every matrix is read or written
 // once.  Measured in bf16 (a large copy runs at 4.9 TB/s on the same card), us and TB/s of those bytes:
 //   rows x cols      y and h        e4m3 and h     gradient
-//   19385 x 4096     114  5.6       100  5.6       127  5.0
-//   19385 x 4095     114  5.6       106  5.3       152  4.2     (rows that begin at any 2 bytes)
-//   8191 x 4096      47   5.7       43   5.4       55   4.9
+//   19385 x 4096     113  5.6       100  5.6       127  5.0
+//   19385 x 4095     135  4.7       119  4.7       152  4.2     (rows that begin at any 2 bytes: lines shared between lanes' loads)
+//   8191 x 4096      44   6.1       41   5.7       55   4.9
 //   512 x 4096       5.2            5.6            11           (two launches)
-//   1 x 4096         2.6            3.2            6
+//   1 x 4096         2.6            3.2            6            (latency; the call from Python takes 9 - 14 us on the host)
 #include "row_access.h"
 
 extern "C" int64_t fp_rmsnorm_residual_backward_workspace_bytes(int rows, int cols);
