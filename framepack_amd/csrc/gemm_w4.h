@@ -195,7 +195,8 @@ struct TrArgs {
 };
 // DUAL (TRW): one launch for two products, so that the second's tiles follow where the first's leave CUs idle: the tiles of
 // a product in fp32 parts of K (all of it described here: c [splits][M, N], N % 8 == 0), then those of the kernel's ordinary
-// arguments (with SPLIT in parts too).  729 rows, [1152, 4304]: 40 us, in two launches 24 + 26.  Workgroup i takes tiles i, i + gridDim.x, .. of that row.
+// arguments (with SPLIT in parts too).  Workgroup i takes tiles i, i + gridDim.x, .. of that row.  729 rows, [1152, 4304]:
+// 40 us, in two launches 24 + 26.
 struct PartsArgs {
     const void *a, *w;
     float* c;

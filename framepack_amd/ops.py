@@ -899,7 +899,8 @@ def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: 
     """K13: h = act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up) in one kernel, act = ACT_SILU or ACT_GELU; returns h
     [M, inner], with keep (h, gate, up): the two projections before the activation, as `gated_ff_backward` takes them.
     x [M, K], w_gate, w_up [inner, K] (nn.Linear layout; row-strided ok, slices of one fused weight too), any sizes (K
-    below 2^20 for more than 48 rows); one type, bf16 or f16.  The block's second linear is `gemm`, with the residual in its epilogue (EPI_RESIDUAL)."""
+    below 2^20 for more than 48 rows); one type, bf16 or f16.  The block's second linear is `gemm`, with the residual in its
+    epilogue (EPI_RESIDUAL)."""
     _dev(x, w_gate, w_up, b_gate, b_up, out)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, (BF16, F16), x.dtype)
     h, h2, ldh = _out(out, "out", x.dtype, M, F, x)
