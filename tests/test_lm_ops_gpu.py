@@ -670,3 +670,18 @@ def test_gated_ff_gradient_each_way_its_products_are_cut(M, F, K):
     check_ff_grad(got, dh, x, wg, wu, g, u, ops.ACT_SILU, BF)
     again = ops.gated_ff_backward(dh, x, wg, wu, g, u, bias=True)
     assert all(torch.equal(a, b) for a, b in zip(again, got))
+
+
+@pytest.mark.parametrize("cols", [1000, 520])
+def test_norm_of_many_short_rows(cols):
+    rows = 2050                                              # four rows a workgroup from 2048 rows on, two chunks a lane
+    x, r, w = randn(rows, cols, seed=1, dtype=BF), randn(rows, cols, seed=2, dtype=BF), randn(cols, seed=3, dtype=BF)
+    h64, y64 = norm64(x, r, w)
+    y, h = ops.rmsnorm_residual(x, w, r)
+    within(y, y64, norm_tol(y64, BF, cols))
+    within(h, h64, h64.abs() * (u_of(BF) + 2 * E32))
+    q, s, _ = ops.rmsnorm_residual_fp8(x, w, r)
+    amax = y64.abs().amax(1)
+    within(s, amax / 448, amax / 448 * (cols / 2 + 10) * E32)
+    # half a step of e4m3: 2^-4 of the value, 2^-10 of the scale below the normal range
+    within(q.double() * s.double()[:, None], y64, y64.abs() * (2.0 ** -4 + 2 * (cols / 2 + 10) * E32) + s.double()[:, None] * 2.0 ** -10)
