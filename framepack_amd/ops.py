@@ -969,4 +969,4 @@ def gated_ff_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w
         _lib.check(fn(d2.data_ptr(), ldd, x2.data_ptr(), ldx, g2.data_ptr(), ldg, u2.data_ptr(), ldu, p2.data_ptr(), ldp,
                       q2.data_ptr(), ldq, dx.data_ptr(), dw.data_ptr(), _ptr(db), M, F, K, act,
                       ws.data_ptr(), n, _stream(x)), name)
-    return dx, dw[:F], dw[F:], None if db is None else db[:F], None if db is None else db[F:]
+    return (dx, *dw.chunk(2), *(db.chunk(2) if bias else (None, None)))
