@@ -11,7 +11,7 @@
 // product at 1440 TFLOP/s in bf16 and 2370 in e4m3.  Measured, [K, F], us:
 //   1 row, [4096, 14336], bf16           44      5.4 TB/s of weights
 //   16 rows, the same, e4m3              24      4.9 TB/s
-//   49 - 256 rows, the same, bf16        70 - 78 3.3 - 3.0 TB/s (a tile of 256 rows is staged whatever the rows)
+//   64 - 256 rows, the same, bf16        63 - 75 3.7 - 3.1 TB/s (128 bytes of a row a K tile)
 //   729 rows, [1152, 4304], f16          22      (204 tiles on 256 CUs; 10 of it first loads and epilogue)
 //   4096 rows, [4096, 14336], e4m3       388     2480 TFLOP/s
 //   19385 rows, [4096, 14336], bf16      3230    1410 TFLOP/s (matrix pipe 78 % busy at 1.74 GHz)
