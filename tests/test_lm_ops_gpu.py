@@ -685,3 +685,42 @@ def test_norm_of_many_short_rows(cols):
     within(s, amax / 448, amax / 448 * (cols / 2 + 10) * E32)
     # half a step of e4m3: 2^-4 of the value, 2^-10 of the scale below the normal range
     within(q.double() * s.double()[:, None], y64, y64.abs() * (2.0 ** -4 + 2 * (cols / 2 + 10) * E32) + s.double()[:, None] * 2.0 ** -10)
+
+
+# one launch for both products with several tiles a workgroup, of whole and of ragged tiles, dw whole and in parts
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("M,F,K", [(512, 4096, 1024), (729, 4304, 1152), (8192, 512, 512), (7777, 520, 392)])
+def test_gated_ff_gradient_of_several_tiles_a_workgroup(M, F, K, dtype):
+    dh, x = randn(M, F, seed=1, dtype=dtype), randn(M, K, seed=2, dtype=dtype)
+    wg, wu = randn(F, K, seed=3, scale=K ** -0.5, dtype=dtype), randn(F, K, seed=4, scale=K ** -0.5, dtype=dtype)
+    g, u = randn(M, F, seed=5, scale=2.0, dtype=dtype), randn(M, F, seed=6, dtype=dtype)
+    want = ops.gated_ff_backward(dh, x, wg, wu, g, u, act=ops.ACT_GELU)
+    check_ff_grad(want, dh, x, wg, wu, g, u, ops.ACT_GELU, dtype)
+    for _ in range(4):
+        got = ops.gated_ff_backward(dh, x, wg, wu, g, u, act=ops.ACT_GELU)
+        assert all(torch.equal(a, b) for a, b in zip(got[:3], want[:3]))
+
+
+# more tiles than workgroups, in either order of the tiles
+@pytest.mark.parametrize("M,F,K", [(3000, 4104, 256), (2816, 3968, 128), (12300, 776, 128)])
+def test_gated_ff_of_several_tiles_a_workgroup(M, F, K):
+    w = [randn(F, K, seed=s, scale=K ** -0.5) for s in (2, 3)]
+    bg, bu = randn(F, seed=4), randn(F, seed=5)
+    for dtype in (BF, HF):
+        x, wg, wu = randn(M, K, seed=1, dtype=dtype), w[0].to(dtype), w[1].to(dtype)
+        b = (bg.to(dtype), bu.to(dtype))
+        h64, g, u, eg, eu = ff64(x, wg, wu, *b, ops.ACT_GELU)
+        h, gate, up = ops.gated_ff(x, wg, wu, *b, act=ops.ACT_GELU, keep=True)
+        within(h, h64, ff_tol(h64, g, u, eg, eu, ops.ACT_GELU, dtype), "h")
+        within(gate, g, g.abs() * u_of(dtype) + 2 * eg + tiny_of(dtype), "gate")
+        within(up, u, u.abs() * u_of(dtype) + 2 * eu + tiny_of(dtype), "up")
+        for _ in range(4):
+            assert torch.equal(ops.gated_ff(x, wg, wu, *b, act=ops.ACT_GELU), h)
+    x, xs = ops.quantize_rows_fp8(randn(M, K, seed=1, dtype=BF))
+    (wg, gs), (wu, us) = quantised(w[0]), quantised(w[1])
+    deq = [q.double() * s.double()[:, None] for q, s in ((x, xs), (wg, gs), (wu, us))]
+    h64, g, u, eg, eu = ff64(*deq, None, None, ops.ACT_SILU)
+    h = ops.gated_ff_fp8(x, xs, wg, gs, wu, us)
+    within(h, h64, ff_tol(h64, g, u, eg + 4 * E32 * g.abs(), eu + 4 * E32 * u.abs(), ops.ACT_SILU, BF), "e4m3")
+    for _ in range(4):
+        assert torch.equal(ops.gated_ff_fp8(x, xs, wg, gs, wu, us), h)
