@@ -949,8 +949,8 @@ def gated_ff_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w
                       up: torch.Tensor, act: int = ACT_SILU, bias: bool = False):
     """Gradient of K13: (dx, dw_gate, dw_up, db_gate, db_up) from dh (of h) and the projections that `gated_ff(keep=True)`
     returned; the biases' are None unless `bias`.  One type throughout, bf16 or f16; the gradients of the projections are
-    rounded to it between the two steps, sums are held in 32 bits and taken in a fixed order.  dw_gate and dw_up are the
-    halves of one [2 * inner, K] tensor (the gradient of a fused weight)."""
+    rounded to it between the two steps (in f16 they overflow past 65504), sums are held in 32 bits and taken in a fixed
+    order.  dw_gate and dw_up are the halves of one [2 * inner, K] tensor (the gradient of a fused weight)."""
     _dev(dh, x, w_gate, w_up, gate, up)
     dt = (x.dtype,)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, _, _ = _gated_ff_args(x, w_gate, w_up, None, None, act, (BF16, F16), x.dtype)
