@@ -395,31 +395,39 @@ __global__ __launch_bounds__(256) void glu_grad_kernel(const T* __restrict__ dh,
         colsum[(int64_t)blockIdx.y * (2 * Fp) + w * Fp + f0 + l] = (cs[w][0][l] + cs[w][1][l]) + (cs[w][2][l] + cs[w][3][l]);
     }
 }
-// out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns, from chunk i0 on.  The
-// last cs.blocks() blocks add up column sums instead.
-template <typename T>
-__global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, int splits, T* __restrict__ out, int64_t M, int N,
-                                                        int Np, int64_t i0, ColumnSums cs, unsigned cs_blocks) {
-    if (blockIdx.x >= gridDim.x - cs_blocks) {
-        column_sums_of<T>(cs, (int)(blockIdx.x - (gridDim.x - cs_blocks)));
-        return;
-    }
-    const int64_t i = i0 + (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int per = Np / 4;
-    if (i >= M * per) return;
+// out [M, N] = sum of the parts [splits][M, Np] (Np % 8 == 0), rounded once; a lane takes four columns, from chunk i0 on.
+struct PartSum {
+    const float* part;
+    void* out;
+    int64_t M, i0;
+    int splits, N, Np;
+    unsigned blocks;
+};
+template <typename T> __device__ __forceinline__ void add_parts_of(const PartSum& q, unsigned block) {
+    const int64_t i = q.i0 + (int64_t)block * 256 + threadIdx.x;
+    const int per = q.Np / 4;
+    if (i >= q.M * per) return;
     const int64_t m = i / per;
     const int n = (int)(i - m * per) * 4;
-    f32x4 s = *reinterpret_cast<const f32x4*>(part + m * Np + n);
-    for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + ((int64_t)k * M + m) * Np + n);
-    T* to = out + m * N + n;
+    f32x4 s = *reinterpret_cast<const f32x4*>(q.part + m * q.Np + n);
+    for (int k = 1; k < q.splits; ++k) s += *reinterpret_cast<const f32x4*>(q.part + ((int64_t)k * q.M + m) * q.Np + n);
+    T* to = reinterpret_cast<T*>(q.out) + m * q.N + n;
     typedef T A4 __attribute__((ext_vector_type(4), aligned(2)));
-    if (n + 4 <= N) {
+    if (n + 4 <= q.N) {
         *reinterpret_cast<A4*>(to) = A4{(T)s[0], (T)s[1], (T)s[2], (T)s[3]};
     } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
-            if (n + j < N) to[j] = (T)s[j];
+            if (n + j < q.N) to[j] = (T)s[j];
     }
+}
+// Up to two such sums, and column sums by the blocks behind theirs.
+template <typename T>
+__global__ __launch_bounds__(256) void add_parts_kernel(PartSum a, PartSum b, ColumnSums cs) {
+    const unsigned i = blockIdx.x;
+    if (i < a.blocks) add_parts_of<T>(a, i);
+    else if (i < a.blocks + b.blocks) add_parts_of<T>(b, i - a.blocks);
+    else column_sums_of<T>(cs, (int)(i - a.blocks - b.blocks));
 }
 
 // How a product [M, N] over K (a multiple of 64) is cut: whole (0 parts: straight to 16 bits) where its 256 x 256 tiles fill
@@ -458,7 +466,7 @@ Pair pair(int M, int F, int K) {
     const int nk = (int)up64(F) / 32, nk_w = (int)up64(M) / 64, tn = (K + 127) / 128;
     const int64_t t = (int64_t)((M + 255) / 256) * tn, t_w = (2 * (int64_t)F + 255) / 256 * tn;
     Pair best{{0, nk, true}, {0, nk_w, true}};
-    if (K % 8 != 0 || !cut(M, K, 64 * nk).narrow || (2 * (int64_t)F + 255) / 256 * ((K + 255) / 256) > 384) return best;
+    if (!cut(M, K, 64 * nk).narrow || (2 * (int64_t)F + 255) / 256 * ((K + 255) / 256) > 384) return best;
     double least = 1e30;
     auto trial = [&](int s, int s_w) {
         const int per = (nk + s - 1) / s, per_w = (nk_w + s_w - 1) / s_w;
@@ -466,11 +474,12 @@ Pair pair(int M, int F, int K) {
         const unsigned all = (n + n_w + 255) / 256, up = (n + 255) / 256, down = n / 256, rest = (n + n_w - n % 256 + 255) / 256;
         // workgroup 0, and the first with an item of dx less
         const unsigned most = std::max(up * (per + 3) + (all - up) * (per_w + 3), down * (per + 3) + (rest - down) * (per_w + 3));
-        const double cost = most + (2.3e-6 * s * M * K) + (s_w > 1 ? 6 + 2.3e-6 * s_w * 2 * F * K : 0);
+        const bool parts_w = s_w > 1 || K % 8 != 0;        // (the 16-bit stores are 16 bytes wide)
+        const double cost = most + (2.3e-6 * s * M * K) + (parts_w ? 2 + 2.3e-6 * s_w * 2 * F * K : 0);
         if (cost < least) {
             least = cost;
             best.dx = {(nk + per - 1) / per, per, true};
-            best.dw = {s_w > 1 ? (nk_w + per_w - 1) / per_w : 0, per_w, true};
+            best.dw = {parts_w ? (nk_w + per_w - 1) / per_w : 0, per_w, true};
         }
     };
     const int most_w = (int)std::min<int64_t>(nk_w / 8, 256 / t_w);
@@ -519,23 +528,31 @@ GradSpace grad_space(const void* x, int64_t ldx, const void* wg, int64_t ldwg, c
     g.w = take(2 * (g.plain_w ? (F % 64 ? 64 : 0) : Fp) * g.ldw * 2);
     g.colsum = take(Mp / 64 * 2 * Fp * 4);
     const Pair both = pair((int)M, (int)F, K);
-    g.parts = take(both.dx.splits > 0 ? (both.dx.splits * M + both.dw.splits * 2 * F) * K * 4
+    g.parts = take(both.dx.splits > 0 ? (both.dx.splits * M + both.dw.splits * 2 * F) * Kp * 4
                                       : std::max(cut_bytes(M, K, (int)(2 * Fp)), cut_bytes(2 * F, K, (int)Mp)));
     g.end = at;
     return g;
 }
 
-// out [M, N] = sum of the parts [splits][M, up8(N)]; sums: taken along by the (first) launch, `sums.sums` is null from then on
+// out [M, N] = sum of the parts [splits][M, up8(N)], `also` with it; sums: taken along by the (first) launch, `sums.sums` is null
+// from then on.  A launch's lanes have to stay below 2^32.
+PartSum part_sum(const float* parts, int splits, void* out, int64_t M, int N) {
+    const int64_t lanes = M * (up8(N) / 4);
+    return {parts, out, M, 0, splits, N, (int)up8(N), (unsigned)((std::min(lanes, int64_t(1) << 30) + 255) / 256)};
+}
 template <typename T>
-int add_parts(const float* parts, int splits, T* out, int64_t M, int N, ColumnSums& sums, hipStream_t st) {
-    const int64_t Np = up8(N), lanes = M * (Np / 4), most = int64_t(1) << 31;        // (a launch's lanes have to stay below 2^32)
-    for (int64_t i = 0; i < lanes; i += most) {
-        const unsigned b = sums.blocks();
-        add_parts_kernel<T><<<dim3((unsigned)((std::min(most, lanes - i) + 255) / 256) + b), dim3(256), 0, st>>>(parts, splits, out, M, N,
-                                                                                                                (int)Np, i, sums, b);
-        FP_CHECK_LAUNCH();
-        sums.sums = nullptr;
+int add_parts(PartSum q, PartSum also, ColumnSums& sums, hipStream_t st) {
+    for (PartSum* one : {&also, &q}) {                      // the rest of a sum of more lanes than one launch is given
+        const int64_t lanes = one->M * (one->Np / 4);
+        for (PartSum more = *one; (more.i0 += int64_t(1) << 30) < lanes;) {
+            more.blocks = (unsigned)((std::min(lanes - more.i0, int64_t(1) << 30) + 255) / 256);
+            add_parts_kernel<T><<<dim3(more.blocks), dim3(256), 0, st>>>(more, PartSum{}, ColumnSums{});
+            FP_CHECK_LAUNCH();
+        }
     }
+    add_parts_kernel<T><<<dim3(q.blocks + also.blocks + sums.blocks()), dim3(256), 0, st>>>(q, also, sums);
+    FP_CHECK_LAUNCH();
+    sums.sums = nullptr;
     return 0;
 }
 
@@ -549,7 +566,7 @@ int product(GradProduct p, T* out, int N, float* parts, ColumnSums& sums, hipStr
     p.N = (int)up8(N);
     p.out = c.splits ? (void*)parts : (void*)out;
     if (int rc = fpi_grad_product(__is_same(T, bf16) ? FF_BF16 : FF_F16, p, st)) return rc;
-    return c.splits == 0 ? 0 : add_parts<T>(parts, c.splits, out, p.M, N, sums, st);
+    return c.splits == 0 ? 0 : add_parts<T>(part_sum(parts, c.splits, out, p.M, N), PartSum{}, sums, st);
 }
 
 // How a forward call runs.  e: bytes of an operand's element.
@@ -694,14 +711,13 @@ int ff_grad_launch(const void* dh, int64_t ldh, const void* x, int64_t ldx, cons
     q.s2 = 1 << 30, q.d2 = 0;
     q.M = 2 * F, q.K = Mp;
     if (const Pair both = pair(M, F, K); both.dx.splits > 0) {
-        float* parts_w = parts + (int64_t)both.dx.splits * M * K;
+        float* parts_w = parts + (int64_t)both.dx.splits * M * Kp;
         p.splits = both.dx.splits, p.ks_per = both.dx.ks_per, p.out = parts;
         q.splits = both.dw.splits, q.ks_per = both.dw.ks_per, q.out = both.dw.splits > 0 ? (void*)parts_w : dw;
-        p.N = q.N = K;
+        p.N = q.N = Kp;
         if (int rc = fpi_grad_pair(__is_same(T, bf16) ? FF_BF16 : FF_F16, p, q, st)) return rc;
-        if (both.dw.splits > 0)
-            if (int rc = add_parts<T>(parts_w, both.dw.splits, (T*)dw, 2 * F, K, sums, st)) return rc;
-        return add_parts<T>(parts, both.dx.splits, (T*)dx, M, K, sums, st);
+        return add_parts<T>(part_sum(parts, both.dx.splits, dx, M, K),
+                            both.dw.splits > 0 ? part_sum(parts_w, both.dw.splits, dw, 2 * F, K) : PartSum{}, sums, st);
     }
     if (int rc = product<T>(p, (T*)dx, K, parts, sums, st)) return rc;
     if (int rc = product<T>(q, (T*)dw, K, parts, sums, st)) return rc;
