@@ -724,3 +724,25 @@ def test_gated_ff_of_several_tiles_a_workgroup(M, F, K):
     within(h, h64, ff_tol(h64, g, u, eg + 4 * E32 * g.abs(), eu + 4 * E32 * u.abs(), ops.ACT_SILU, BF), "e4m3")
     for _ in range(4):
         assert torch.equal(ops.gated_ff_fp8(x, xs, wg, gs, wu, us), h)
+
+
+def test_gated_ff_gradient_of_more_weights_than_a_launch_adds_up():
+    M, F, K = 2, 1 << 17, 16385                              # dw: 2^32 values and more, in 32-bit parts (an odd width)
+    dh, x = randn(M, F, seed=1, dtype=BF), randn(M, K, seed=2, dtype=BF)
+    g, u = randn(M, F, seed=5, scale=2.0, dtype=BF), randn(M, F, seed=6, dtype=BF)
+    gen = torch.Generator(DEV).manual_seed(3)
+    wg, wu = (torch.empty(F, K, dtype=BF, device=DEV).normal_(generator=gen) for _ in range(2))
+    dx, dwg, dwu, _, _ = ops.gated_ff_backward(dh, x, wg, wu, g, u)
+    dg, du = ff_grad64(dh, x, wg[:1], wu[:1], g, u, ops.ACT_SILU)[:2]
+    ug = u_of(BF) * dg.abs() + 3 * 400 * E32 * dh.double().abs() * u.double().abs()
+    uu = (u_of(BF) + 400 * E32) * du.abs()
+    n = 2 * (M + 8) * E32
+    for d, e, o in ((dg, ug, dwg), (du, uu, dwu)):
+        for at in (slice(0, 200), slice(F - 300, F)):
+            want = d[:, at].t() @ x.double()
+            within(o[at], want, want.abs() * u_of(BF) + (e + n * d.abs())[:, at].t() @ x.double().abs(), "dw")
+    n = 2 * (2 * F + 8) * E32
+    for at in (slice(0, 40), slice(K - 40, K)):
+        a, b = wg[:, at].double(), wu[:, at].double()
+        want = dg @ a + du @ b
+        within(dx[:, at], want, want.abs() * u_of(BF) + (ug + n * dg.abs()) @ a.abs() + (uu + n * du.abs()) @ b.abs(), "dx")
