@@ -166,14 +166,17 @@ struct GluArgs {
     int64_t ldp;
     int act;                                    // 0: SiLU, 1: tanh-GELU
 };
-// act(v) = v / (1 + 2^-z),  z = log2(e) v (SiLU) or 2 log2(e) sqrt(2/pi) (v + 0.044715 v^3) (tanh-GELU): one expression with
-// two constants.  v is clamped in z only (past 1e4 the quotient has long run into 0 or v), so that v^2 stays finite.
-__device__ __forceinline__ float glu_act(float v, float c0, float c1) {
-    const float t = __builtin_amdgcn_fmed3f(v, -1e4f, 1e4f);
-    return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-t * __builtin_fmaf(t * t, c1, c0)));
+// act(v) = v / (1 + 2^-z),  z = log2(e) v (SiLU) or 2 log2(e) sqrt(2/pi) (v + 0.044715 v^3) (tanh-GELU).  v is clamped in the
+// latter's z (past 1e4 the quotient has long run into 0 or v), so that v^2 stays finite.
+template <int ACT> __device__ __forceinline__ float glu_act(float v) {
+    constexpr float l = 1.4426950408889634f, k = 2.f * l * 0.7978845608028654f;
+    float z = l * v;
+    if constexpr (ACT != 0) {
+        const float t = __builtin_amdgcn_fmed3f(v, -1e4f, 1e4f);
+        z = t * __builtin_fmaf(t * t, k * 0.044715f, k);
+    }
+    return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z));
 }
-__device__ __forceinline__ float glu_c0(int act) { return 1.4426950408889634f * (act ? 2.f * 0.7978845608028654f : 1.f); }
-__device__ __forceinline__ float glu_c1(int act) { return act ? 1.4426950408889634f * 2.f * 0.7978845608028654f * 0.044715f : 0.f; }
 // SPLIT > 0 (gated_ff.hip: few output tiles, a long K): the K tiles are dealt to `splits` workgroups per output tile in runs of
 // ks_per, and part s goes to rows [s M, (s + 1) M) of the fp32 output; the caller adds them up.  With GLU, both projections'
 // sums: the first from column 0 on, the second from column ldp on (ldp >= N a multiple of 4; columns up to it are written).
@@ -751,7 +754,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
     // GLU: lane (fr, fq) holds, for ni < NT / 2, both projections of row em0 + wr*128 + mi*16 + fr, columns en0 + wc * OCW +
     // ni*16 + 4 fq + (0..3).  Rows leave through the wave's stage as below, OCW columns (2 OCW bytes) a row; KEEP: three images.
     typedef TO Tx8_any __attribute__((ext_vector_type(8), aligned(2)));
-    auto glu_epilogue = [&](int em0, int en0) __attribute__((always_inline)) {
+    // ACT, BIAS: two choices made once, outside: a lone wave per SIMD pays 4 cycles for every instruction of its 128 outputs a lane
+    auto glu_epilogue = [&](auto ACT, auto BIAS, int em0, int en0) __attribute__((always_inline)) {
         unsigned stage_off = 2 * BUF_BYTES + wave * 8192;
         asm volatile("" : "+v"(stage_off));
         unsigned char* stage = smem + stage_off;
@@ -763,8 +767,7 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
 #pragma unroll
         for (int ni = 0; ni < NT / 2; ++ni) {
             const int n = nb + ni * 16;
-            bv[0][ni] = bv[1][ni] = Tx4{0, 0, 0, 0};
-            if (bias_) {
+            if constexpr (BIAS) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     bv[0][ni][j] = bias_[min(n + j, N - 1)];
@@ -776,7 +779,6 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                 ws[1][ni] = *reinterpret_cast<const f32x4*>(glu.w_scale2 + min(n, N - 4));
             }
         }
-        const float c0 = glu_c0(glu.act), c1 = glu_c1(glu.act);
         const int lrow = el / CPR, lchk = el % CPR;
         const int gcol = en0 + wc * OCW + lchk * 8;
         static_for<8>([&](auto MI_) __attribute__((always_inline)) {
@@ -794,9 +796,12 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                 Tx4 o, og, ou;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float g = (SCALED ? ag[j] * (as * ws[0][ni][j]) : ag[j]) + (float)bv[0][ni][j];
-                    const float u = (SCALED ? au[j] * (as * ws[1][ni][j]) : au[j]) + (float)bv[1][ni][j];
-                    o[j] = (TO)(glu_act(g, c0, c1) * u);
+                    float g = SCALED ? ag[j] * (as * ws[0][ni][j]) : ag[j], u = SCALED ? au[j] * (as * ws[1][ni][j]) : au[j];
+                    if constexpr (BIAS) {
+                        g += (float)bv[0][ni][j];
+                        u += (float)bv[1][ni][j];
+                    }
+                    o[j] = (TO)(glu_act<ACT>(g) * u);
                     og[j] = (TO)g;
                     ou[j] = (TO)u;
                 }
@@ -1088,7 +1093,15 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
         fence();
         asm volatile("s_nop 15\ns_nop 15" ::: "memory");        // the last MFMAs retire before their tiles are read
         if constexpr (GLU && SPLIT) glu_parts(em0, en0, epart);
-        else if constexpr (GLU) glu_epilogue(em0, en0);
+        else if constexpr (GLU) {
+            if (glu.act == 0) {
+                if (bias_) glu_epilogue(ic<0>{}, ic<1>{}, em0, en0);
+                else glu_epilogue(ic<0>{}, ic<0>{}, em0, en0);
+            } else {
+                if (bias_) glu_epilogue(ic<1>{}, ic<1>{}, em0, en0);
+                else glu_epilogue(ic<1>{}, ic<0>{}, em0, en0);
+            }
+        }
         else if (eparts) dual_parts(em0, en0, epart);
         else epilogue(em0, en0, ecw, epart);
 #if defined(FP_PROBE_REG_LOAD)
