@@ -41,6 +41,13 @@ __device__ __forceinline__ float group16_sum(float v) {
     return v;
 }
 
+// K3's sum of squared deviations (its 16-bit and its e4m3 form have to give the same bits): every square is rounded before it is
+// added, under every compiler option.
+__device__ __forceinline__ float k3_add_square(float ss, float d) {
+#pragma clang fp contract(off)
+    return ss + d * d;
+}
+
 // K2's arithmetic between its rounding points (norm_kernels.hip and the GEMM epilogue that replaces it, gemm_w4.h, have to give
 // the same bits): what is fused and what is not is written out, so that no compiler option decides it for one of them alone.
 __device__ __forceinline__ float k2_sum_of_squares(const float (&f)[8]) {

@@ -104,10 +104,7 @@ __global__ __launch_bounds__(256) void ln_modulate_fp8_kernel(const bf16* __rest
         const int col = c * 512 + lane * 8;
         if (col < cols) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = v[c][j] - mean;
-                ss += d * d;
-            }
+            for (int j = 0; j < 8; ++j) ss = k3_add_square(ss, v[c][j] - mean);
         }
     }
     const float rstd = rsqrtf(wave_sum(ss) / (float)cols + eps);
