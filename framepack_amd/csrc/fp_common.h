@@ -58,9 +58,16 @@ __device__ __forceinline__ float k2_sum_of_squares(const float (&f)[8]) {
     return ss;
 }
 __device__ __forceinline__ float k2_rstd(float row_ss, float eps) { return rsqrtf(__builtin_fmaf(row_ss, 1.f / 128.f, eps)); }
-// the rotary pair (re, im): (re c0 - im s0, im c1 + re s1)
-__device__ __forceinline__ float k2_rot_re(float re, float im, float c0, float s0) { return __builtin_fmaf(re, c0, -(im * s0)); }
-__device__ __forceinline__ float k2_rot_im(float re, float im, float c1, float s1) { return __builtin_fmaf(im, c1, re * s1); }
+// Rotary pair p of a lane's four, (re, im): (re c0 - im s0, im c1 + re s1).  Both products of the last pair are rounded before they
+// are added, of the others' only the one with the sine: the results that these kernels have given from the start.
+__device__ __forceinline__ float k2_rot_re(int p, float re, float im, float c0, float s0) {
+#pragma clang fp contract(off)
+    return p == 3 ? re * c0 - im * s0 : __builtin_fmaf(re, c0, -(im * s0));
+}
+__device__ __forceinline__ float k2_rot_im(int p, float re, float im, float c1, float s1) {
+#pragma clang fp contract(off)
+    return p == 3 ? im * c1 + re * s1 : __builtin_fmaf(im, c1, re * s1);
+}
 
 // Bijective XCD-aware remap (blocks b and b+8 share an XCD's L2): gives each XCD a contiguous run of
 // work items so that neighbours in work order share operands through one L2.

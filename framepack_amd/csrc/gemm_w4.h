@@ -1020,8 +1020,8 @@ __global__ __launch_bounds__(256, 1) void gemm_w4_kernel(const T* __restrict__ A
                             const float sn[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
 #pragma unroll
                             for (int p2 = 0; p2 < 4; ++p2) {
-                                ov[2 * p2] = (TO)k2_rot_re(nn[2 * p2], nn[2 * p2 + 1], c[2 * p2], sn[2 * p2]);
-                                ov[2 * p2 + 1] = (TO)k2_rot_im(nn[2 * p2], nn[2 * p2 + 1], c[2 * p2 + 1], sn[2 * p2 + 1]);
+                                ov[2 * p2] = (TO)k2_rot_re(p2, nn[2 * p2], nn[2 * p2 + 1], c[2 * p2], sn[2 * p2]);
+                                ov[2 * p2 + 1] = (TO)k2_rot_im(p2, nn[2 * p2], nn[2 * p2 + 1], c[2 * p2 + 1], sn[2 * p2 + 1]);
                             }
                         } else {
 #pragma unroll

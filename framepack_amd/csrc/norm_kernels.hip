@@ -153,8 +153,8 @@ __global__ __launch_bounds__(256) void qk_rmsnorm_rope_kernel(bf16* __restrict__
         const float s[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
 #pragma unroll
         for (int p = 0; p < 4; ++p) {                        // pair (2p, 2p+1): rot = (-imag, real)
-            o[2 * p] = (bf16)k2_rot_re(n[2 * p], n[2 * p + 1], c[2 * p], s[2 * p]);
-            o[2 * p + 1] = (bf16)k2_rot_im(n[2 * p], n[2 * p + 1], c[2 * p + 1], s[2 * p + 1]);
+            o[2 * p] = (bf16)k2_rot_re(p, n[2 * p], n[2 * p + 1], c[2 * p], s[2 * p]);
+            o[2 * p + 1] = (bf16)k2_rot_im(p, n[2 * p], n[2 * p + 1], c[2 * p + 1], s[2 * p + 1]);
         }
     } else {
 #pragma unroll
