@@ -411,6 +411,7 @@ __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(const float* __res
 bool aligned2(const void* p) { return ((uintptr_t)p & 1) == 0; }
 
 constexpr int MOST_COLS = 1 << 28;   // 32-bit columns, and a launch's lanes below 2^32 (rmsnorm_dweight_kernel: 8 a column)
+constexpr int MOST = 1 << 21;        // rows of a launch with a workgroup per row: its lanes have to stay below 2^32
 constexpr int REG_COLS = 65536;      // the longest row that is held in registers (1024 lanes, 8 chunks each)
 // Lanes per row: a wave where half of a workgroup's would have nothing to do and the rows alone fill the chip, else a workgroup
 // (us, wave / workgroup: 20000 x 1024 29 / 34; 19385 x 4096 118 / 114; 1 x 4096 4.4 / 2.6), of 1024 lanes where 256 would hold
@@ -463,7 +464,6 @@ int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, co
     FP_REQUIRE(!Q8 || (q_scale && ((uintptr_t)q_scale & 3) == 0));
     if (rows == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
-    constexpr int MOST = 1 << 21;      // rows a launch: its lanes have to stay below 2^32
     for (int64_t r = 0; r < rows; r += MOST) {
         // (y_rs counts bytes where y is e4m3)
         T* yr = Q8 ? (T*)((unsigned char*)y + r * y_rs) : (T*)y + r * y_rs;
@@ -478,7 +478,7 @@ int norm_launch(const void* x, int64_t x_rs, const void* resid, int64_t r_rs, co
 template <typename T>
 int grad_launch(const void* dy, int64_t dy_rs, const void* h, int64_t h_rs, const void* dh, int64_t dh_rs, const void* w,
                 void* dx, int64_t dx_rs, void* dw, int rows, int cols, float eps, void* ws, int64_t ws_bytes, void* stream) {
-    FP_REQUIRE(cols <= MOST_COLS && (cols <= GRAD_COLS || rows <= 1 << 21));           // (a workgroup per row there)
+    FP_REQUIRE(cols <= MOST_COLS);
     FP_REQUIRE(dy && h && w && dx && dw && rows > 0 && cols > 0 && dy_rs >= 0 && h_rs >= 0 && dx_rs >= cols && eps >= 0.f);
     FP_REQUIRE(!dh || dh_rs >= 0);
     FP_REQUIRE(aligned2(dy) && aligned2(h) && aligned2(dh) && aligned2(w) && aligned2(dx) && aligned2(dw));
@@ -487,21 +487,26 @@ int grad_launch(const void* dy, int64_t dy_rs, const void* h, int64_t h_rs, cons
     const int parts = grad_parts(rows, cols);
     float* part = (float*)ws;
     float* rstd = part + (int64_t)parts * ((cols + 7) & ~7);
-#define FP_GRAD(TPR, NCH, AHEAD, DW, GRID, PART)                                                                        \
-    rmsnorm_grad_kernel<T, TPR, NCH, AHEAD, DW><<<dim3((unsigned)(GRID)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(        \
-        (const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh, dh_rs, (const T*)w, (T*)dx, dx_rs, PART, rows, cols, eps)
+#define FP_GRAD(TPR, NCH, AHEAD, DW, GRID, R, N, PART)                                                                            \
+    rmsnorm_grad_kernel<T, TPR, NCH, AHEAD, DW><<<dim3((unsigned)(GRID)), dim3(TPR < 256 ? 256 : TPR), 0, st>>>(                  \
+        (const T*)dy + (R) * dy_rs, dy_rs, (const T*)h + (R) * h_rs, h_rs, dh ? (const T*)dh + (R) * dh_rs : nullptr, dh_rs,      \
+        (const T*)w, (T*)dx + (R) * dx_rs, dx_rs, PART, N, cols, eps)
     const int nch = (cols + 7) / 8;
-    if (nch <= 64) FP_GRAD(64, 1, true, true, parts, part);
-    else if (nch <= 128) FP_GRAD(64, 2, true, true, parts, part);
-    else if (nch <= 256) FP_GRAD(256, 1, true, true, parts, part);
-    else if (nch <= 512) FP_GRAD(256, 2, true, true, parts, part);
-    else if (nch <= 1024) FP_GRAD(256, 4, true, true, parts, part);
-    else if (nch <= 2048) FP_GRAD(512, 4, false, true, parts, part);
+    if (nch <= 64) FP_GRAD(64, 1, true, true, parts, 0, rows, part);
+    else if (nch <= 128) FP_GRAD(64, 2, true, true, parts, 0, rows, part);
+    else if (nch <= 256) FP_GRAD(256, 1, true, true, parts, 0, rows, part);
+    else if (nch <= 512) FP_GRAD(256, 2, true, true, parts, 0, rows, part);
+    else if (nch <= 1024) FP_GRAD(256, 4, true, true, parts, 0, rows, part);
+    else if (nch <= 2048) FP_GRAD(512, 4, false, true, parts, 0, rows, part);
     else {
-        if (nch <= 4096) FP_GRAD(1024, 4, false, false, rows, rstd);
-        else rmsnorm_grad_rows_kernel<T><<<dim3((unsigned)rows), dim3(256), 0, st>>>((const T*)dy, dy_rs, (const T*)h, h_rs, (const T*)dh,
-                                                                                    dh_rs, (const T*)w, (T*)dx, dx_rs, rstd, cols, eps);
-        FP_CHECK_LAUNCH();
+        for (int64_t r = 0; r < rows; r += MOST) {
+            const int n = rows - r < MOST ? (int)(rows - r) : MOST;
+            if (nch <= 4096) FP_GRAD(1024, 4, false, false, n, r, n, rstd + r);
+            else rmsnorm_grad_rows_kernel<T><<<dim3((unsigned)n), dim3(256), 0, st>>>(
+                (const T*)dy + r * dy_rs, dy_rs, (const T*)h + r * h_rs, h_rs, dh ? (const T*)dh + r * dh_rs : nullptr, dh_rs,
+                (const T*)w, (T*)dx + r * dx_rs, dx_rs, rstd + r, cols, eps);
+            FP_CHECK_LAUNCH();
+        }
         rmsnorm_dweight_rows_kernel<T><<<dim3((unsigned)((nch + 255) / 256), (unsigned)parts), dim3(256), 0, st>>>(
             (const T*)dy, dy_rs, (const T*)h, h_rs, rstd, part, rows, cols);
     }

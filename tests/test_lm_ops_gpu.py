@@ -746,3 +746,24 @@ def test_gated_ff_gradient_of_more_weights_than_a_launch_adds_up():
         a, b = wg[:, at].double(), wu[:, at].double()
         want = dg @ a + du @ b
         within(dx[:, at], want, want.abs() * u_of(BF) + (ug + n * dg.abs()) @ a.abs() + (uu + n * du.abs()) @ b.abs(), "dx")
+
+
+def test_norm_gradient_of_more_wide_rows_than_a_launch_takes():
+    rows, cols, step = (1 << 21) + 5, 16392, 8             # dx 69 GB; the inputs' rows overlap each other, 8 values apart
+    g = torch.Generator(DEV).manual_seed(1)
+    one, two = (torch.randn(rows * step + cols, generator=g, device=DEV).to(BF) for _ in range(2))
+    two[step << 21:] *= 1000                               # the rows behind the first launch's count
+    h, dy = (t.as_strided((rows, cols), (step, 1)) for t in (one, two))
+    w = (1 + randn(cols, seed=3, scale=0.3)).to(BF)
+    dx, dw = ops.rmsnorm_residual_backward(dy, h, w)
+    for a in (0, (1 << 21) - 4, rows - 7):
+        s = slice(a, a + 7)
+        dx64, _, tx, _ = norm_grad64(dy[s], h[s], w, None)
+        within(dx[s], dx64, dx64.abs() * u_of(BF) + tx * (cols + 16) * E32 * 2, "dx")
+    del dx
+    sq = torch.cat([torch.zeros(1, device=DEV, dtype=torch.float64), one.double().square().cumsum(0)])
+    r = 1 / torch.sqrt((sq[cols::step][:rows] - sq[:-cols:step][:rows]) / cols + EPS)
+    at = torch.arange(0, 40, device=DEV)                   # columns in which only the last rows see the factor
+    want = (torch.stack([two[c:c + rows * step:step].double() * one[c:c + rows * step:step].double() for c in at.tolist()], 1) * r[:, None]).sum(0)
+    # 32-bit sums of 2^15 terms a part err by far less than the last rounding does
+    assert rel_l2(dw[at], want) < 1.0 * u_of(BF)
