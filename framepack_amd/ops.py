@@ -885,6 +885,9 @@ def _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, dtypes, bias_dtype):
     u2, _, _, ldu = _mat(w_up, "w_up", (x.dtype,), F, K)
     if F == 0:
         raise ValueError("w_gate: expected at least one row")
+    for name, ld in (("w_gate", ldg), ("w_up", ldu)):
+        if ld < K:
+            raise ValueError(f"{name}: rows of {K} values overlap at a row stride of {ld}")
     if act not in (ACT_SILU, ACT_GELU):
         raise ValueError(f"act: expected ACT_SILU or ACT_GELU, got {act!r}")
     if (b_gate is None) != (b_up is None):

@@ -204,8 +204,8 @@ int fp_gemm_fp8_bf16(const void* a, int64_t lda, const void* a_scale, const void
 
 /* ---- K12, K13: a language model's pre-norm and gated feed-forward block (no counterpart in the reference) ---------
  * Pointers need their type's alignment only and strides and sizes are free unless noted; 16-byte aligned pointers with
- * strides and sizes of multiples of 8 elements take the wide paths.  Input rows may repeat (stride 0); output rows must
- * not overlap.  `dtype` suffix: the type of every matrix and vector of the call unless noted. */
+ * strides and sizes of multiples of 8 elements take the wide paths.  Input rows may repeat (stride 0) or overlap, but for the
+ * gated block's weights, whose row strides are at least K; output rows must not overlap.  `dtype` suffix: the type of every matrix and vector of the call unless noted. */
 
 /* K12  h = resid + x;  y = h / sqrt(mean(h^2) + eps) * weight,  x, resid, y, h: [rows, cols], weight: [cols].
  * The norm is taken of the 32-bit sum, h receives it rounded.  resid and h may both be NULL: h = x, nothing but y is

@@ -225,3 +225,24 @@ def test_fragment_reads_of_the_gated_blocks_products_all_feed_an_mfma(tmp_path):
             assert int(re.search(re.escape(name) + r"\.num_vgpr, (\d+)", text).group(1)) <= 256
             assert int(re.search(re.escape(name) + r"\.private_seg_size, (\d+)", text).group(1)) == 0
     assert seen >= 16 and transposing > 0
+
+
+def test_weights_with_overlapping_rows_are_refused_by_name(no_device_check):
+    x, w, one = torch.zeros(4, 64, dtype=BF), torch.zeros(16, 64, dtype=BF), torch.zeros(1, 64, dtype=BF).expand(16, 64)
+    near = torch.zeros(16 * 63 + 64, dtype=BF).as_strided((16, 64), (63, 1))
+    g = torch.zeros(4, 16, dtype=BF)
+    x8, w8, s4, s16 = torch.zeros(4, 128, dtype=ops.FP8), torch.zeros(16, 128, dtype=ops.FP8), torch.ones(4), torch.ones(16)
+    one8 = w8[:1].expand(16, 128)
+    for call, name in ((lambda: ops.gated_ff(x, one, w), "w_gate"), (lambda: ops.gated_ff(x, w, near), "w_up"),
+                       (lambda: ops.gated_ff_fp8(x8, s4, one8, s16, w8, s16), "w_gate"),
+                       (lambda: ops.gated_ff_backward(g, x, w, one, g, g), "w_up"),
+                       (lambda: ops.gated_ff_backward(g, x, near, w, g, g), "w_gate")):
+        with pytest.raises(ValueError, match=name + ": rows of .* overlap"):
+            call()
+
+
+def test_the_library_refuses_weights_with_overlapping_rows():
+    L, p, F, K = fplib.load(), 1 << 20, 16, 128
+    for ld in (0, K - 1):
+        assert L.fp_gated_ff_bf16(p, K, p, ld, p, K, None, None, p, F, None, None, 0, 4, F, K, 0, None, 0, None) == 1
+        assert L.fp_gated_ff_backward_bf16(p, F, p, K, p, K, p, ld, p, F, p, F, p, p, None, 4, F, K, 0, p, 1 << 30, None) == 1
