@@ -89,8 +89,9 @@ __device__ __forceinline__ float row_max(float v, float* red) {
 
 // TPR lanes per row (64: four rows a workgroup), the row in registers (NCH chunks of 8 a lane) between the sum of squares
 // and the write: one read of x and resid, one write of y and h.  The sum h is held in 32 bits for the norm and rounded
-// once where it is stored.  (y and h may lie on x and resid: those four are not __restrict__; a lane has read all its
-// elements of the row before it writes one, and no other lane reads them.)
+// once where it is stored.  (y and h may lie on x and resid: those four are not __restrict__.  A lane has read its own elements
+// before it writes them.  The lane with the row's partial last chunk also reads up to 7 elements in front of its own, as load8
+// does; their lane, of another wave perhaps, may have overwritten them by then, and `fit` drops them before anything uses them.)
 template <typename T, bool Q8, int TPR, int NCH>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_kernel(const T* x, int64_t x_rs, const T* resid, int64_t r_rs,
                                                                         const T* __restrict__ w, T* y, int64_t y_rs,
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(const T* x, int64_t x
 // of its columns in registers over all of them and leaves one partial row of it: one read of dy, h and dh, one write of dx.
 // DW = false (longer rows, whose share of dweight does not fit the registers as well): the row's r is left in part[row].
 // AHEAD: the next row is loaded before the current one's sums, so that the loads of two rows are in flight at every barrier
-// (where the registers hold them).
+// (where the registers hold them).  dx may lie on dh: what holds for rmsnorm_kernel's partial last chunk holds for dh's here.
 template <typename T, int TPR, int NCH, bool AHEAD, bool DW>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rmsnorm_grad_kernel(const T* __restrict__ dy, int64_t dy_rs, const T* __restrict__ h,
                                                                              int64_t h_rs, const T* dh, int64_t dh_rs,

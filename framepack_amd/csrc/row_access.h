@@ -6,6 +6,8 @@
 // (unaligned accesses are on for global memory on this target), so rows of any stride and length take it.  A row's partial
 // last chunk is read as its last 8 elements and moved into place by `fit` where it is used, so that the load itself is one
 // instruction that nothing waits for (as seven conditional loads it cost a row of 4095 columns a third of its time).
+// The elements in front of the chunk's own may be written by another lane meanwhile where an output lies on the row: a chunk is not
+// used before `fit` has dropped them.
 template <typename T> struct vec8;
 template <> struct vec8<bf16> { typedef bf16x8 type; };
 template <> struct vec8<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8))); };

@@ -767,3 +767,28 @@ def test_norm_gradient_of_more_wide_rows_than_a_launch_takes():
     want = (torch.stack([two[c:c + rows * step:step].double() * one[c:c + rows * step:step].double() for c in at.tolist()], 1) * r[:, None]).sum(0)
     # 32-bit sums of 2^15 terms a part err by far less than the last rounding does
     assert rel_l2(dw[at], want) < 1.0 * u_of(BF)
+
+
+# widths whose partial last chunk begins a wave, so that another wave owns (and in place overwrites) the values in front of it
+@pytest.mark.parametrize("cols", [1537, 2561, 8705, 16897, 33281])
+def test_ragged_rows_in_place(cols):
+    rows = 4100 if cols < 10000 else 300                    # several rows a workgroup in the gradient
+    x, r, dy = (randn(rows, cols, seed=i, dtype=BF) for i in (1, 2, 3))
+    w = (1 + randn(cols, seed=4, scale=0.3)).to(BF)
+    y, h = ops.rmsnorm_residual(x, w, r)
+    dx, dw = ops.rmsnorm_residual_backward(dy, h, w, dh=r)
+    for _ in range(3):
+        a, b = x.clone(), r.clone()
+        ops.rmsnorm_residual(a, w, b, out=a, resid_out=b)
+        assert torch.equal(a, y) and torch.equal(b, h)
+        a, b = x.clone(), r.clone()
+        ops.rmsnorm_residual(a, w, b, out=b, resid_out=a)
+        assert torch.equal(b, y) and torch.equal(a, h)
+        d = r.clone()
+        assert torch.equal(ops.rmsnorm_residual_backward(dy, h, w, dh=d, dx=d)[1], dw) and torch.equal(d, dx)
+    for at in (0, rows - 20):
+        s = slice(at, at + 20)
+        h64, y64 = norm64(x[s], r[s], w)
+        within(y[s], y64, norm_tol(y64, BF, cols))
+        dx64, _, tx, _ = norm_grad64(dy[s], h[s], w, r[s])
+        within(dx[s], dx64, dx64.abs() * u_of(BF) + tx * (cols + 16) * E32 * 2, "dx")
