@@ -792,3 +792,26 @@ def test_ragged_rows_in_place(cols):
         within(y[s], y64, norm_tol(y64, BF, cols))
         dx64, _, tx, _ = norm_grad64(dy[s], h[s], w, r[s])
         within(dx[s], dx64, dx64.abs() * u_of(BF) + tx * (cols + 16) * E32 * 2, "dx")
+
+
+# weights of more than 2^31 values: copied into rows (an odd width), and read as they lie but for the last 24 rows.  dx rounds twice
+# (dg and du, then itself), each of relative rms at most u / sqrt(3); its 32-bit sums err by far less.
+@pytest.mark.parametrize("K", [16385, 16384])
+def test_gated_ff_gradient_reads_weights_past_two_to_the_31(K):
+    M, F = 2, (1 << 17) + 24
+    dh, x = randn(M, F, seed=1, dtype=BF), randn(M, K, seed=2, dtype=BF)
+    g, u = randn(M, F, seed=5, scale=2.0, dtype=BF), randn(M, F, seed=6, dtype=BF)
+    gen = torch.Generator(DEV).manual_seed(3)
+    wg, wu = (torch.empty(F, K, dtype=BF, device=DEV).normal_(generator=gen) for _ in range(2))
+    dx, dwg, dwu, _, _ = ops.gated_ff_backward(dh, x, wg, wu, g, u)
+    dg, du = ff_grad64(dh, x, wg[:1], wu[:1], g, u, ops.ACT_SILU)[:2]
+    at = torch.cat([torch.arange(0, 40), torch.arange(K // 2, K // 2 + 40), torch.arange(K - 40, K)]).to(DEV)
+    a, b = wg[:, at].double(), wu[:, at].double()
+    want = dg @ a + du @ b
+    assert rel_l2(dx[:, at], want) < 1.0 * u_of(BF)
+    # the bound sees any of these: nothing at all, one projection alone, a last K tile of 24 rows left out
+    for wrong in (0 * want, dg @ a, du @ b, want - dg[:, -24:] @ a[-24:], want - du[:, -24:] @ b[-24:]):
+        assert rel_l2(wrong, want) > 1.5 * u_of(BF)
+    for d, o in ((dg, dwg), (du, dwu)):
+        for rows in (slice(0, 200), slice(F // 2, F // 2 + 200), slice(F - 200, F)):
+            assert rel_l2(o[rows], d[:, rows].t() @ x.double()) < 1.0 * u_of(BF)
