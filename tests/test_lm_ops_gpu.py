@@ -815,3 +815,33 @@ def test_gated_ff_gradient_reads_weights_past_two_to_the_31(K):
     for d, o in ((dg, dwg), (du, dwu)):
         for rows in (slice(0, 200), slice(F // 2, F // 2 + 200), slice(F - 200, F)):
             assert rel_l2(o[rows], d[:, rows].t() @ x.double()) < 1.0 * u_of(BF)
+
+
+def test_sums_over_rows_past_four_gigabytes():
+    rows, cols, F, far = 140000, 16384, 64, 131072          # row `far` begins 2^31 elements, 2^32 bytes behind the first
+    base, grad = randn(64, cols, seed=1, dtype=BF), randn(64, cols, seed=2, dtype=BF)
+    x = base.repeat(rows // 64 + 1, 1)[:rows]
+    dy = grad.repeat(rows // 64 + 1, 1)[:rows]
+    x[far:] *= 4                                           # (the rows repeat every 64: these would not be told apart)
+    dy[far:] *= 4
+    w = (1 + randn(cols, seed=3, scale=0.3)).to(BF)
+    _, dw = ops.rmsnorm_residual_backward(dy, x, w)
+    n = torch.stack([((t := f * base.double()) / torch.sqrt((t * t).mean(1, keepdim=True) + EPS)) * f for f in (1.0, 4.0)])
+    per = torch.bincount(torch.arange(rows, device=DEV) % 64 + (torch.arange(rows, device=DEV) >= far) * 64).double().view(2, 64, 1)
+    want = (n * per * grad.double()).sum((0, 1))
+    # parts of 547 rows are added up in 32 bits: 547 2^-24 of the sum of |terms|, six times the sum; then one rounding
+    assert rel_l2(dw, want) < 1.0 * u_of(BF)
+    assert rel_l2((n[:1] * per[:1] * grad.double()).sum((0, 1)), want) > 10 * u_of(BF)          # (the far rows count)
+    del dy
+    dh, g, u = randn(rows, F, seed=4, dtype=BF), randn(rows, F, seed=5, dtype=BF), randn(rows, F, seed=6, dtype=BF)
+    wg = randn(F, cols, seed=7, scale=cols ** -0.5, dtype=BF)
+    _, dwg, dwu, dbg, dbu = ops.gated_ff_backward(dh, x, wg, wg, g, u, bias=True)
+    dg, du = ff_grad64(dh, x[:1], wg, wg, g, u, ops.ACT_SILU)[:2]
+    for at in (slice(0, 128), slice(cols - 128, cols)):
+        xs = x[:, at].double()
+        for d, o in ((dg, dwg), (du, dwu)):
+            want = d.t() @ xs
+            assert rel_l2(o[:, at], want) < 1.0 * u_of(BF)
+            assert rel_l2(d[:far].t() @ xs[:far], want) > 10 * u_of(BF)
+    for d, o in ((dg, dbg), (du, dbu)):
+        assert rel_l2(o, d.sum(0)) < 1.0 * u_of(BF)
