@@ -845,3 +845,14 @@ def test_sums_over_rows_past_four_gigabytes():
             assert rel_l2(d[:far].t() @ xs[:far], want) > 10 * u_of(BF)
     for d, o in ((dg, dbg), (du, dbu)):
         assert rel_l2(o, d.sum(0)) < 1.0 * u_of(BF)
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 72), (33, 1152), (7, 1001), (257, 4096), (3, 5003), (2, 20000), (2, 70000)])
+def test_norm_to_8_bits_into_strided_rows_gives_the_same_bytes(rows, cols):
+    x, r, w = randn(rows, cols, seed=1, dtype=BF), randn(rows, cols, seed=2, dtype=BF), randn(cols, seed=3, dtype=BF)
+    q, s, h = ops.rmsnorm_residual_fp8(x, w, r)
+    for left, right in ((16, 16), (5, 6)):
+        out = torch.zeros(rows, left + cols + right, dtype=torch.uint8, device=DEV).view(ops.FP8)[:, left:left + cols]
+        q2, s2, h2 = ops.rmsnorm_residual_fp8(embed(x, left, right)[0], w, embed(r, left, right)[0], out=out)
+        assert q2.data_ptr() == out.data_ptr() and torch.equal(q2.contiguous().view(torch.uint8), q.view(torch.uint8))
+        assert torch.equal(s2, s) and torch.equal(h2, h)
