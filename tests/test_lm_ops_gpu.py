@@ -856,3 +856,40 @@ def test_norm_to_8_bits_into_strided_rows_gives_the_same_bytes(rows, cols):
         q2, s2, h2 = ops.rmsnorm_residual_fp8(embed(x, left, right)[0], w, embed(r, left, right)[0], out=out)
         assert q2.data_ptr() == out.data_ptr() and torch.equal(q2.contiguous().view(torch.uint8), q.view(torch.uint8))
         assert torch.equal(s2, s) and torch.equal(h2, h)
+
+
+# One rounding of relative rms at most u / sqrt(3), and sums that err by a hundredth of that or less: a bound in norm, and one on
+# how many values are not the type's nearest.  An error of e before the rounding moves a value to its neighbour with probability
+# 2 e / ulp, ulp >= u of the value.  e: 32-bit sums of K / 32 steps and the activation's exponential, 2^-21 of a value of ordinary
+# size (K <= 4096); the matrix instructions for e4m3 drop what lies 2^13 below the largest of eight products, 2^-15 of such a
+# value; ten times as much for the values that are small by cancellation.
+def off_nearest(got, want, dtype):
+    return (got != want.to(dtype)).double().mean().item()
+
+
+FF_NORM_SHAPES = [(1, 4096, 1024), (16, 1040, 512), (33, 264, 520), (40, 72, 2048), (48, 8208, 256), (64, 520, 256), (129, 256, 640),
+                  (300, 136, 4096), (300, 1000, 1152), (600, 8192, 256)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("M,F,K", FF_NORM_SHAPES)
+def test_gated_ff_in_norm(M, F, K, dtype):
+    x, wg, wu = randn(M, K, seed=1, dtype=dtype), randn(F, K, seed=2, scale=2 * K ** -0.5, dtype=dtype), randn(F, K, seed=3, scale=K ** -0.5, dtype=dtype)
+    for act in (ops.ACT_SILU, ops.ACT_GELU):
+        h64, g, u, _, _ = ff64(x, wg, wu, None, None, act)
+        got = ops.gated_ff(x, wg, wu, act=act, keep=True)
+        for o, want in zip(got, (h64, g, u)):
+            assert rel_l2(o, want) < 0.6 * u_of(dtype)
+            assert off_nearest(o, want, dtype) < 10 * 2 * 2.0 ** -21 / u_of(dtype)
+
+
+@pytest.mark.parametrize("M,F,K", [(m, f, k) for m, f, k in FF_NORM_SHAPES if k % 128 == 0])
+def test_gated_ff_in_8_bits_in_norm(M, F, K):
+    x, xs = ops.quantize_rows_fp8(randn(M, K, seed=1, dtype=BF))
+    (wg, gs), (wu, us) = quantised(randn(F, K, seed=2, scale=2 * K ** -0.5)), quantised(randn(F, K, seed=3, scale=K ** -0.5))
+    deq = [q.double() * s.double()[:, None] for q, s in ((x, xs), (wg, gs), (wu, us))]
+    for act in (ops.ACT_SILU, ops.ACT_GELU):
+        h64 = ff64(*deq, None, None, act)[0]
+        h = ops.gated_ff_fp8(x, xs, wg, gs, wu, us, act=act)
+        assert rel_l2(h, h64) < 0.6 * u_of(BF)
+        assert off_nearest(h, h64, BF) < 10 * 2 * 2.0 ** -15 / u_of(BF)
