@@ -928,7 +928,8 @@ def gated_ff_fp8(x_q: torch.Tensor, x_scale: torch.Tensor, wg_q: torch.Tensor, w
     """K13 on e4m3 operands: bf16 h = act(g) * u with g = x_scale[m] * wg_scale[n] * (x_q @ wg_q.T) + b_gate and u alike.
     x_q [M, K] with x_scale [M] as `rmsnorm_residual_fp8` and `quantize_rows_fp8` return them, weights [inner, K] with
     scales [inner] as `quantize_weight_fp8` prepares them; biases bf16.  K a multiple of 128, inner of 8, all 16-byte
-    aligned, matrices with row strides of multiples of 16, as `gemm_fp8`."""
+    aligned, matrices with row strides of multiples of 16, as `gemm_fp8`.  As there, the fp8 matrix instructions drop what lies
+    2^13 below the largest of eight neighbouring products: sums are good to some 2^-16 of their size."""
     _dev(x_q, x_scale, wg_q, wg_scale, wu_q, wu_scale, b_gate, b_up, out)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x_q, wg_q, wu_q, b_gate, b_up, act, (FP8,), BF16)
     xs, gs, us = (_vec(t, n, torch.float32, k) for t, n, k in ((x_scale, "x_scale", M), (wg_scale, "wg_scale", F),

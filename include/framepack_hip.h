@@ -257,7 +257,9 @@ int fp_gated_ff_f16(const void* x, int64_t ldx, const void* w_gate, int64_t ldwg
                     int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* K13 on e4m3 operands: g = x_scale[m] * wg_scale[n] * (x . w_gate^T) + b_gate and u alike; h and the biases bf16, the
- * scales fp32.  K % 128 == 0, F % 8 == 0, the matrices 16-byte aligned with row strides of multiples of 16 elements
+ * scales fp32.  The matrix instructions cut the products x w, towards zero, at 2^-13 of the largest of eight neighbours (k = 8 i
+ * .. 8 i + 7) before they are added in 32 bits: g and u are off by up to 7 2^-13 of that for every eight, 2^-16 of their size where
+ * the values are normally distributed.  K % 128 == 0, F % 8 == 0, the matrices 16-byte aligned with row strides of multiples of 16 elements
  * (h: of 8), scales and biases 16-byte aligned; x's and the weights' row strides below 2^22.  workspace:
  * fp_gated_ff_fp8_workspace_bytes(M, F, K) bytes, 16-byte aligned, or NULL where that is 0. */
 int64_t fp_gated_ff_fp8_workspace_bytes(int M, int F, int K);

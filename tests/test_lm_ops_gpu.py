@@ -893,3 +893,21 @@ def test_gated_ff_in_8_bits_in_norm(M, F, K):
         h = ops.gated_ff_fp8(x, xs, wg, gs, wu, us, act=act)
         assert rel_l2(h, h64) < 0.6 * u_of(BF)
         assert off_nearest(h, h64, BF) < 10 * 2 * 2.0 ** -15 / u_of(BF)
+
+
+# e4m3 products are cut, towards zero, at 2^-13 of the binade of the largest of eight neighbours (k = 8 i .. 8 i + 7): an error of
+# up to 7 2^-13 of it for every eight, beside the 32-bit sums'
+@pytest.mark.parametrize("M", [3, 40, 70])
+def test_gated_ff_in_8_bits_of_products_that_cancel(M):
+    K, F = 1024, 8
+    big = torch.arange(K, device=DEV) % 8 == 0
+    x = torch.where(big, 16.0, 0.234375).expand(M, K).contiguous()
+    wu = torch.where(big, 16.0 - 32.0 * (torch.arange(K, device=DEV) // 8 % 2), 0.234375).expand(F, K).contiguous()
+    wg = torch.zeros(F, K, device=DEV)
+    wg[:, 0] = 4.0                                         # g = 64: act(g) = 64 in 32 bits
+    h64, _, u, _, eu = ff64(x, wg, wu, None, None, ops.ACT_SILU)
+    cut = 7 * 2.0 ** -13 * 256 * (K / 8)
+    one = torch.ones(max(M, F), device=DEV)
+    h = ops.gated_ff_fp8(x.to(ops.FP8), one[:M], wg.to(ops.FP8), one[:F], wu.to(ops.FP8), one[:F])
+    within(h, h64, h64.abs() * u_of(BF) + 64 * (cut + eu) * (1 + u_of(BF)))
+    assert cut < u.min()                                   # (the sum of what is small is seen)
