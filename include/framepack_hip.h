@@ -267,7 +267,8 @@ int fp_gated_ff_fp8(const void* x, int64_t ldx, const void* x_scale, const void*
                     const void* w_up, int64_t ldwu, const void* wu_scale, const void* b_gate, const void* b_up, void* h,
                     int64_t ldh, int M, int F, int K, int act, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Gradient of K13 from dh and the kept g and u:  dg = dh u act'(g), du = dh act(g) (rounded to the type), then
+/* Gradient of K13 from dh and the kept g and u:  dg = dh u act'(g), du = dh act(g) (computed in fp32, rounded to the type: in f16
+ * infinite past 65504), then
  *   dx = dg . w_gate + du . w_up [M, K];  dw [2 F, K] = dg^T . x over du^T . x;  db [2 F] (or NULL) = column sums of dg, du.
  * The outputs are contiguous, dx and dw 16-byte aligned.  M > 0; M, F, K <= 2^20 - 64.  Sums in fp32 in a fixed order.
  * workspace: fp_gated_ff_backward_workspace_bytes(...) bytes for these operands, 16-byte aligned. */
