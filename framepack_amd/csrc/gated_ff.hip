@@ -9,14 +9,16 @@
 // tiles, by the operands' way into LDS).  The gradient: one element-wise pass that writes dg | du as rows and as columns (HBM),
 // then two products on the same tile, which read Wg, Wu and x as they lie.  A large copy runs at 4.9 TB/s on this card, a large
 // product at 1440 TFLOP/s in bf16 and 2370 in e4m3.  Measured, [K, F], us:
-//   1 row, [4096, 14336], bf16           44      5.4 TB/s of weights
-//   16 rows, the same, e4m3              24      4.9 TB/s
-//   64 - 256 rows, the same, bf16        63 - 75 3.7 - 3.1 TB/s (128 bytes of a row a K tile)
+//   1 row, [4096, 14336], bf16           44      5.3 TB/s of weights
+//   16 rows, the same, e4m3              23      5.2 TB/s
+//   64 - 256 rows, the same, bf16        59 - 67 4.0 - 3.5 TB/s (128 bytes of a row a K tile)
 //   729 rows, [1152, 4304], f16          22      (204 tiles on 256 CUs; 10 of it first loads and epilogue)
 //   4096 rows, [4096, 14336], e4m3       388     2480 TFLOP/s
-//   19385 rows, [4096, 14336], bf16      3230    1410 TFLOP/s (matrix pipe 78 % busy at 1.74 GHz)
-//   gradient, 729 rows, [1152, 4304]     60      element-wise 15, products 40, parts 5
-//   gradient, 4096 rows, [4096, 11008]   1185    element-wise 108 (5.8 TB/s), products 2 x 535 (1380 TFLOP/s)
+//   19385 rows, [4096, 14336], bf16      3190    1430 TFLOP/s (matrix pipe 78 % busy at 1.82 GHz)
+//   gradient, 729 rows, [1152, 4304]     61      element-wise 14.5, products 41, parts 5
+//   gradient, 4096 rows, [4096, 11008]   1185    element-wise 109 (5.8 TB/s), products 2 x 535 (1380 TFLOP/s)
+// (calls one after the other for half a second, by when the clock has settled: the first some twenty of the long ones after a pause
+// take up to a fifth more or less.)
 #include <algorithm>
 #include <type_traits>
 #include "gated_ff.h"
@@ -501,8 +503,15 @@ Pair pair(int M, int F, int K) {
     return best;
 }
 
-// Rows up to which the weights are streamed (glu_few_kernel).  [K, F] = [4096, 14336], streamed / matrix-core kernel, us:
-// bf16 45 / 70 at 1 row, 56 / 69 at 32, 64 / 71 at 48, 70 / 73 at 64; e4m3 21 / 30 at 1, 32 / 34 at 48, 37 / 35 at 64.
+// Rows up to which the weights are streamed (glu_few_kernel).  Streamed / matrix-core kernel, us, at 16, 32, 48 and 64 rows (64: with
+// a fourth token tile, which is not built):
+//   [K, F]         bf16                                          e4m3
+//   [1152, 4304]   9.2 / 15   11.2 / 15   13.4 / 15   16 / 16    6.6 / 12   7.9 / 12   9.1 / 12   11 / 13
+//   [2048, 5504]   15 / 18    17.6 / 19   21.5 / 19   26 / 20    8.8 / 17   10.7 / 18  13 / 18    15 / 19
+//   [4096, 4096]   15 / 26    18.5 / 25   22 / 26     26 / 27    12 / 17    13 / 17    14 / 18    16 / 18
+//   [4096, 11008]  48 / 51    53 / 52     60 / 53     69 / 53    23 / 30    27 / 32    33 / 32    37 / 33
+//   [4096, 14336]  48 / 60    53 / 58     62 / 58     94 / 59    25 / 34    28 / 33    34 / 34    47 / 34
+// One number for all: within 1 - 13 % of the better form at 33 - 48 rows in 16 bits, ahead of it or level in 8.
 constexpr int FEW = 48;
 constexpr int64_t FAR = int64_t(1) << 22;   // gemm_w4.h: 32-bit offsets within a tile
 constexpr int MOST_F = 1 << 27;             // glu_few_kernel's lanes, 16 a column, have to stay below 2^32

@@ -157,7 +157,7 @@ struct Rows2 {
 // are accumulators of one lane (column tiles ni and ni + NT / 2) and the epilogue multiplies them in registers; the output
 // tile is 256 x (16 NT).  A wave stages its LDS rows from one of the two matrices only (wave & 1), whose base and row
 // stride stay in scalar registers: the main loop is the dense one.  KEEP: both projections are written out as well.
-// 19385 rows, [4096, 14336] in bf16: 3.23 ms, 1410 TFLOP/s; the largest dense products run at 1440 (figures: gated_ff.hip).
+// 19385 rows, [4096, 14336] in bf16: 3.19 ms, 1430 TFLOP/s; the largest dense products run at 1440 (figures: gated_ff.hip).
 struct GluArgs {
     const void *w2, *bias2;
     int64_t ldw2;

@@ -804,7 +804,8 @@ def rmsnorm_residual(x: torch.Tensor, weight: torch.Tensor, resid: Optional[torc
                      out: Optional[torch.Tensor] = None, resid_out: Optional[torch.Tensor] = None):
     """K12: h = resid + x, out = h / sqrt(mean(h^2) + eps) * weight; returns (out, h).  Without resid, h is x itself.
     x, resid [rows, cols] (row-strided ok, any cols), weight [cols], one type: bf16 or f16.  The norm is taken of the
-    32-bit sum; h is that sum rounded to the type.  out and resid_out may each be x or resid itself."""
+    32-bit sum; h is that sum rounded to the type.  out and resid_out may each be x or resid itself (without resid, out = x overwrites
+    the h that the gradient takes).  No autograd graph is recorded: the gradient is `rmsnorm_residual_backward`."""
     x2, rows, cols, xs, w, r2, rs, h, h2, hs = _rmsnorm_args(x, weight, resid, resid_out, (BF16, F16), eps)
     y, y2, ys = _out(out, "out", x.dtype, rows, cols, x, x2 is x and x.is_contiguous())
     if out is not None or resid_out is not None:
@@ -901,9 +902,9 @@ def gated_ff(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: 
              b_up: Optional[torch.Tensor] = None, act: int = ACT_SILU, out: Optional[torch.Tensor] = None, keep: bool = False):
     """K13: h = act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up) in one kernel, act = ACT_SILU or ACT_GELU; returns h
     [M, inner], with keep (h, gate, up): the two projections before the activation, as `gated_ff_backward` takes them.
-    x [M, K], w_gate, w_up [inner, K] (nn.Linear layout; row-strided ok, slices of one fused weight too), any sizes (K
-    below 2^20 for more than 48 rows); one type, bf16 or f16.  The block's second linear is `gemm`, with the residual in its
-    epilogue (EPI_RESIDUAL)."""
+    x [M, K], w_gate, w_up [inner, K] (nn.Linear layout; row-strided ok, slices of one fused weight too), any sizes (inner up
+    to 2^27; K up to 2^20 - 64 for more than 48 rows); one type, bf16 or f16.  The block's second linear is `gemm`, with the
+    residual in its epilogue (EPI_RESIDUAL).  No autograd graph is recorded: the gradient is `gated_ff_backward`."""
     _dev(x, w_gate, w_up, b_gate, b_up, out)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, bg, bu = _gated_ff_args(x, w_gate, w_up, b_gate, b_up, act, (BF16, F16), x.dtype)
     h, h2, ldh = _out(out, "out", x.dtype, M, F, x)
@@ -954,7 +955,8 @@ def gated_ff_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w
     """Gradient of K13: (dx, dw_gate, dw_up, db_gate, db_up) from dh (of h) and the projections that `gated_ff(keep=True)`
     returned; the biases' are None unless `bias`.  One type throughout, bf16 or f16; the gradients of the projections are
     rounded to it between the two steps (in f16 they overflow past 65504), sums are held in 32 bits and taken in a fixed
-    order.  dw_gate and dw_up are the halves of one [2 * inner, K] tensor (the gradient of a fused weight)."""
+    order.  dw_gate and dw_up are the halves of one [2 * inner, K] tensor (the gradient of a fused weight).  M, inner and K up to
+    2^20 - 64 each."""
     _dev(dh, x, w_gate, w_up, gate, up)
     dt = (x.dtype,)
     x2, M, K, ldx, g2, F, ldg, u2, ldu, _, _ = _gated_ff_args(x, w_gate, w_up, None, None, act, (BF16, F16), x.dtype)
