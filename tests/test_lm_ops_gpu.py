@@ -911,3 +911,84 @@ def test_gated_ff_in_8_bits_of_products_that_cancel(M):
     h = ops.gated_ff_fp8(x.to(ops.FP8), one[:M], wg.to(ops.FP8), one[:F], wu.to(ops.FP8), one[:F])
     within(h, h64, h64.abs() * u_of(BF) + 64 * (cut + eu) * (1 + u_of(BF)))
     assert cut < u.min()                                   # (the sum of what is small is seen)
+
+
+# ---- at the limits that the entry points document ------------------------------------------------------------------
+
+def test_norm_of_the_most_columns():
+    cols = 1 << 28
+    g = torch.Generator(DEV).manual_seed(1)
+    x, w = torch.randn(1, cols, generator=g, device=DEV).to(BF), torch.randn(cols, generator=g, device=DEV).to(BF)
+    y, h = ops.rmsnorm_residual(x, w, x)
+    r = 1 / math.sqrt(sum((2 * v.double()).square().sum().item() for v in x[0].split(1 << 24)) / cols + EPS)
+    for at in (slice(0, 1000), slice(cols // 2 - 500, cols // 2 + 500), slice(cols - 1000, cols)):
+        assert torch.equal(h[0, at], 2 * x[0, at])
+        # 2^20 squares a lane: their sum's roundings stay far below the output's
+        assert rel_l2(y[0, at], 2 * x[0, at].double() * r * w[at].double()) < 1.0 * u_of(BF)
+    q, s, _ = ops.rmsnorm_residual_fp8(x, w, x)
+    for at in (slice(0, 1000), slice(cols - 1000, cols)):
+        # half a step of e4m3, 2^-4 of a value (2^-10 of the scale below the normal range)
+        want = 2 * x[0, at].double() * r * w[at].double()
+        within(q[0, at].double() * s.double(), want, want.abs() * (2.0 ** -4 + 1e-3) + s.double() * 2.0 ** -10)
+    dx, dw = ops.rmsnorm_residual_backward(y, h, w)
+    dot = sum((a.double() * b.double() * c.double()).sum().item() for a, b, c in zip(y[0].split(1 << 24), w.split(1 << 24), h[0].split(1 << 24)))
+    for at in (slice(0, 1000), slice(cols - 1000, cols)):
+        hs, ys, ws = h[0, at].double(), y[0, at].double(), w[at].double()
+        assert rel_l2(dw[at], ys * hs * r) < 1.0 * u_of(BF)
+        assert rel_l2(dx[0, at], r * (ys * ws - hs * r * r * dot / cols)) < 1.0 * u_of(BF)
+
+
+@pytest.mark.parametrize("M,F,K", [(1, 1 << 27, 8), (3, 40, (1 << 24) + 24), (49, 40, (1 << 20) - 64), (49, 24, (1 << 20) - 65), ((1 << 20) + 1, 16, 64)])
+def test_gated_ff_at_its_limits(M, F, K):
+    g = torch.Generator(DEV).manual_seed(1)
+    x, wg, wu = (torch.randn(r, K, generator=g, device=DEV).mul_(K ** -0.5 if i else 1).to(BF) for i, r in enumerate((M, F, F)))
+    h = ops.gated_ff(x, wg, wu)
+    rows, cols = sorted({0, M // 2, M - 1}), torch.tensor(sorted({0, min(F - 1, 7), F // 2, F - 2, F - 1}), device=DEV)
+    h64, gt, up, eg, eu = ff64(x[rows], wg[cols], wu[cols], None, None, ops.ACT_SILU)
+    # (K roundings of a sum's terms grow as their root: 2^-24 sqrt(K) of the sum of |terms| is a hundred times what is met)
+    few = min(1.0, 16 * K ** -0.5)
+    within(h[rows][:, cols], h64, ff_tol(h64, gt, up, eg * few, eu * few, ops.ACT_SILU, BF))
+
+
+@pytest.mark.parametrize("M,F,K", [((1 << 20) - 64, 16, 64), ((1 << 20) - 65, 24, 40), (3, (1 << 20) - 64, 64), (3, 24, (1 << 20) - 64)])
+def test_gated_ff_gradient_at_its_limits(M, F, K):
+    gen = torch.Generator(DEV).manual_seed(1)
+    dh, g, u = (torch.randn(M, F, generator=gen, device=DEV).to(BF) for _ in range(3))
+    x = torch.randn(M, K, generator=gen, device=DEV).to(BF)
+    wg, wu = (torch.randn(F, K, generator=gen, device=DEV).to(BF) for _ in range(2))
+    dx, dwg, dwu, dbg, dbu = ops.gated_ff_backward(dh, x, wg, wu, g, u, bias=True)
+    dg, du = ff_grad64(dh, x[:1], wg[:1], wu[:1], g, u, ops.ACT_SILU)[:2]
+    rows = torch.cat([torch.arange(0, min(M, 200)), torch.arange(max(0, M - 200), M)]).unique().to(DEV)
+    cols = torch.cat([torch.arange(0, min(K, 200)), torch.arange(max(0, K - 200), K)]).unique().to(DEV)
+    want = dg[rows] @ wg[:, cols].double() + du[rows] @ wu[:, cols].double()
+    assert rel_l2(dx[rows][:, cols], want) < 1.0 * u_of(BF)
+    inner = torch.cat([torch.arange(0, min(F, 200)), torch.arange(max(0, F - 200), F)]).unique().to(DEV)
+    for d, o, b in ((dg, dwg, dbg), (du, dwu, dbu)):
+        assert rel_l2(o[inner][:, cols], d[:, inner].t() @ x[:, cols].double()) < 1.0 * u_of(BF)
+        assert rel_l2(b, d.sum(0)) < 1.0 * u_of(BF)
+
+
+def test_gated_ff_of_rows_far_apart_and_of_rows_that_overlap():
+    M, F, K = 64, 24, 64
+    x, w = randn(M, K, seed=1, dtype=BF), randn(2 * F, K, seed=2, scale=K ** -0.5, dtype=BF)
+    far = torch.zeros(2 * F, (1 << 22) + 16, dtype=BF, device=DEV)           # a stride that the wide reads' offsets do not hold
+    far[:, :K] = w
+    wv = far[:, :K]
+    near = randn(M * 8 + K, seed=3, dtype=BF).as_strided((M, K), (8, 1))
+    dh, g, u = (randn(M, F, seed=i, dtype=BF) for i in (4, 5, 6))
+    for rows in (3, M):
+        for a in (x[:rows], near[:rows]):
+            h64, gt, up, eg, eu = ff64(a, w[:F], w[F:], None, None, ops.ACT_SILU)
+            within(ops.gated_ff(a, wv[:F], wv[F:]), h64, ff_tol(h64, gt, up, eg, eu, ops.ACT_SILU, BF))
+            t = (dh[:rows], a, wv[:F], wv[F:], g[:rows], u[:rows])
+            check_ff_grad(ops.gated_ff_backward(*t, bias=True), *t, ops.ACT_SILU, BF)
+
+
+@pytest.mark.parametrize("cols", [64, 1537, 4096, 20000, 70000])
+def test_norm_to_8_bits_with_the_sum_in_place(cols):
+    x, r, w = randn(9, cols, seed=1, dtype=BF), randn(9, cols, seed=2, dtype=BF), randn(cols, seed=3, dtype=BF)
+    q, s, h = ops.rmsnorm_residual_fp8(x, w, r)
+    for into in (0, 1):
+        a = [x.clone(), r.clone()]
+        q2, s2, h2 = ops.rmsnorm_residual_fp8(a[0], w, a[1], resid_out=a[into])
+        assert h2 is a[into] and torch.equal(h2, h) and torch.equal(s2, s) and torch.equal(q2.view(torch.uint8), q.view(torch.uint8))
